@@ -220,9 +220,10 @@ def run_sparse(s):
     c = s["case"]
     if own:
         from heterocache_b200 import ops
-        return ops.flash_decode_sparse(s["q"], s["kp"], s["vp"], s["table"], s["lens"], s["bounds"],
-                                       num_kv_heads=c["kv"], n_select=c["select"], sink=c["sink"], recent=c["recent"],
-                                       workspace=_workspace(s), err=s["err"])
+        out, blocks, counts = ops.flash_decode_sparse(s["q"], s["kp"], s["vp"], s["table"], s["lens"], s["bounds"],
+                                                      num_kv_heads=c["kv"], n_select=c["select"], sink=c["sink"],
+                                                      recent=c["recent"], workspace=_workspace(s), err=s["err"])
+        return {"out": out, "blocks": blocks, "counts": counts}
     return plain_sparse(s)
 
 
