@@ -52,6 +52,24 @@ SIGNATURES = {
     "hc_flash_decode_noalloc": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p,
                                         c_void_p, c_int, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p,
                                         c_void_p]),
+    "hc_rope_append": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64,
+                       c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                       c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                       c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                       c_void_p, c_void_p, c_void_p, c_void_p]),
+    "hc_block_bounds": (c_int, [c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                       c_int, c_void_p, c_void_p, c_void_p]),
+    "hc_block_select_workspace_size": (c_size_t, [c_int, c_int, c_int]),
+    "hc_block_select": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int,
+                       c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_size_t,
+                       c_void_p, c_void_p]),
+    "hc_flash_decode_blocks": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p,
+                       c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p,
+                       c_void_p, c_size_t, c_void_p, c_void_p]),
+    "hc_flash_decode_shared_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "hc_flash_decode_shared": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p,
+                       c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                       c_int64, c_int64, c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "hc_drift_check_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "hc_drift_check": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_double,
                                c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,

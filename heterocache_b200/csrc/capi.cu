@@ -817,4 +817,215 @@ int hc_profile_overlap(const uint32_t* a, int64_t a_stride, int na, const uint32
                                                 (cudaStream_t)stream));
 }
 
+
+int hc_rope_append(int dtype, int trig_dtype, int bsz, int num_heads, int num_kv_heads, int n_tokens, int head_dim,
+                   const void* q, int64_t qsb, int64_t qsh, int64_t qst, const void* k, int64_t ksb, int64_t ksh,
+                   int64_t kst, const void* v, int64_t vsb, int64_t vsh, int64_t vst, const void* cos, int64_t csb,
+                   int64_t cst, const void* sin, int64_t ssb, int64_t sst, void* q_out, int64_t osb, int64_t osh,
+                   int64_t ost, const int32_t* counts, void* k_pool, void* v_pool, int n_pool_blocks,
+                   int32_t* block_table, int max_blocks, const int32_t* heads_len, int32_t* heads_len_out,
+                   const int32_t* free_blocks, int n_free, int32_t* free_ptr, void* bounds, int32_t* counter,
+                   int32_t* err_flag, void* stream) {
+  if (!valid_dtype(dtype) || (trig_dtype != dtype && trig_dtype != HC_F32)) return HC_ERR_DTYPE;
+  if (head_dim != HC_HEAD_DIM || bsz <= 0 || num_heads < 0 || num_kv_heads <= 0 || n_tokens < 0 || max_blocks <= 0 ||
+      n_pool_blocks < 0 || n_free < 0)
+    return HC_ERR_INVALID;
+  if (!heads_len || !heads_len_out || !block_table || !free_ptr || !counter || (n_free > 0 && !free_blocks))
+    return HC_ERR_INVALID;
+  if ((int64_t)max_blocks * HC_PAGE_SIZE > 0x7fffffffLL || (int64_t)bsz * num_kv_heads > 0x7fffffffLL)
+    return HC_ERR_UNSUPPORTED;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(cos) || !aligned16(sin) || !aligned16(q_out) ||
+      !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(bounds))
+    return HC_ERR_INVALID;
+  // a dimension of extent 1 is never stepped over, whatever its stride
+  if (n_tokens == 1) qst = kst = vst = ost = cst = sst = 0;
+  if (bsz == 1) qsb = ksb = vsb = osb = csb = ssb = 0;
+  if (num_heads == 1) qsh = osh = 0;
+  if (num_kv_heads == 1) ksh = vsh = 0;
+  const int64_t st[] = {qsb, qsh, qst, ksb, ksh, kst, vsb, vsh, vst, osb, osh, ost};
+  for (int64_t x : st)
+    if (!stride_ok(dtype, x)) return HC_ERR_INVALID;
+  const int64_t tr[] = {csb, cst, ssb, sst};
+  for (int64_t x : tr)
+    if (!stride_ok(trig_dtype, x)) return HC_ERR_INVALID;
+  hc::RAParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.qsb = qsb;
+  p.qsh = qsh;
+  p.qst = qst;
+  p.ksb = ksb;
+  p.ksh = ksh;
+  p.kst = kst;
+  p.vsb = vsb;
+  p.vsh = vsh;
+  p.vst = vst;
+  p.cos = cos;
+  p.sin = sin;
+  p.csb = csb;
+  p.cst = cst;
+  p.ssb = ssb;
+  p.sst = sst;
+  p.trig_f32 = trig_dtype == HC_F32;
+  p.q_out = q_out;
+  p.osb = osb;
+  p.osh = osh;
+  p.ost = ost;
+  p.kp = k_pool;
+  p.vp = v_pool;
+  p.n_blocks = n_pool_blocks;
+  p.bt = block_table;
+  p.max_blocks = max_blocks;
+  p.heads_len = heads_len;
+  p.heads_len_out = heads_len_out;
+  p.counts = counts;
+  p.free_blocks = free_blocks;
+  p.n_free = n_free;
+  p.free_ptr = free_ptr;
+  p.bounds = bounds;
+  p.done = reinterpret_cast<unsigned int*>(counter);
+  p.B = bsz;
+  p.H = num_heads;
+  p.KV = num_kv_heads;
+  p.T = n_tokens;
+  p.err = err_flag;
+  return note_cuda(hc::rope_append_dispatch(dtype, p, (cudaStream_t)stream));
+}
+
+int hc_block_bounds(int dtype, int rows_total, int head_dim, const void* k_pool, int n_pool_blocks,
+                    const int32_t* block_table, int max_blocks, const int32_t* heads_len, const int32_t* rows,
+                    int n_rows, int last, void* bounds, int32_t* err_flag, void* stream) {
+  if (!valid_dtype(dtype)) return HC_ERR_DTYPE;
+  if (head_dim != HC_HEAD_DIM || rows_total <= 0 || max_blocks <= 0 || n_pool_blocks < 0 || last < 0 || n_rows < 0)
+    return HC_ERR_INVALID;
+  if (!aligned16(k_pool) || !aligned16(bounds) || !block_table || !heads_len) return HC_ERR_INVALID;
+  if ((int64_t)max_blocks * HC_PAGE_SIZE > 0x7fffffffLL) return HC_ERR_UNSUPPORTED;
+  if (rows && n_rows == 0) return HC_OK;
+  hc::BBParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.kp = k_pool;
+  p.n_blocks = n_pool_blocks;
+  p.bt = block_table;
+  p.max_blocks = max_blocks;
+  p.heads_len = heads_len;
+  p.R = rows_total;
+  p.rows = rows;
+  p.n_rows = n_rows;
+  p.last = last;
+  p.bounds = bounds;
+  p.err = err_flag;
+  return note_cuda(hc::block_bounds_dispatch(dtype, p, (cudaStream_t)stream));
+}
+
+size_t hc_block_select_workspace_size(int bsz, int num_kv_heads, int max_blocks) {
+  if (bsz <= 0 || num_kv_heads <= 0 || max_blocks <= 0) return 0;
+  return hc::block_select_ws_bytes(bsz * num_kv_heads, max_blocks);
+}
+
+int hc_block_select(int dtype, int bsz, int num_kv_heads, int groups, int head_dim, const void* q, int64_t qsb,
+                    int64_t qsh, const void* bounds, int n_pool_blocks, const int32_t* block_table, int max_blocks,
+                    const int32_t* heads_len, int n_select, int sink, int recent, int32_t* blocks, int32_t* counts,
+                    void* workspace, size_t workspace_bytes, int32_t* err_flag, void* stream) {
+  if (!valid_dtype(dtype)) return HC_ERR_DTYPE;
+  if (head_dim != HC_HEAD_DIM || bsz <= 0 || num_kv_heads <= 0 || groups <= 0 || max_blocks <= 0 || n_pool_blocks < 0)
+    return HC_ERR_INVALID;
+  if (n_select < 1 || sink < 0 || recent < 0 || (int64_t)sink + recent > n_select) return HC_ERR_INVALID;
+  if (!aligned16(q) || !aligned16(bounds) || !block_table || !heads_len || !blocks || !counts) return HC_ERR_INVALID;
+  if (!stride_ok(dtype, qsb) || !stride_ok(dtype, qsh)) return HC_ERR_INVALID;
+  hc::BSParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.qsb = qsb;
+  p.qsh = qsh;
+  p.bounds = bounds;
+  p.n_blocks = n_pool_blocks;
+  p.bt = block_table;
+  p.max_blocks = max_blocks;
+  p.heads_len = heads_len;
+  p.R = bsz * num_kv_heads;
+  p.KV = num_kv_heads;
+  p.G = groups;
+  p.n_select = n_select;
+  p.sink = sink;
+  p.recent = recent;
+  p.blocks = blocks;
+  p.counts = counts;
+  p.err = err_flag;
+  return note_cuda(hc::block_select_dispatch(dtype, p, workspace, workspace_bytes, (cudaStream_t)stream));
+}
+
+int hc_flash_decode_blocks(int dtype, int bsz, int num_kv_heads, int groups, int head_dim, const void* q, int64_t qsb,
+                           int64_t qsh, const void* k_pool, const void* v_pool, int n_pool_blocks,
+                           const int32_t* block_table, int max_blocks, const int32_t* heads_len,
+                           const int32_t* blocks, const int32_t* counts, int n_select, float scale, void* out,
+                           void* workspace, size_t workspace_bytes, int32_t* err_flag, void* stream) {
+  hc::FDParams p;
+  const int rc = with_new_params(p, dtype, bsz, num_kv_heads, groups, head_dim, q, qsb, qsh, k_pool, v_pool,
+                                 n_pool_blocks, block_table, max_blocks, heads_len, nullptr, nullptr, 0, 0, 0, 0,
+                                 scale, out, nullptr, err_flag, false);
+  if (rc != HC_OK) return rc;
+  if (!blocks || !counts || n_select < 1) return HC_ERR_INVALID;
+  if ((int64_t)max_blocks * HC_PAGE_SIZE > 0x7fffffffLL ||
+      (int64_t)bsz * num_kv_heads * n_select * HC_SPARSE_BLOCK > 0x7fffffffLL)
+    return HC_ERR_UNSUPPORTED;
+  p.blocks = blocks;
+  p.counts = counts;
+  p.n_select = n_select;
+  return note_cuda(
+      hc::flash_decode_dispatch(dtype, p, workspace, workspace_bytes, (cudaStream_t)stream, hc::FD_BLOCKS));
+}
+
+size_t hc_flash_decode_shared_workspace_size(int dtype, int bsz, int num_kv_heads, int groups, int head_dim) {
+  (void)head_dim;
+  if (!valid_dtype(dtype) || bsz <= 0 || num_kv_heads <= 0 || groups <= 0) return 0;
+  return hc::shared_prefix_ws_bytes(dtype, bsz, num_kv_heads, groups) +
+         hc::flash_decode_ws_bytes(bsz * num_kv_heads, groups);
+}
+
+int hc_flash_decode_shared(int dtype, int bsz, int num_kv_heads, int groups, int head_dim, const void* q, int64_t qsb,
+                           int64_t qsh, const void* k_pool, const void* v_pool, int n_pool_blocks,
+                           const int32_t* block_table, int max_blocks, const int32_t* heads_len,
+                           const int32_t* shared_len, const void* k_new, const void* v_new, int64_t kn_sb,
+                           int64_t kn_sh, int64_t vn_sb, int64_t vn_sh, float scale, void* out, void* workspace,
+                           size_t workspace_bytes, int32_t* err_flag, void* stream) {
+  hc::FDParams p;
+  const int rc = with_new_params(p, dtype, bsz, num_kv_heads, groups, head_dim, q, qsb, qsh, k_pool, v_pool,
+                                 n_pool_blocks, block_table, max_blocks, heads_len, k_new, v_new, kn_sb, kn_sh,
+                                 vn_sb, vn_sh, scale, out, nullptr, err_flag, false);
+  if (rc != HC_OK) return rc;
+  if (!shared_len) return HC_ERR_INVALID;
+  if (groups > hc::kGMax || (int64_t)bsz * num_kv_heads > hc::kMaxRowsFD ||
+      (int64_t)max_blocks * HC_PAGE_SIZE > 0x7fffffffLL)
+    return HC_ERR_UNSUPPORTED;
+  hc::SPParams s;
+  std::memset(&s, 0, sizeof(s));
+  s.q = q;
+  s.qsb = qsb;
+  s.qsh = qsh;
+  s.kp = k_pool;
+  s.vp = v_pool;
+  s.bt = block_table;
+  s.max_blocks = max_blocks;
+  s.n_blocks = n_pool_blocks;
+  s.shared_len = shared_len;
+  s.B = bsz;
+  s.KV = num_kv_heads;
+  s.G = groups;
+  s.scale_log2 = p.scale_log2;
+  s.err = err_flag;
+  // the workspace: the prefix part's partials, then those of the tails
+  const size_t front = hc::shared_prefix_ws_bytes(dtype, bsz, num_kv_heads, groups);
+  if (!workspace || !aligned16(workspace) ||
+      workspace_bytes < front + hc::flash_decode_ws_bytes(bsz * num_kv_heads, groups))
+    return HC_ERR_WORKSPACE;
+  const int rp = note_cuda(hc::shared_prefix_dispatch(dtype, s, workspace, front, (cudaStream_t)stream));
+  if (rp != HC_OK) return rp;
+  p.shared_len = shared_len;
+  p.pre = s.plan;
+  return note_cuda(hc::flash_decode_dispatch(dtype, p, static_cast<unsigned char*>(workspace) + front,
+                                             workspace_bytes - front, (cudaStream_t)stream, hc::FD_TAIL));
+}
+
 }  // extern "C"

@@ -33,12 +33,53 @@ namespace hc {
 
 
 
+// FD_TAIL: the first token of row r that the launch reads, before (base: a
+// multiple of the padding) and after (lo) rounding down.
+__device__ __forceinline__ int fd_tail_lo(const FDParams& p, int r) {
+  return min(max(p.shared_len[r % p.KV], 0), p.max_blocks * kPage);
+}
+__device__ __forceinline__ int fd_tail_base(const FDParams& p, int r) { return fd_tail_lo(p, r) & ~(p.gran - 1); }
+
+// The length of row r in the launch's token space.
+template <int kMode>
+__device__ __forceinline__ int fd_row_len(const FDParams& p, int r) {
+  if constexpr (kMode == FD_BLOCKS) return min(max(p.counts[r], 0), p.n_select) * HC_SPARSE_BLOCK;
+  const int len = p.heads_len[r];
+  if constexpr (kMode == FD_TAIL) return len > fd_tail_lo(p, r) ? len - fd_tail_base(p, r) : 0;
+  return len;
+}
+
+// Where token t (a multiple of 16) of row r's part of the launch's token
+// space is in the row, and how many tokens from it on (of `n`) are read, the
+// first `first` of them masked; valid = 0: none (a listed block that is out
+// of the row).
+template <int kMode>
+__device__ __forceinline__ int fd_locate(const FDParams& p, int r, int t, int n, int& valid, int& first) {
+  first = 0;
+  if constexpr (kMode == FD_BLOCKS) {
+    const int blk = p.blocks[(int64_t)r * p.n_select + t / HC_SPARSE_BLOCK];
+    if (blk < 0 || blk >= p.max_blocks * (kPage / HC_SPARSE_BLOCK)) {
+      valid = 0;
+      return 0;
+    }
+    const int pos = blk * HC_SPARSE_BLOCK + (t & (HC_SPARSE_BLOCK - 1));
+    valid = min(n, p.heads_len[r] - pos);
+    return pos;
+  } else {
+    const int base = kMode == FD_TAIL ? fd_tail_base(p, r) : 0;
+    if constexpr (kMode == FD_TAIL) first = max(0, fd_tail_lo(p, r) - base - t);
+    valid = min(n, p.heads_len[r] - base - t);
+    return base + t;
+  }
+}
+
 // Padded prefix of row lengths into s_start[0..R]; returns total.
+template <int kMode>
 __device__ __forceinline__ int row_prefix(const FDParams& p, int* s_start, int* s_warp, int* s_len = nullptr) {
   int carry = 0;
   for (int c0 = 0; c0 < p.R; c0 += blockDim.x) {
     int r = c0 + threadIdx.x;
-    int len = r < p.R ? p.heads_len[r] : 0;
+    int len = r < p.R ? fd_row_len<kMode>(p, r) : 0;
     len = len < 0 ? 0 : len;
     if (s_len && r < p.R) s_len[r] = len;
     int l16 = (len + p.gran - 1) / p.gran * p.gran;
@@ -177,9 +218,9 @@ __device__ __forceinline__ void fd_group_compute(const FDParams& p, WarpState<T>
 // fp32: lanes over dims, warp all-reduce per (query head, token).
 __device__ __forceinline__ void fd_group_f32(const FDParams& p, WarpState<float>& st, const float (&qf)[kGMax][4],
                                              const float* kbase, const float* vbase, int valid, float (&mrow)[kGMax],
-                                             float (&lrow)[kGMax]) {
+                                             float (&lrow)[kGMax], int first = 0) {
   const int lane = threadIdx.x & 31;
-  for (int i = 0; i < 16; ++i) {
+  for (int i = first; i < 16; ++i) {
     if (i >= valid) break;
     const float4 k4 = *reinterpret_cast<const float4*>(kbase + i * kD + 4 * lane);
     const float4 v4 = *reinterpret_cast<const float4*>(vbase + i * kD + 4 * lane);
@@ -203,7 +244,7 @@ __device__ __forceinline__ void fd_group_f32(const FDParams& p, WarpState<float>
   }
 }
 
-template <typename T>
+template <typename T, int kMode>
 __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   int* s_start = reinterpret_cast<int*>(smem_raw);
@@ -217,7 +258,7 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
   const int gid = lane >> 2, tig = lane & 3;
   pdl_wait();  // as in the TMA kernel
   pdl_trigger();
-  const int total = row_prefix(p, s_start, s_warp);
+  const int total = row_prefix<kMode>(p, s_start, s_warp);
   const int span = span_of(total, gridDim.x, p.gran);
   const int beg = blockIdx.x * span;
   if (beg >= total) return;
@@ -232,7 +273,6 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
     const int rs = s_start[r], re = s_start[r + 1];
     if (re <= beg || re == rs) continue;
     const int a = max(rs, beg) - rs, bnd = min(re, end) - rs;
-    const int len = p.heads_len[r];
     const int b = r / p.KV, h = r % p.KV;
     const T* qrow0 = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G) * p.qsh;
 
@@ -257,12 +297,19 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
         }
       }
       for (int t16 = a + warp * 16; t16 < bnd; t16 += kFWarps * 16) {
-        const int page = t16 >> 8;
+        int valid, first;
+        const int t = fd_locate<kMode>(p, r, t16, 16, valid, first);
+        if (kMode == FD_BLOCKS && valid <= 0) {
+          // a listed block's last groups may lie behind the row's end, its first may not
+          if ((t16 & (HC_SPARSE_BLOCK - 1)) == 0) set_err(p.err, HC_ERR_RANGE);
+          continue;
+        }
+        const int page = t >> 8;
         int blk = page < p.max_blocks ? p.bt[(int64_t)r * p.max_blocks + page] : -1;
         if (blk < 0 || blk >= p.n_blocks) { set_err(p.err, HC_ERR_RANGE); continue; }
-        const int64_t off = ((int64_t)blk * kPage + (t16 & (kPage - 1))) * kD;
+        const int64_t off = ((int64_t)blk * kPage + (t & (kPage - 1))) * kD;
         fd_group_f32(p, st, qf, reinterpret_cast<const float*>(p.kp) + off,
-                     reinterpret_cast<const float*>(p.vp) + off, min(16, len - t16), mrow, lrow);
+                     reinterpret_cast<const float*>(p.vp) + off, valid, mrow, lrow, first);
       }
       if (lane == 0) {
         for (int g = 0; g < kGMax; ++g) { s_m[warp][g] = mrow[g]; s_l[warp][g] = lrow[g]; }
@@ -279,6 +326,7 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
           qa[2 * s + u][1] = w.y;
         }
       for (int t16 = a + warp * 16; t16 < bnd; t16 += kFWarps * 16) {
+        const int len = p.heads_len[r];
         const int page = t16 >> 8;
         int blk = page < p.max_blocks ? p.bt[(int64_t)r * p.max_blocks + page] : -1;
         if (blk < 0 || blk >= p.n_blocks) { set_err(p.err, HC_ERR_RANGE); continue; }
@@ -377,10 +425,12 @@ struct TcState {
 };
 
 // One 16-token group; kst/vst = shared addresses of the stage's key/value
-// boxes, tok0 = first tile row of the group, valid = tokens to use.
-template <typename T>
+// boxes, tok0 = first tile row of the group, valid = tokens to use (kMode
+// other than FD_ALL: those from `first` on, and the values of the others are
+// taken as zeros, whatever the page holds there).
+template <typename T, int kMode>
 __device__ __forceinline__ void fd_group_tc(const FDParams& p, TcState& st, const uint32_t (&qa)[8][2],
-                                            uint32_t kst, uint32_t vst, int tok0, int valid) {
+                                            uint32_t kst, uint32_t vst, int tok0, int valid, int first = 0) {
   const int lane = threadIdx.x & 31;
   const int tig = lane & 3;
   const int mi = lane >> 3, j = lane & 7;
@@ -400,7 +450,8 @@ __device__ __forceinline__ void fd_group_tc(const FDParams& p, TcState& st, cons
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int t = 8 * nt + 2 * tig + e;
-      const float x = t < valid ? acc[nt][e] * p.scale_log2 : -INFINITY;
+      const bool in = t < valid && (kMode != FD_TAIL || t >= first);
+      const float x = in ? acc[nt][e] * p.scale_log2 : -INFINITY;
       sv[nt * 2 + e] = x;
       mx = fmaxf(mx, x);
     }
@@ -433,10 +484,23 @@ __device__ __forceinline__ void fd_group_tc(const FDParams& p, TcState& st, cons
   const uint32_t b0 = pack2<T>(sv[0], sv[1]);
   const uint32_t b1 = pack2<T>(sv[2], sv[3]);
   const int vrow = tok0 + 8 * (mi >> 1) + j;
+  // this lane's values are tokens 2tig, 2tig+1 (a[0], a[1]) and 8 + 2tig, .. (a[2], a[3])
+  uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+  if (kMode != FD_ALL && (valid < 16 || first > 0)) {
+    auto in = [&](int t) -> uint32_t { return t < valid && t >= first ? 0xffffu : 0u; };
+    keep0 = in(2 * tig) | in(2 * tig + 1) << 16;
+    keep1 = in(8 + 2 * tig) | in(9 + 2 * tig) << 16;
+  }
 #pragma unroll
   for (int mt = 0; mt < 8; ++mt) {
     uint32_t a[4];
     ldsm_x4_t(a, swz(vst, vrow, 2 * mt + (mi & 1)));
+    if (kMode != FD_ALL) {
+      a[0] &= keep0;
+      a[1] &= keep0;
+      a[2] &= keep1;
+      a[3] &= keep1;
+    }
     // a[0]: dims 16mt..+7 x tokens 0-7, a[1]: dims +8.. x tokens 0-7,
     // a[2]: dims 16mt.. x tokens 8-15, a[3]: dims +8.. x tokens 8-15
     mma16816<T>(st.ot[mt], a[0], a[1], a[2], a[3], b0, b1);
@@ -452,7 +516,7 @@ __host__ __device__ constexpr size_t fd_tma_smem(int R, int G) {
          (size_t)kTConsumers * G * kD * sizeof(float);
 }
 
-template <typename T>
+template <typename T, int kMode>
 __global__ void __launch_bounds__(kTThreads, 2)
     flash_decode_tma_kernel(FDParams p, const __grid_constant__ CUtensorMap tmk,
                             const __grid_constant__ CUtensorMap tmv) {
@@ -467,7 +531,9 @@ __global__ void __launch_bounds__(kTThreads, 2)
   float* s_ob = reinterpret_cast<float*>(s_len + fd_round4(p.R));
   auto s_o = [&](int w, int g) { return s_ob + ((size_t)w * p.G + g) * kD; };
   __shared__ __align__(8) uint64_t full_bar[kTStages], empty_bar[kTStages];
-  __shared__ int s_tile_ok[kTStages];  // page id of the stage's tile was valid
+  // FD_ALL: the page id of the stage's tile was valid; else the tile's valid
+  // tokens (0: skipped) and the masked ones before them
+  __shared__ int s_tile_ok[kTStages], s_tile_first[kTStages];
   __shared__ int s_warp[32];
   __shared__ float s_m[kTConsumers][kGMax], s_l[kTConsumers][kGMax];
 
@@ -478,7 +544,7 @@ __global__ void __launch_bounds__(kTThreads, 2)
   // lengths before its own wait and waits for this grid's partials
   pdl_wait();
   pdl_trigger();
-  const int total = row_prefix(p, s_start, s_warp, s_len);
+  const int total = row_prefix<kMode>(p, s_start, s_warp, s_len);
   const int span = span_of(total, gridDim.x, kTTile);
   const int beg = blockIdx.x * span;
   if (threadIdx.x == 0) {
@@ -513,16 +579,18 @@ __global__ void __launch_bounds__(kTThreads, 2)
         }
         const int tok = beg + i * kTTile;
         while (s_start[r + 1] <= tok) ++r;
-        const int t = tok - s_start[r];
+        int t = tok - s_start[r], valid = 1, first = 0;
+        if constexpr (kMode != FD_ALL) t = fd_locate<kMode>(p, r, t, kTTile, valid, first);
         const int page = t >> 8;
-        const int blk = page < p.max_blocks ? p.bt[(int64_t)r * p.max_blocks + page] : -1;
+        const int blk = page < p.max_blocks && valid > 0 ? p.bt[(int64_t)r * p.max_blocks + page] : -1;
         if (blk < 0 || blk >= p.n_blocks) {  // consumers skip this tile
           set_err(p.err, HC_ERR_RANGE);
           s_tile_ok[s] = 0;
           mbar_arrive(&full_bar[s]);  // release: orders the flag before the consumers' wait
           continue;
         }
-        s_tile_ok[s] = 1;
+        s_tile_ok[s] = valid;
+        if constexpr (kMode != FD_ALL) s_tile_first[s] = first;
         const int y = blk * kPage + (t & (kPage - 1));
         unsigned char* dst = stages + (size_t)s * kStageBytes;
         mbar_arrive_expect_tx(&full_bar[s], kStageBytes);
@@ -611,10 +679,16 @@ __global__ void __launch_bounds__(kTThreads, 2)
     }
     if (!dead) {
       const int t = tok - s_start[r];
-      const int valid = s_tile_ok[s] ? min(16, s_len[r] - t - 16 * warp) : 0;
-      if (valid > 0) {
+      int valid, first = 0;
+      if constexpr (kMode == FD_ALL) {
+        valid = s_tile_ok[s] ? min(16, s_len[r] - t - 16 * warp) : 0;
+      } else {
+        valid = min(16, s_tile_ok[s] - 16 * warp);
+        if (valid > 0) first = max(0, s_tile_first[s] - 16 * warp);
+      }
+      if (valid > first) {
         const uint32_t kst = smem_u32(stages + (size_t)s * kStageBytes);
-        fd_group_tc<T>(p, st, qa, kst, kst + 2 * kTBox, 16 * warp, valid);
+        fd_group_tc<T, kMode>(p, st, qa, kst, kst + 2 * kTBox, 16 * warp, valid, first);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_bar[s]);
@@ -631,11 +705,60 @@ __global__ void __launch_bounds__(kTThreads, 2)
 // to 131072 tokens at the decode grid's spans); the partial's (m, l) comes
 // with it (a broadcast load); then the block maximum, each thread rescales
 // its own partials, and the 32 groups' sums are added in shared memory.
+// FD_TAIL: where the prefix part's partials of one (row, query head) are.
+struct PrefixRow {
+  int n;          // partials
+  int per;        // partials a piece (a CTA's part of the segment) has for the row
+  int64_t first;  // the first partial's index
+  int64_t step;   // from one piece's to the next, and between a piece's streams
+  int64_t stream;
+  __device__ __forceinline__ size_t at(int c) const { return (size_t)(first + (c / per) * step + (c % per) * stream); }
+};
+
+// s: two ints of shared memory.  Called by all threads.
+__device__ __forceinline__ PrefixRow prefix_row(const FDParams& p, int r, int g, int* s) {
+  const int h = r % p.KV, i = (r / p.KV) * p.G + g;
+  const PrefixPlan& pl = p.pre;
+  auto tiles_of = [&](int k) { return (fd_tail_lo(p, k) + pl.gran - 1) / pl.gran; };  // k < KV: row k is head k's
+  if (threadIdx.x < 32) {
+    int before = 0, all = 0;
+    for (int k = threadIdx.x; k < p.KV; k += 32) {
+      const int t = tiles_of(k);
+      all += t;
+      before += k < h ? t : 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    if (threadIdx.x == 0) {
+      s[0] = before;
+      s[1] = all;
+    }
+  }
+  __syncthreads();
+  const int tiles = tiles_of(h);
+  const int ng = i / pl.rows_per, ii = i % pl.rows_per;
+  const int span = (s[1] * pl.n_groups + pl.n_ctas - 1) / pl.n_ctas;
+  PrefixRow out = {0, 1, 0, 0, 0};
+  if (tiles == 0) return out;
+  const int beg = s[0] * pl.n_groups + ng * tiles;
+  const int c0 = beg / span, c1 = (beg + tiles - 1) / span;
+  const int set = pl.streams * pl.stream_rows;
+  out.per = set > pl.rows_per ? pl.streams : 1;  // the streams split the tokens, or the rows
+  out.n = (c1 - c0 + 1) * out.per;
+  out.first = (int64_t)(c0 + h * pl.n_groups + ng) * set + ii;
+  out.step = set;
+  out.stream = pl.stream_rows;
+  return out;
+}
+
 constexpr int kCThreads = 256;
 constexpr int kCSlices = 4;
 constexpr int kCSliceDims = kD / kCSlices;  // 32
 
-template <typename T>
+template <typename T, int kMode>
 __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, int nctas) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   int* s_start = reinterpret_cast<int*>(smem_raw);
@@ -646,7 +769,7 @@ __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, in
   __shared__ float s_red[NW], s_redl[NW];
   __shared__ float s_mrun;  // running maximum over the rounds of 128 partials
   __shared__ float4 s_acc[NG][kCSliceDims / 4];
-  const int total = row_prefix(p, s_start, s_warp);
+  const int total = row_prefix<kMode>(p, s_start, s_warp);
   const int span = span_of(total, nctas, p.gran);
   const int rg = blockIdx.x / kCSlices, sl = blockIdx.x % kCSlices;
   const int r = rg / p.G, g = rg % p.G;
@@ -695,12 +818,17 @@ __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, in
           reinterpret_cast<const T*>(p.v_new)[b * p.vn_sb + (int64_t)h * p.vn_sh + d0 + threadIdx.x]);
     __syncthreads();
   }
-  if (re == rs || span == 0) {  // no pages: the new token alone, or nothing
+  const int c0 = span ? rs / span : 0, n_own = re == rs || span == 0 ? 0 : (re - 1) / span - c0 + 1;
+  const size_t slot0 = (size_t)(c0 + r);
+  // FD_TAIL: the prefix part's partials of this row's query head follow
+  __shared__ int s_pre[2];
+  PrefixRow pre = {0, 1, 0, 0, 0};
+  if constexpr (kMode == FD_TAIL) pre = prefix_row(p, r, g, s_pre);
+  const int n = n_own + pre.n;
+  if (n == 0) {  // no pages: the new token alone, or nothing
     if (threadIdx.x < kCSliceDims) store(threadIdx.x, has_new ? v_new_d : 0.f);
     return;
   }
-  const int c0 = rs / span, n = (re - 1) / span - c0 + 1;
-  const size_t slot0 = (size_t)(c0 + r);
   // the partials are written by the decode kernel launched just before
   pdl_wait();
   pdl_trigger();  // the next kernel may get resident; it waits for this grid
@@ -713,9 +841,16 @@ __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, in
     for (int u = 0; u < DEPTH; ++u) {
       const int c = cb0 + (warp * GPW + sub) + u * NG;
       const bool ok = c < n;
-      ml[u] = ok ? p.part_ml[(slot0 + c) * p.G + g] : make_float2(-INFINITY, 0.f);
-      o[u] = ok ? *reinterpret_cast<const float4*>(p.part_o + ((slot0 + c) * p.G + g) * kD + d0 + 4 * q4)
-                : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float* po = p.part_o;
+      const float2* pml = p.part_ml;
+      size_t at = (slot0 + c) * p.G + g;
+      if (kMode == FD_TAIL && c >= n_own) {
+        po = p.pre.part_o;
+        pml = p.pre.part_ml;
+        at = pre.at(c - n_own);
+      }
+      ml[u] = ok ? pml[at] : make_float2(-INFINITY, 0.f);
+      o[u] = ok ? *reinterpret_cast<const float4*>(po + at * kD + d0 + 4 * q4) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float mw = -INFINITY;
 #pragma unroll
@@ -880,9 +1015,9 @@ static int fd_grid(int dtype) {
   int occ = 0;
   size_t dsm = (kMaxRowsFD + 1) * sizeof(int);
   switch (dtype) {
-    case HC_F32: cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, flash_decode_kernel<float>, kFThreads, dsm); break;
-    case HC_BF16: cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, flash_decode_kernel<__nv_bfloat16>, kFThreads, dsm); break;
-    default: cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, flash_decode_kernel<__half>, kFThreads, dsm); break;
+    case HC_F32: cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, flash_decode_kernel<float, FD_ALL>, kFThreads, dsm); break;
+    case HC_BF16: cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, flash_decode_kernel<__nv_bfloat16, FD_ALL>, kFThreads, dsm); break;
+    default: cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, flash_decode_kernel<__half, FD_ALL>, kFThreads, dsm); break;
   }
   if (occ <= 0) occ = 1;
   std::lock_guard<std::mutex> g(host_lock());
@@ -895,7 +1030,7 @@ size_t flash_decode_ws_bytes(int R, int G) {
   return slots * G * kD * sizeof(float) + slots * G * sizeof(float2) + 256;
 }
 
-template <typename T>
+template <typename T, int kMode>
 static int fd_combine(FDParams& p, int grid, cudaStream_t st) {
   // launched as a programmatic dependent of the decode kernel: its CTAs may
   // start early and wait (griddepcontrol.wait) for the partials
@@ -910,7 +1045,7 @@ static int fd_combine(FDParams& p, int grid, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, flash_combine_kernel<T>, p, grid) != cudaSuccess) return HC_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, flash_combine_kernel<T, kMode>, p, grid) != cudaSuccess) return HC_ERR_CUDA;
   return HC_OK;
 }
 
@@ -934,6 +1069,7 @@ static cudaError_t pdl_launch(void (*kern)(KArgs...), int grid, int threads, siz
 }
 
 // fp32 pools: the global-load kernel, rows padded to 16.
+template <int kMode>
 static int fd_launch_f32(FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st) {
   const int grid = fd_grid(HC_F32);
   const size_t slots = (size_t)grid + p.R;
@@ -941,20 +1077,21 @@ static int fd_launch_f32(FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = reinterpret_cast<float2*>(reinterpret_cast<unsigned char*>(ws) + slots * p.G * kD * sizeof(float));
   p.gran = 16;
-  if (pdl_launch(flash_decode_kernel<float>, grid, kFThreads, (size_t)(p.R + 1) * sizeof(int), st, p) != cudaSuccess)
+  if (pdl_launch(flash_decode_kernel<float, kMode>, grid, kFThreads, (size_t)(p.R + 1) * sizeof(int), st, p) !=
+      cudaSuccess)
     return HC_ERR_CUDA;
-  return fd_combine<float>(p, grid, st);
+  return fd_combine<float, kMode>(p, grid, st);
 }
 
 // Co-resident CTAs of the 16-bit TMA decode kernel for `dsm` bytes of dynamic
 // shared memory on the current device, 0 if it cannot run.  The kernel's
 // shared-memory limit is raised and the occupancy queried once per device and
 // size; later calls make no CUDA call but cudaGetDevice.
-template <typename T>
+template <typename T, int kMode>
 static int fd_tma_grid(size_t dsm) {
   static bool attr_set[kMaxDevices];
   static ShapeCache<8> grids;
-  auto kern = flash_decode_tma_kernel<T>;
+  auto kern = flash_decode_tma_kernel<T, kMode>;
   const int dev = current_device();
   if (dev < 0) return 0;
   std::lock_guard<std::mutex> g(host_lock());
@@ -978,16 +1115,16 @@ static int fd_tma_grid(size_t dsm) {
 }
 
 // 16-bit pools: the TMA pipeline, rows padded to 64.
-template <typename T>
+template <typename T, int kMode>
 static int fd_launch_tma(FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st) {
-  auto kern = flash_decode_tma_kernel<T>;
+  auto kern = flash_decode_tma_kernel<T, kMode>;
   const int dtype = std::is_same<T, __nv_bfloat16>::value ? HC_BF16 : HC_F16;
   CUtensorMap tmk, tmv;
   const long long rows = (long long)p.n_blocks * kPage;
   if (!pool_tensor_map(&tmk, p.kp, rows, dtype, kTTile)) return HC_ERR_CUDA;
   if (!pool_tensor_map(&tmv, p.vp, rows, dtype, kTTile)) return HC_ERR_CUDA;
   const size_t dsm = fd_tma_smem(p.R, p.G);
-  const int grid = fd_tma_grid<T>(dsm);
+  const int grid = fd_tma_grid<T, kMode>(dsm);
   if (grid <= 0) return HC_ERR_UNSUPPORTED;
   const size_t slots = (size_t)grid + p.R;
   if (!ws || ws_bytes < slots * p.G * kD * sizeof(float) + slots * p.G * sizeof(float2)) return HC_ERR_WORKSPACE;
@@ -995,7 +1132,7 @@ static int fd_launch_tma(FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st
   p.part_ml = reinterpret_cast<float2*>(reinterpret_cast<unsigned char*>(ws) + slots * p.G * kD * sizeof(float));
   p.gran = kTTile;
   if (pdl_launch(kern, grid, kTThreads, dsm, st, p, tmk, tmv) != cudaSuccess) return HC_ERR_CUDA;
-  return fd_combine<T>(p, grid, st);
+  return fd_combine<T, kMode>(p, grid, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -1014,8 +1151,8 @@ static size_t flash_decode_scratch_need(int dtype, int R, int G) {
   int grid = 0;
   switch (dtype) {
     case HC_F32: grid = fd_grid(HC_F32); break;
-    case HC_BF16: grid = fd_tma_grid<__nv_bfloat16>(fd_tma_smem(R, G)); break;
-    case HC_F16: grid = fd_tma_grid<__half>(fd_tma_smem(R, G)); break;
+    case HC_BF16: grid = fd_tma_grid<__nv_bfloat16, FD_ALL>(fd_tma_smem(R, G)); break;
+    case HC_F16: grid = fd_tma_grid<__half, FD_ALL>(fd_tma_smem(R, G)); break;
     default: return 0;
   }
   if (grid <= 0) return 0;
@@ -1047,15 +1184,24 @@ int flash_decode_noalloc_dispatch(int dtype, FDParams& p, cudaStream_t st, size_
   return flash_decode_dispatch(dtype, p, scratch, HC_NOALLOC_SCRATCH_BYTES, st);
 }
 
-int flash_decode_dispatch(int dtype, FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st) {
+template <int kMode>
+static int fd_launch(int dtype, FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st) {
+  switch (dtype) {
+    case HC_F32: return fd_launch_f32<kMode>(p, ws, ws_bytes, st);
+    case HC_BF16: return fd_launch_tma<__nv_bfloat16, kMode>(p, ws, ws_bytes, st);
+    case HC_F16: return fd_launch_tma<__half, kMode>(p, ws, ws_bytes, st);
+    default: return HC_ERR_DTYPE;
+  }
+}
+
+int flash_decode_dispatch(int dtype, FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st, int mode) {
   p.wait_ns = wait_limit_ns(kMbarTimeoutNs);
   if (p.R <= 0 || p.R > kMaxRowsFD) return HC_ERR_UNSUPPORTED;
   if (p.G <= 0 || p.G > kGMax) return HC_ERR_UNSUPPORTED;
-  switch (dtype) {
-    case HC_F32: return fd_launch_f32(p, ws, ws_bytes, st);
-    case HC_BF16: return fd_launch_tma<__nv_bfloat16>(p, ws, ws_bytes, st);
-    case HC_F16: return fd_launch_tma<__half>(p, ws, ws_bytes, st);
-    default: return HC_ERR_DTYPE;
+  switch (mode) {
+    case FD_ALL: return fd_launch<FD_ALL>(dtype, p, ws, ws_bytes, st);
+    case FD_TAIL: return fd_launch<FD_TAIL>(dtype, p, ws, ws_bytes, st);
+    default: return fd_launch<FD_BLOCKS>(dtype, p, ws, ws_bytes, st);
   }
 }
 

@@ -124,6 +124,36 @@ int drift_batch_per_launch(int dtype, int n_jobs, int L, int Rq, int S, int want
 int score_dispatch(int dtype, ScoreParams& p, void* ws, size_t ws_bytes, cudaStream_t st,
                    const DriftBatch* batch = nullptr);
 
+// ---- shared-prefix decode: the prefix part (shared_attn.cu)
+// Query rows i = b * G + g of KV head h are cut into groups of `rows_per`;
+// segment h * NG + group holds tiles of `gran` tokens of the head's shared
+// tokens; all segments' tiles are laid end to end and cut into equal spans,
+// one a CTA.  A CTA's partials of a segment are at slot (cta + segment):
+// `streams` sets of `stream_rows` rows each (max in the log2 domain, sum,
+// 128 outputs).
+struct PrefixPlan {
+  int n_ctas, n_groups, rows_per, gran, streams, stream_rows;
+  float* part_o;
+  float2* part_ml;
+};
+struct SPParams {
+  const void* q;
+  int64_t qsb, qsh;
+  const void *kp, *vp;
+  const int32_t* bt;  // rows 0 .. KV - 1: the first sequence's pages
+  int max_blocks, n_blocks;
+  const int32_t* shared_len;  // [KV]
+  int B, KV, G;
+  float scale_log2;
+  PrefixPlan plan;
+  int32_t* err;
+  uint64_t wait_ns;
+};
+// The plan of a launch, and the bytes of its partials (part_o and part_ml
+// are taken from the front of a workspace of at least that size).
+size_t shared_prefix_ws_bytes(int dtype, int B, int KV, int G);
+int shared_prefix_dispatch(int dtype, SPParams& p, void* ws, size_t ws_bytes, cudaStream_t st);
+
 // ---- paged flash-decode (decode_attn.cu)
 constexpr int kMaxPeers = 8;  // GPUs of one node a head-sharded output is mirrored to
 constexpr int kFThreads = 128;
@@ -161,7 +191,18 @@ struct FDParams {
   void* mirror[kMaxPeers];
   int32_t* err;
   uint64_t wait_ns;  // mbarrier wait limit (set at dispatch)
+  // which tokens of a row the launch attends over (FD_* below)
+  const int32_t* shared_len;  // FD_TAIL: [KV] tokens of the shared prefix
+  PrefixPlan pre;             // FD_TAIL: the prefix part's partials, for the combine
+  const int32_t* blocks;      // FD_BLOCKS: [R, n_select] ascending 64-token blocks
+  const int32_t* counts;      // FD_BLOCKS: [R] how many
+  int n_select;
 };
+
+// FD_ALL: a row's heads_len tokens.  FD_TAIL: those from shared_len[head] on
+// (the tokens before them come from the prefix part).  FD_BLOCKS: those of
+// the row's listed blocks.
+enum { FD_ALL = 0, FD_TAIL = 1, FD_BLOCKS = 2 };
 
 size_t flash_decode_ws_bytes(int R, int G);
 // One step barrier across the GPUs of a head-sharded cache: the caller's
@@ -172,7 +213,7 @@ int peer_put_dispatch(int n_seg, const int32_t* const* srcs, const int64_t* seg_
                       int32_t* const* dsts, cudaStream_t st);
 int peer_barrier_dispatch(int rank, int world, int32_t* const* peer_flags, int32_t* counter, int32_t* err,
                           cudaStream_t st);
-int flash_decode_dispatch(int dtype, FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st);
+int flash_decode_dispatch(int dtype, FDParams& p, void* ws, size_t ws_bytes, cudaStream_t st, int mode = FD_ALL);
 int flash_decode_noalloc_dispatch(int dtype, FDParams& p, cudaStream_t st, size_t* need_out);
 
 // ---- causal prefill attention (prefill_attn.cu)
@@ -189,6 +230,67 @@ struct PAParams {
 int prefill_attn_dispatch(int dtype, PAParams& p, const void* q, int64_t qsb, int64_t qsh, int64_t qst,
                           const void* k, int64_t ksb, int64_t ksh, int64_t kst, const void* v, int64_t vsb,
                           int64_t vsh, int64_t vst, cudaStream_t st);
+
+// ---- append with rotation (rope_append.cu)
+struct RAParams {
+  const void *q, *k, *v;
+  int64_t qsb, qsh, qst, ksb, ksh, kst, vsb, vsh, vst;
+  const void *cos, *sin;  // [B or one, T, D], in the cache type or (trig_f32) fp32
+  int64_t csb, cst, ssb, sst;
+  int trig_f32;
+  void* q_out;
+  int64_t osb, osh, ost;
+  void *kp, *vp;
+  int n_blocks;
+  int32_t* bt;
+  int max_blocks;
+  const int32_t* heads_len;
+  int32_t* heads_len_out;  // may be heads_len
+  const int32_t* counts;   // tokens of each sequence, or null: T
+  const int32_t* free_blocks;
+  int n_free;
+  int32_t* free_ptr;
+  void* bounds;  // block bounds to keep up to date, or null
+  unsigned int* done;  // zero before and after a launch
+  int B, H, KV, T;
+  int units, kv_ctas;  // 64-token blocks a row may touch; key/value CTAs (set at launch)
+  int32_t* err;
+};
+int rope_append_dispatch(int dtype, RAParams& p, cudaStream_t st);
+
+// ---- block bounds and block selection (block_sparse.cu)
+struct BBParams {
+  const void* kp;
+  int n_blocks;
+  const int32_t* bt;
+  int max_blocks;
+  const int32_t* heads_len;
+  int R;
+  const int32_t* rows;  // n_rows row indices, or null: all R
+  int n_rows;
+  int last;  // only the blocks that hold a row's last `last` tokens (0: all)
+  void* bounds;
+  int32_t* err;
+};
+int block_bounds_dispatch(int dtype, const BBParams& p, cudaStream_t st);
+
+struct BSParams {
+  const void* q;
+  int64_t qsb, qsh;
+  const void* bounds;
+  int n_blocks;
+  const int32_t* bt;
+  int max_blocks;
+  const int32_t* heads_len;
+  int R, KV, G;
+  int n_select, sink, recent;
+  int32_t* blocks;  // [R, n_select], ascending, -1 behind the count
+  int32_t* counts;  // [R]
+  double* scores;   // workspace [R, 4 * max_blocks]
+  int32_t* err;
+};
+size_t block_select_ws_bytes(int R, int max_blocks);
+int block_select_dispatch(int dtype, BSParams& p, void* ws, size_t ws_bytes, cudaStream_t st);
 
 // ---- page copies (kv_copy.cu)
 int prefill_keep_dispatch(int dtype, int bsz, int KV, int L, const int32_t* keep, int n_keep, const void* k,

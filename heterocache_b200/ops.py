@@ -7,7 +7,8 @@ the reference's tensors: q ``[bsz, H, L, D]``, k/v ``[bsz, KV, L, D]``, pools
 """
 from __future__ import annotations
 
-from typing import Optional
+import contextlib
+from typing import Optional, Tuple
 
 import torch
 
@@ -17,6 +18,7 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 POOLING = {"avgpool": 0, "maxpool": 1}
 HEAD_DIM = 128
 PAGE = 256
+BLOCK = 64  # tokens of a block of the sparse decode attention (HC_SPARSE_BLOCK)
 
 # Kernel launches issued through this module (flash-decode is two kernels).
 LAUNCHES = [0]
@@ -64,6 +66,8 @@ class Workspace:
     def __init__(self, device):
         self.device = torch.device(device)
         self.buf = torch.zeros(0, dtype=torch.uint8, device=self.device)
+        # rope_append's counter: apart from buf, where other calls leave their scratch
+        self.counter = torch.zeros(4, dtype=torch.int32, device=self.device)
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf.numel() < nbytes:
@@ -72,6 +76,7 @@ class Workspace:
 
     def reset(self) -> None:
         self.buf.zero_()
+        self.counter.zero_()
 
 
 def set_wait_limits(limit_ns: int = 0, inject_stall: bool = False) -> None:
@@ -337,6 +342,255 @@ def flash_decode(q, k_pool, v_pool, block_table, heads_len, *, num_kv_heads, out
     check("hc_flash_decode", rc)
     LAUNCHES[0] += 2
     return out
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _same_device(*ts: Optional[torch.Tensor]):
+    """All tensors on one CUDA device; a context in which that device is the
+    current one (the library launches on the current device)."""
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"heterocache_b200: tensors on different devices ({dev} and {t.device})")
+    if dev.type != "cuda":
+        raise ValueError("heterocache_b200: tensors must live on a CUDA device")
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _pool(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    _need(t.dim() == 4 and t.shape[1:] == (PAGE, 1, HEAD_DIM) and t.is_contiguous(),
+          f"{name} must be a contiguous [n_blocks, {PAGE}, 1, {HEAD_DIM}] pool")
+    _need(t.dtype == like.dtype, f"{name} must have the dtype of the other operands")
+
+
+def _cache_rows(block_table, heads_len, rows: int) -> None:
+    _i32(block_table, "block_table"), _i32(heads_len, "heads_len")
+    _need(block_table.dim() == 2 and block_table.shape[0] >= rows and heads_len.numel() >= rows,
+          "block_table and heads_len need a row per (batch row, KV head)")
+
+
+def _bounds(bounds, n_blocks: int, like: torch.Tensor) -> None:
+    _need(bounds.dtype == like.dtype and bounds.is_contiguous()
+          and tuple(bounds.shape) == (n_blocks, PAGE // BLOCK, 2, HEAD_DIM),
+          f"bounds must be a contiguous [n_blocks, {PAGE // BLOCK}, 2, {HEAD_DIM}] tensor in the pool dtype")
+
+
+def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_blocks, free_ptr, err, *,
+                workspace: Workspace, counts=None, q_out=None, heads_len_out=None, bounds=None) -> torch.Tensor:
+    """Rotate the new tokens' queries and keys and append keys and values to
+    the paged cache, in one launch (hc_rope_append): q [bsz, H, T, D], k, v
+    [bsz, KV, T, D] not yet rotated (strided, contiguous last dim), cos, sin
+    [bsz or 1, T, D] in the cache dtype or fp32, as a model's rotary embedding
+    gives them.  Returns the rotated queries, in ``q_out`` (default: a new
+    contiguous tensor; may be ``q``).
+
+    Token t of row r = b * KV + h goes to position heads_len[r] + t; unmapped
+    pages come from the free list in (row, page) order.  ``counts`` [bsz]
+    int32 says how many of the T tokens each sequence has (a padded batch);
+    the rest is left as it was.  The new lengths go to ``heads_len_out``
+    (default: heads_len).  ``bounds`` [n_blocks, 4, 2, D]: block bounds of
+    ``flash_decode_sparse`` to keep up to date.  A bad length, count or page,
+    or a free list that is too short, is reported in ``err`` and leaves the
+    cache as it was.  ``workspace`` holds a counter; calls that may overlap
+    need a workspace each."""
+    _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    _same_shape(k, v)
+    _need(q.dim() == 4 and k.dim() == 4, "q, k, v need [bsz, heads, tokens, D]")
+    bsz, H, T, D = q.shape
+    KV = k.shape[1]
+    dt = dtype_code(q)
+    _need(k.shape[0] == bsz and k.shape[2] == T and k.dtype == q.dtype, "q, k and v must share batch, tokens and dtype")
+    _need(bsz > 0 and KV > 0 and H > 0, "q, k and v need at least one sequence and one head")
+    _pool(k_pool, "k_pool", q), _pool(v_pool, "v_pool", q)
+    _need(k_pool.shape == v_pool.shape, "k_pool and v_pool must have the same shape")
+    _cache_rows(block_table, heads_len, bsz * KV)
+    _i32(free_blocks, "free_blocks"), _i32(free_ptr, "free_ptr"), _i32(err, "err")
+    _need(free_ptr.numel() >= 1 and err.numel() >= 1, "free_ptr and err need an entry")
+    trig = []
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        _rows(t, name)
+        t = t.unsqueeze(0) if t.dim() == 2 else t
+        _need(t.dim() == 3 and t.shape[0] in (1, bsz) and t.shape[1] == T, f"{name} needs [bsz or 1, tokens, D]")
+        _need(t.dtype in (q.dtype, torch.float32) and t.dtype == cos.dtype,
+              "cos and sin must share a dtype: the queries', or float32")
+        trig += [0 if t.shape[0] == 1 else t.stride(0), t.stride(1)]
+    if counts is not None:
+        _i32(counts, "counts")
+        _need(counts.numel() >= bsz, "counts needs an entry per sequence")
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _rows(q_out, "q_out")
+        _need(q_out.shape == q.shape and q_out.dtype == q.dtype, "q_out must have the queries' shape and dtype")
+    if heads_len_out is None:
+        heads_len_out = heads_len
+    else:
+        _i32(heads_len_out, "heads_len_out")
+        _need(heads_len_out.numel() >= bsz * KV, "heads_len_out needs a row per (batch row, KV head)")
+    if bounds is not None:
+        _bounds(bounds, k_pool.shape[0], q)
+    counter = workspace.counter
+    (qb, qh, qt, _), (kb, kh, kt, _), (vb, vh, vt, _), (ob, oh, ot, _) = (q.stride(), k.stride(), v.stride(),
+                                                                          q_out.stride())
+    with _same_device(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, heads_len_out, free_blocks, free_ptr,
+                      err, counts, q_out, bounds, counter):
+        rc = lib().hc_rope_append(dt, DTYPES[cos.dtype], bsz, H, KV, T, D, q.data_ptr(), qb, qh, qt, k.data_ptr(), kb,
+                                  kh, kt, v.data_ptr(), vb, vh, vt, cos.data_ptr(), trig[0], trig[1], sin.data_ptr(),
+                                  trig[2], trig[3], q_out.data_ptr(), ob, oh, ot, _ptr(counts), k_pool.data_ptr(),
+                                  v_pool.data_ptr(), k_pool.shape[0], block_table.data_ptr(), block_table.shape[1],
+                                  heads_len.data_ptr(), heads_len_out.data_ptr(), free_blocks.data_ptr(),
+                                  free_blocks.numel(), free_ptr.data_ptr(), _ptr(bounds), counter.data_ptr(),
+                                  err.data_ptr(), _stream(q))
+    check("hc_rope_append", rc)
+    LAUNCHES[0] += 1
+    return q_out
+
+
+def _decode_operands(q, k_pool, v_pool, block_table, heads_len, num_kv_heads, out):
+    """Checks that the decode attentions below share; returns (out, bsz, G)."""
+    _rows(q, "q")
+    _need(q.dim() == 4 and q.shape[2] == 1, "decode attention takes one query position, [bsz, H, 1, D]")
+    bsz, H = q.shape[0], q.shape[1]
+    _need(bsz > 0 and num_kv_heads > 0 and H > 0 and H % num_kv_heads == 0,
+          f"the {H} query heads do not split evenly over {num_kv_heads} KV heads")
+    _pool(k_pool, "k_pool", q), _pool(v_pool, "v_pool", q)
+    _need(k_pool.shape == v_pool.shape, "k_pool and v_pool must have the same shape")
+    _cache_rows(block_table, heads_len, bsz * num_kv_heads)
+    if out is None:
+        out = torch.empty(bsz, H, HEAD_DIM, dtype=q.dtype, device=q.device)
+    else:
+        _need(out.is_contiguous() and out.numel() == bsz * H * HEAD_DIM and out.dtype == q.dtype,
+              "out must be a contiguous [bsz, H, D] buffer in the query dtype")
+    return out, bsz, H // num_kv_heads
+
+
+def flash_decode_shared(q, k_pool, v_pool, block_table, heads_len, shared_len, *, num_kv_heads, out=None,
+                        scale: float = 0.0, workspace: Workspace, err, k_new=None, v_new=None) -> torch.Tensor:
+    """Decode attention of a batch that shares a prefix (hc_flash_decode_shared):
+    q [bsz, H, 1, D] -> out [bsz, H, D].  The first ``shared_len[h]`` tokens of
+    KV head h ([KV] int32) are every sequence's; they are read once, through
+    the first sequence's rows of the page table.  Each row's own tokens follow
+    from position shared_len[h] to heads_len[r] - 1; with k_new / v_new [bsz,
+    KV, 1, D] one more token a row, not in the pages."""
+    out, bsz, G = _decode_operands(q, k_pool, v_pool, block_table, heads_len, num_kv_heads, out)
+    _i32(shared_len, "shared_len"), _i32(err, "err")
+    _need(shared_len.numel() >= num_kv_heads, "shared_len needs an entry per KV head")
+    _need((k_new is None) == (v_new is None), "k_new and v_new come together")
+    kn = vn = (0, 0)
+    if k_new is not None:
+        _rows(k_new, "k_new"), _rows(v_new, "v_new")
+        _same_shape(k_new, v_new)
+        _need(tuple(k_new.shape) == (bsz, num_kv_heads, 1, HEAD_DIM) and k_new.dtype == q.dtype,
+              "k_new/v_new must be [bsz, KV, 1, D] in the query dtype")
+        kn, vn = k_new.stride(), v_new.stride()
+    dt = dtype_code(q)
+    with _same_device(q, k_pool, v_pool, block_table, heads_len, shared_len, out, err, k_new, v_new):
+        ws = workspace.get(lib().hc_flash_decode_shared_workspace_size(dt, bsz, num_kv_heads, G, HEAD_DIM))
+        rc = lib().hc_flash_decode_shared(dt, bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), q.stride(0), q.stride(1),
+                                          k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0],
+                                          block_table.data_ptr(), block_table.shape[1], heads_len.data_ptr(),
+                                          shared_len.data_ptr(), _ptr(k_new), _ptr(v_new), kn[0], kn[1], vn[0], vn[1],
+                                          float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr(),
+                                          _stream(q))
+    check("hc_flash_decode_shared", rc)
+    LAUNCHES[0] += 3
+    return out
+
+
+def block_bounds(k_pool, block_table, heads_len, bounds, err, *, rows=None, last: int = 0) -> torch.Tensor:
+    """Least and greatest key per channel of each 64-token block (hc_block_bounds)
+    into ``bounds`` [n_blocks, 4, 2, D]: of every row, or of those listed in
+    ``rows`` (int32); of all its blocks, or of those that hold its last
+    ``last`` tokens."""
+    _pool(k_pool, "k_pool", k_pool)
+    n = block_table.shape[0]
+    _cache_rows(block_table, heads_len, n)
+    _bounds(bounds, k_pool.shape[0], k_pool)
+    _i32(err, "err")
+    _need(last >= 0, "last must not be negative")
+    if rows is not None:
+        _i32(rows, "rows")
+    with _same_device(k_pool, block_table, heads_len, bounds, err, rows):
+        rc = lib().hc_block_bounds(dtype_code(k_pool), n, HEAD_DIM, k_pool.data_ptr(), k_pool.shape[0],
+                                   block_table.data_ptr(), block_table.shape[1], heads_len.data_ptr(), _ptr(rows),
+                                   0 if rows is None else rows.numel(), int(last), bounds.data_ptr(), err.data_ptr(),
+                                   _stream(k_pool))
+    check("hc_block_bounds", rc)
+    LAUNCHES[0] += 1
+    return bounds
+
+
+def block_select(q, bounds, block_table, heads_len, *, num_kv_heads, n_select: int, sink: int = 1, recent: int = 1,
+                 workspace: Workspace, err, blocks=None, counts=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The blocks that ``flash_decode_sparse`` attends to (hc_block_select): of
+    each row the first ``sink``, the last ``recent`` and those of the highest
+    bound on their scores, n_select in all.  Returns (blocks [rows, n_select]
+    int32 ascending, -1 behind; counts [rows] int32)."""
+    _rows(q, "q")
+    _need(q.dim() == 4 and q.shape[2] == 1, "block_select takes one query position, [bsz, H, 1, D]")
+    bsz, H = q.shape[0], q.shape[1]
+    _need(bsz > 0 and num_kv_heads > 0 and H > 0 and H % num_kv_heads == 0,
+          f"the {H} query heads do not split evenly over {num_kv_heads} KV heads")
+    _need(n_select >= 1 and sink >= 0 and recent >= 0 and sink + recent <= n_select,
+          "sink + recent blocks must not be more than n_select, which must be at least 1")
+    R = bsz * num_kv_heads
+    _cache_rows(block_table, heads_len, R)
+    _bounds(bounds, bounds.shape[0], q)
+    _i32(err, "err")
+    if blocks is None:
+        blocks = torch.empty(R, n_select, dtype=torch.int32, device=q.device)
+    if counts is None:
+        counts = torch.empty(R, dtype=torch.int32, device=q.device)
+    _i32(blocks, "blocks"), _i32(counts, "counts")
+    _need(tuple(blocks.shape) == (R, n_select) and counts.numel() >= R,
+          "blocks needs [rows, n_select] and counts an entry per row")
+    G = H // num_kv_heads
+    with _same_device(q, bounds, block_table, heads_len, err, blocks, counts):
+        ws = workspace.get(lib().hc_block_select_workspace_size(bsz, num_kv_heads, block_table.shape[1]))
+        rc = lib().hc_block_select(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), q.stride(0),
+                                   q.stride(1), bounds.data_ptr(), bounds.shape[0], block_table.data_ptr(),
+                                   block_table.shape[1], heads_len.data_ptr(), int(n_select), int(sink), int(recent),
+                                   blocks.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr(),
+                                   _stream(q))
+    check("hc_block_select", rc)
+    LAUNCHES[0] += 2
+    return blocks, counts
+
+
+def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, counts, *, num_kv_heads, out=None,
+                        scale: float = 0.0, workspace: Workspace, err) -> torch.Tensor:
+    """Decode attention over each row's listed 64-token blocks alone
+    (hc_flash_decode_blocks): blocks [rows, n] int32 ascending, the first
+    counts[row] of them used."""
+    out, bsz, G = _decode_operands(q, k_pool, v_pool, block_table, heads_len, num_kv_heads, out)
+    R = bsz * num_kv_heads
+    _i32(blocks, "blocks"), _i32(counts, "counts"), _i32(err, "err")
+    _need(blocks.dim() == 2 and blocks.shape[0] >= R and blocks.shape[1] >= 1 and counts.numel() >= R,
+          "blocks needs [rows, n] and counts an entry per row")
+    with _same_device(q, k_pool, v_pool, block_table, heads_len, blocks, counts, out, err):
+        ws = workspace.get(lib().hc_flash_decode_workspace_size(bsz, num_kv_heads, G, HEAD_DIM))
+        rc = lib().hc_flash_decode_blocks(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), q.stride(0),
+                                          q.stride(1), k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0],
+                                          block_table.data_ptr(), block_table.shape[1], heads_len.data_ptr(),
+                                          blocks.data_ptr(), counts.data_ptr(), blocks.shape[1], float(scale),
+                                          out.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr(), _stream(q))
+    check("hc_flash_decode_blocks", rc)
+    LAUNCHES[0] += 2
+    return out
+
+
+def flash_decode_sparse(q, k_pool, v_pool, block_table, heads_len, bounds, *, num_kv_heads, n_select: int,
+                        sink: int = 1, recent: int = 1, out=None, scale: float = 0.0, workspace: Workspace, err,
+                        blocks=None, counts=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Block-sparse decode attention: ``block_select``, then ``flash_decode_blocks``
+    over what it lists.  Returns (out [bsz, H, D], blocks, counts)."""
+    blocks, counts = block_select(q, bounds, block_table, heads_len, num_kv_heads=num_kv_heads, n_select=n_select,
+                                  sink=sink, recent=recent, workspace=workspace, err=err, blocks=blocks, counts=counts)
+    out = flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, counts, num_kv_heads=num_kv_heads,
+                              out=out, scale=scale, workspace=workspace, err=err)
+    return out, blocks, counts
 
 
 def drift_check(qbuf, k_pool, block_table, *, num_kv_heads, groups, steps, seq_len, pooling, kernel_size, topk,

@@ -239,6 +239,104 @@ int hc_flash_decode_with_new(int dtype, int bsz, int num_kv_heads, int groups, i
                              void* workspace, size_t workspace_bytes, int32_t* err_flag, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Append with rotation: n_tokens new tokens a sequence, queries and keys not
+ * yet rotated.  No counterpart in the reference, whose attention rotates
+ * first (apply_rotary_pos_emb, heterocache/llama_model.py:318-319) and appends
+ * one rotated token a step (hc_decode_append); this does both in one launch,
+ * for decode steps, drafted tokens and chunks of a prompt.
+ *   With x = (x1, x2) the halves of a row and cos, sin split alike:
+ *     y1 = x1 cos1 - x2 sin1,  y2 = x2 cos2 + x1 sin2   (fp32, rounded once)
+ *   q [bsz, num_heads, n_tokens, D], k and v [bsz, num_kv_heads, n_tokens, D],
+ *   q_out as q, all strided (batch, head, token); q_out may be q itself.
+ *   cos, sin [bsz, n_tokens, D] strided (batch, token; a batch stride of 0
+ *   shares them), of type trig_dtype: the cache's or HC_F32.
+ *   counts: device int32[bsz], how many of the n_tokens each sequence has (a
+ *   padded batch; the tokens behind are neither appended nor rotated, their
+ *   rows of q_out stay as they were), or NULL: all.
+ * Token t of row r = b*KV + h goes to position heads_len[r] + t.  Pages of the
+ * row's table that are -1 are taken from free_blocks, from *free_ptr on, in
+ * (row, page) order; mapped ones are written in place.  heads_len_out[r] =
+ * heads_len[r] + count: heads_len itself, or another array (drafted tokens
+ * that may be dropped: the pages stay mapped to the row).
+ *   bounds: block bounds to keep up to date (see hc_block_bounds), or NULL.
+ *   counter: one int32 of device memory, zero before the first call; a call
+ *   leaves it zero.  Calls that may overlap need one each, and a call that
+ *   was cut off leaves it to be zeroed by the caller.
+ * If a length or count is out of range, a page id is bad (HC_ERR_RANGE) or
+ * the free list too short (HC_ERR_OOM), err_flag says so and pools, tables,
+ * lengths and bounds stay as they were (q_out may have been written).  No
+ * two rows may hold the page that they append to.
+ */
+int hc_rope_append(int dtype, int trig_dtype, int bsz, int num_heads, int num_kv_heads, int n_tokens, int head_dim,
+                   const void* q, int64_t qsb, int64_t qsh, int64_t qst, const void* k, int64_t ksb, int64_t ksh,
+                   int64_t kst, const void* v, int64_t vsb, int64_t vsh, int64_t vst, const void* cos, int64_t csb,
+                   int64_t cst, const void* sin, int64_t ssb, int64_t sst, void* q_out, int64_t osb, int64_t osh,
+                   int64_t ost, const int32_t* counts, void* k_pool, void* v_pool, int n_pool_blocks,
+                   int32_t* block_table, int max_blocks, const int32_t* heads_len, int32_t* heads_len_out,
+                   const int32_t* free_blocks, int n_free, int32_t* free_ptr, void* bounds, int32_t* counter,
+                   int32_t* err_flag, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Block-sparse decode attention.  No counterpart in the reference: its
+ * volatile and pivot heads are attended whole at every step
+ * (heterocache/llama_model.py:370-397); here a step may read, of each row, the
+ * HC_SPARSE_BLOCK-token blocks that a bound on their scores selects.
+ *
+ * hc_block_bounds: bounds [n_pool_blocks, 256 / HC_SPARSE_BLOCK, 2, D] in the
+ * pool's type: per block of a page and per channel the least and the greatest
+ * key of the tokens its row holds (NaN if a key is).  Written for the blocks
+ * of the rows listed in rows (device int32[n_rows] of 0 .. rows_total - 1;
+ * NULL: every row) that hold their last `last` tokens (0: all of them).
+ *
+ * hc_block_select: for each row, n_select of its blocks (all, if it has no
+ * more): the first `sink`, the last `recent`, and of the others those of the
+ * highest score
+ *   max over the row's query heads of sum_d max(q_d lo_d, q_d hi_d),
+ * which no key of the block exceeds; sums in 64 bits, equal scores to the
+ * lowest block, a NaN counts as the highest score.  blocks [rows, n_select]:
+ * ascending, -1 behind the counts[row] listed ones.  q as in hc_flash_decode.
+ *
+ * hc_flash_decode_blocks: hc_flash_decode over the listed blocks of each row
+ * alone (a row with none gives zeros); workspace as hc_flash_decode's.
+ */
+#define HC_SPARSE_BLOCK 64
+int hc_block_bounds(int dtype, int rows_total, int head_dim, const void* k_pool, int n_pool_blocks,
+                    const int32_t* block_table, int max_blocks, const int32_t* heads_len, const int32_t* rows,
+                    int n_rows, int last, void* bounds, int32_t* err_flag, void* stream);
+size_t hc_block_select_workspace_size(int bsz, int num_kv_heads, int max_blocks);
+int hc_block_select(int dtype, int bsz, int num_kv_heads, int groups, int head_dim, const void* q, int64_t qsb,
+                    int64_t qsh, const void* bounds, int n_pool_blocks, const int32_t* block_table, int max_blocks,
+                    const int32_t* heads_len, int n_select, int sink, int recent, int32_t* blocks, int32_t* counts,
+                    void* workspace, size_t workspace_bytes, int32_t* err_flag, void* stream);
+int hc_flash_decode_blocks(int dtype, int bsz, int num_kv_heads, int groups, int head_dim, const void* q, int64_t qsb,
+                           int64_t qsh, const void* k_pool, const void* v_pool, int n_pool_blocks,
+                           const int32_t* block_table, int max_blocks, const int32_t* heads_len,
+                           const int32_t* blocks, const int32_t* counts, int n_select, float scale, void* out,
+                           void* workspace, size_t workspace_bytes, int32_t* err_flag, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Decode attention of a batch that shares a long prefix: continuations of
+ * one prompt.  No counterpart in the reference (batch 1,
+ * heterocache/cache_utils.py:1093).  As hc_flash_decode, but the first
+ * shared_len[h] tokens of KV head h (device int32[num_kv_heads]) are the same
+ * for every sequence: they are read once for the whole batch, through row h
+ * of the page table (the first sequence's); the other sequences' entries for
+ * pages that hold shared tokens only are not read.  Row r = b*KV + h attends
+ * to those tokens and to its own from shared_len[h] to heads_len[r] - 1 (none
+ * if it is not longer).  k_new, v_new: one more token a row, not in the
+ * pages, as in hc_flash_decode_with_new, or both NULL.  Workspace as large as
+ * hc_flash_decode_shared_workspace_size says, 16-byte aligned; it need not be
+ * zero.
+ */
+size_t hc_flash_decode_shared_workspace_size(int dtype, int bsz, int num_kv_heads, int groups, int head_dim);
+int hc_flash_decode_shared(int dtype, int bsz, int num_kv_heads, int groups, int head_dim, const void* q, int64_t qsb,
+                           int64_t qsh, const void* k_pool, const void* v_pool, int n_pool_blocks,
+                           const int32_t* block_table, int max_blocks, const int32_t* heads_len,
+                           const int32_t* shared_len, const void* k_new, const void* v_new, int64_t kn_sb,
+                           int64_t kn_sh, int64_t vn_sb, int64_t vn_sh, float scale, void* out, void* workspace,
+                           size_t workspace_bytes, int32_t* err_flag, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Head-sharded decode: the all-gather of head outputs done by the attention
  * kernels themselves.  Replaces the NCCL all-gather of per-rank head outputs
  * (the head-sharded mode has no reference counterpart: the reference runs
