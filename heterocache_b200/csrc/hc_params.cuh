@@ -147,7 +147,8 @@ struct SPParams {
   float scale_log2;
   PrefixPlan plan;
   int32_t* err;
-  uint64_t wait_ns;
+  uint64_t wait_ns;    // mbarrier wait limit (set at dispatch)
+  unsigned int stall;  // injected stall (tests of the timeout path)
 };
 // The plan of a launch, and the bytes of its partials (part_o and part_ml
 // are taken from the front of a workspace of at least that size).

@@ -8,6 +8,7 @@
 
 #include "hc_host.cuh"
 #include "hc_params.cuh"
+#include "umma.cuh"
 
 namespace hc {
 
@@ -198,18 +199,428 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
   }
 }
 
+// ---------------------------------------------------------------------------
+// Tensor-core form (16-bit types): one CTA per SM, tiles of 128 tokens.
+//   S = Q K^T  (M = 128 query rows on the TMEM lanes, N = 128 tokens)
+//   O += P V   (A = P from tensor memory, B = V as loaded, MN-major)
+// Two streams X = 0, 1, each with its own S (P is written over its first 64
+// columns) and O accumulators, so that the tensor core works on one while
+// the softmax warps work on the other.  With at most 128 query rows a group
+// both streams hold the same rows and take the tiles in turn (X takes tiles
+// X, X + 2, ...): two independent splits of the tokens.  With up to 256 the
+// streams hold 128 rows each and every tile serves both.
+// Warps: 0 key producer, 2 value producer (TMA), 1 MMA issuer, 4-7 and 8-11
+// softmax of stream 0 and 1 (one query row a thread); 3 has no role.  The
+// CTA's span may cover several segments (KV head, row group); between them
+// the softmax warps store the partials and put the next queries into shared
+// memory, while the producers run ahead.
+// Tokens behind the shared ones in the last tile (and a bad page's) are
+// masked, and their values zeroed in shared memory before the MMA, whatever
+// the page holds there.
+// Every wait is bounded; a role whose wait gives up marks the launch failed
+// (HC_ERR_TIMEOUT) and waits no more; copies and MMAs in flight are waited
+// for (bounded) before tensor memory is released.
+constexpr int kTcThreads = 12 * 32;
+constexpr int kTcTile = 128;
+constexpr int kTcBox = 128 * 128;        // bytes: 128 rows x 64 16-bit elements
+constexpr int kTcTileBytes = 2 * kTcBox;
+constexpr int kTcTiles = 7;              // tile buffers: queries, keys, values
+constexpr size_t kTcSmem = 1024 + (size_t)kTcTiles * kTcTileBytes;
+constexpr int kTcK = 3;                  // key stages; values have the rest
+constexpr int kTcValidRing = 8;          // tiles whose valid counts are kept
+constexpr uint32_t kTcColS = 0, kTcColO = 256;
+
+// The same answer for the whole warp (each lane polls for itself).
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit_ns));
+}
+
+// One CTA's part of one segment.
+struct TcPiece {
+  int h, ng, t0, t1;
+};
+// Walks the CTA's pieces in order.
+struct TcWalk {
+  int beg, end, start, h, ng;
+  __device__ __forceinline__ bool next(const SPParams& p, TcPiece& out) {
+    while (h < p.KV) {
+      const int tiles = (sp_len(p, h) + kTcTile - 1) / kTcTile;
+      if (start >= end) return false;
+      const int t0 = max(beg, start) - start, t1 = min(end, start + tiles) - start;
+      out.h = h;
+      out.ng = ng;
+      out.t0 = t0;
+      out.t1 = t1;
+      start += tiles;
+      if (++ng == p.plan.n_groups) {
+        ng = 0;
+        ++h;
+      }
+      if (t0 < t1) return true;
+    }
+    return false;
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    shared_prefix_tc_kernel(const SPParams p, const __grid_constant__ CUtensorMap tmk,
+                            const __grid_constant__ CUtensorMap tmv) {
+  extern __shared__ __align__(16) unsigned char smem_dyn[];
+  unsigned char* sq = smem_dyn + ((1024 - (smem_u32(smem_dyn) & 1023)) & 1023);
+  const bool wide = p.plan.rows_per > 128;  // the streams hold different rows
+  const int nq = wide ? 2 : 1;
+  const int vst = kTcTiles - kTcK - nq;
+  unsigned char* sk = sq + nq * kTcTileBytes;
+  unsigned char* sv = sk + kTcK * kTcTileBytes;
+  __shared__ __align__(8) uint64_t q_full, k_full[kTcK], k_empty[kTcK], v_full[kTcTiles - kTcK],
+      v_empty[kTcTiles - kTcK], s_full[2], p_ready[2], o_done[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_fail, s_kissued, s_vissued;
+  __shared__ int s_valid[kTcValidRing];  // tokens of the tile that count, by the CTA's tile number
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 8);
+    for (int i = 0; i < kTcK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < vst; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_ready[x], 4);
+      mbar_init(&o_done[x], 1);
+    }
+    s_fail = 0;
+    s_kissued = s_vissued = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&s_tmem, 512u);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  pdl_wait();
+  pdl_trigger();
+  const int total = sp_total(p);
+  const int span = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+  TcWalk walk = {(int)blockIdx.x * span, min(total, ((int)blockIdx.x + 1) * span), 0, 0, 0};
+  TcPiece pc;
+
+  if (warp == 0 || warp == 2) {
+    // ---- producers
+    if (lane == 0) {
+      const bool keys = warp == 0;
+      const int NS = keys ? kTcK : vst;
+      uint64_t* full = keys ? k_full : v_full;
+      uint64_t* empty = keys ? k_empty : v_empty;
+      unsigned char* ring = keys ? sk : sv;
+      const CUtensorMap* map = keys ? &tmk : &tmv;
+      const uint64_t pol = l2_evict_first_policy();
+      int n = 0;
+      bool ok = true;
+      while (ok && walk.next(p, pc)) {
+        const int len = sp_len(p, pc.h);
+        const int32_t* bt = p.bt + (int64_t)pc.h * p.max_blocks;
+        // an injected stall (hc_set_wait_limits) loads no key tile: every wait
+        // on one runs out, for tests of the timeout path
+        for (int t = keys && p.stall ? pc.t1 : pc.t0; t < pc.t1; ++t, ++n) {
+          const int pos = t * kTcTile;
+          int blk = bt[pos >> 8];
+          const bool in = blk >= 0 && blk < p.n_blocks;
+          const int s = n % NS;
+          if (!mbar_wait_sleep(&empty[s], ((n / NS) & 1) ^ 1, p.wait_ns)) {
+            atomicExch(&s_fail, 1);
+            ok = false;
+            break;
+          }
+          if (keys) {
+            if (!in) set_err(p.err, HC_ERR_RANGE);
+            s_valid[n % kTcValidRing] = in ? min(kTcTile, len - pos) : 0;
+          }
+          unsigned char* dst = ring + (size_t)s * kTcTileBytes;
+          const int y = (in ? blk : 0) * kPage + (pos & (kPage - 1));
+          mbar_arrive_expect_tx(&full[s], (uint32_t)kTcTileBytes);
+          tma_load_2d(dst, map, 0, y, &full[s], pol);
+          tma_load_2d(dst + kTcBox, map, 64, y, &full[s], pol);
+          if (keys) s_kissued = n + 1;
+          else s_vissued = n + 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer: all lanes wait, lane 0 issues
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    const uint32_t id_s = idesc_f16_m128(kBf16, 128);
+    const uint32_t id_o = idesc_f16_m128(kBf16, 128) | kIdescBMajorMN;
+    int kbase = 0;                 // the piece's first tile's number
+    int ns[2] = {0, 0};            // S and O MMAs issued per stream
+    int nv[2] = {0, 0};
+    int piece = 0;
+    bool ok = true;
+    int kw = -1, vw = -1;          // last key / value tile waited for
+    while (ok && walk.next(p, pc)) {
+      const int nt = pc.t1 - pc.t0;
+      // steps of each stream: its tiles of the piece
+      const int n0 = wide ? nt : (nt + 1) >> 1;
+      const int n1 = wide ? (p.B * p.G - pc.ng * 256 > 128 ? nt : 0) : nt >> 1;
+      auto tile_of = [&](int x, int j) { return kbase + (wide ? j : 2 * j + x); };
+      auto issue_s = [&](int x, int j) -> bool {
+        const int n = tile_of(x, j);
+        if (n > kw) {
+          if (!mbar_wait_warp(&k_full[n % kTcK], (n / kTcK) & 1, p.wait_ns)) return false;
+          kw = n;
+        }
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t aq = smem_u32(sq + (wide ? x : 0) * kTcTileBytes);
+          const uint32_t bk = smem_u32(sk + (size_t)(n % kTcK) * kTcTileBytes);
+          const uint32_t d = tmem + kTcColS + (uint32_t)(128 * x);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = (uint32_t)((kk >> 2) * kTcBox + (kk & 3) * 32);
+            umma_f16(d, smem_desc_sw128(aq + off), smem_desc_sw128(bk + off), id_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[x]);
+          // the key stage is free once the last stream that reads it has
+          if (!wide || x == 1 || n1 == 0) umma_commit(&k_empty[n % kTcK]);
+        }
+        __syncwarp();
+        ++ns[x];
+        return true;
+      };
+      auto issue_pv = [&](int x, int j) -> bool {
+        const int n = tile_of(x, j);
+        unsigned char* vt = sv + (size_t)(n % vst) * kTcTileBytes;
+        if (n > vw) {
+          if (!mbar_wait_warp(&v_full[n % vst], (n / vst) & 1, p.wait_ns)) return false;
+          vw = n;
+          const int valid = s_valid[n % kTcValidRing];
+          if (valid < kTcTile) {  // zero the other tokens' values
+            for (int i = valid * 8 + lane; i < kTcTile * 8; i += 32) {
+              *reinterpret_cast<uint4*>(vt + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(vt + kTcBox + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        if (!mbar_wait_warp(&p_ready[x], nv[x] & 1, p.wait_ns)) return false;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t bv = smem_u32(vt);
+          const uint32_t d = tmem + kTcColO + (uint32_t)(128 * x);
+          const uint32_t pa = tmem + kTcColS + (uint32_t)(128 * x);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_f16_ts(d, pa + (uint32_t)(8 * kk), smem_desc_sw128_mn(bv + (uint32_t)(kk * 16 * 128), kTcBox), id_o,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&o_done[x]);
+          if (!wide || x == 1 || n1 == 0) umma_commit(&v_empty[n % vst]);
+        }
+        __syncwarp();
+        ++nv[x];
+        return true;
+      };
+      ok = mbar_wait_warp(&q_full, piece & 1, p.wait_ns);
+      if (ok && n0 > 0) ok = issue_s(0, 0);
+      if (ok && n1 > 0) ok = issue_s(1, 0);
+      for (int j = 0; ok && j < n0; ++j) {
+        ok = issue_pv(0, j);
+        if (ok && j + 1 < n0) ok = issue_s(0, j + 1);
+        if (ok && j < n1) ok = issue_pv(1, j);
+        if (ok && j + 1 < n1) ok = issue_s(1, j + 1);
+      }
+      kbase += nt;
+      ++piece;
+    }
+    if (!ok && lane == 0) atomicExch(&s_fail, 1);
+    // every MMA issued has completed before the tensor memory is released
+    for (int x = 0; x < 2; ++x) {
+      if (ns[x]) (void)mbar_wait_sleep(&s_full[x], (ns[x] - 1) & 1, p.wait_ns);
+      if (nv[x]) (void)mbar_wait_sleep(&o_done[x], (nv[x] - 1) & 1, p.wait_ns);
+    }
+  } else if (warp >= 4) {
+    // ---- softmax: one query row per thread (TMEM lane)
+    const int x = (warp - 4) >> 2;
+    const int row = 32 * (warp & 3) + lane;
+    const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t cs = tmem + lane_off + kTcColS + (uint32_t)(128 * x);
+    const uint32_t co = tmem + lane_off + kTcColO + (uint32_t)(128 * x);
+    const float sl2 = p.scale_log2;
+    const int tid = threadIdx.x - 128;  // of 256
+    int kbase = 0, steps = 0;
+    bool dead = false;
+    while (walk.next(p, pc)) {
+      const int nt = pc.t1 - pc.t0;
+      const int g0 = pc.ng * p.plan.rows_per;                       // the group's first query row
+      const int grows = min(p.plan.rows_per, p.B * p.G - g0);       // its rows
+      const int srows = min(128, grows - (wide ? 128 * x : 0));     // this stream's rows (may be <= 0)
+      const int n = wide ? (srows > 0 ? nt : 0) : (nt + 1 - x) >> 1;
+      // the queries, 128-byte swizzled; the MMAs that read the old ones have completed
+      named_bar_sync(1, 256);
+      for (int i = tid; i < nq * 128 * 16; i += 256) {
+        const int r = i >> 4, c = i & 15;
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (r < grows) {
+          const int qi = g0 + r, b = qi / p.G, g = qi % p.G;
+          w = ldg128(reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(pc.h * p.G + g) * p.qsh + c * 8);
+        }
+        *reinterpret_cast<uint4*>(sq + (r >> 7) * kTcTileBytes + (c >> 3) * kTcBox + swz128(r & 127, c & 7)) = w;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+      const bool active = 32 * (warp & 3) < srows;  // the warp's lanes hold query rows
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; j < n && !dead; ++j) {
+        if (!mbar_wait_warp(&s_full[x], (steps + j) & 1, p.wait_ns)) {
+          dead = true;
+          break;
+        }
+        tc_fence_after();
+        if (active) {
+          const int valid = s_valid[(kbase + (wide ? j : 2 * j + x)) % kTcValidRing];
+          const bool part = valid < kTcTile;
+          float mx = -INFINITY;
+#pragma unroll
+          for (int c2 = 0; c2 < 2; ++c2) {
+            uint32_t v[64];
+            tmem_ld32(cs + (uint32_t)(64 * c2), v);
+            tmem_ld32(cs + (uint32_t)(64 * c2 + 32), v + 32);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 64; ++i) {
+              const float s = (part && 64 * c2 + i >= valid) ? -INFINITY : __uint_as_float(v[i]);
+              mx = fmaxf(mx, s);
+            }
+          }
+          const float m_new = fmaxf(m_used, mx * sl2);  // log2 domain (scale > 0)
+          const bool resc = j > 0 && m_new > m_used + 8.f;
+          if (j == 0) m_used = m_new;
+          if (__any_sync(0xffffffffu, resc)) {
+            if (!mbar_wait_warp(&o_done[x], (steps + j - 1) & 1, p.wait_ns)) {
+              dead = true;
+              break;
+            }
+            tc_fence_after();
+            const float alpha = resc ? exp2_approx(m_used - m_new) : 1.f;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v[32];
+              tmem_ld32(co + (uint32_t)(32 * c), v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+              tmem_st32(co + (uint32_t)(32 * c), v);
+            }
+            if (resc) {
+              l *= alpha;
+              m_used = m_new;
+            }
+          }
+          const float nm = m_used == -INFINITY ? 0.f : -m_used;  // (no token so far: every P is 0)
+          float ps = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld32(cs + (uint32_t)(32 * c), v);
+            tmem_ld_wait();
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int k0 = 32 * c + 2 * i;
+              const float s0 = (part && k0 >= valid) ? -INFINITY : __uint_as_float(v[2 * i]);
+              const float s1 = (part && k0 + 1 >= valid) ? -INFINITY : __uint_as_float(v[2 * i + 1]);
+              const float e0 = exp2_approx(fmaf(s0, sl2, nm));
+              const float e1 = exp2_approx(fmaf(s1, sl2, nm));
+              ps += e0 + e1;
+              w[i] = Elem<T>::cvt2(e0, e1);
+            }
+            tmem_st16(cs + (uint32_t)(16 * c), w);
+          }
+          l += ps;
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[x]);
+      }
+      // the piece's partials: O relative to m_used, not divided by the sum
+      if (n > 0 && !dead && !mbar_wait_warp(&o_done[x], (steps + n - 1) & 1, p.wait_ns)) dead = true;
+      if (active && !dead) {
+        tc_fence_after();
+        const int64_t slot = (int64_t)blockIdx.x + pc.h * p.plan.n_groups + pc.ng;
+        const int64_t at = (slot * 2 + x) * 128 + row;
+        float* dst = p.plan.part_o + at * kD;
+        if (row < srows) p.plan.part_ml[at] = make_float2(m_used, l);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          if (n > 0) {
+            tmem_ld32(co + (uint32_t)(32 * c), v);
+            tmem_ld_wait();
+          } else {  // a stream without a tile in this piece
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0u;
+          }
+          if (row < srows)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(dst + 32 * c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2],
+                                                                          v[4 * i + 3]);
+        }
+        tc_fence_before();
+      }
+      steps += n;
+      kbase += nt;
+    }
+    if (dead && lane == 0) atomicExch(&s_fail, 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && s_fail) {
+    set_err(p.err, HC_ERR_TIMEOUT);
+    // the copies still in flight land before the CTA's shared memory is released
+    for (int j = max(0, s_kissued - kTcK); j < s_kissued; ++j)
+      (void)mbar_wait_sleep(&k_full[j % kTcK], (j / kTcK) & 1, p.wait_ns);
+    for (int j = max(0, s_vissued - vst); j < s_vissued; ++j)
+      (void)mbar_wait_sleep(&v_full[j % vst], (j / vst) & 1, p.wait_ns);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512u);
+  }
+}
+
 // Rows a CTA of the CUDA-core form: the fewest of 16, 32, 64 that hold the
 // batch's (a tile's work is the same for the rows it does not fill).
 static int sp_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-static PrefixPlan sp_plan(int B, int KV, int G, int sms) {
+static PrefixPlan sp_plan(int dtype, int B, int G, int sms) {
   PrefixPlan pl = {};
-  pl.rows_per = sp_rows(B * G);
-  pl.n_groups = (B * G + pl.rows_per - 1) / pl.rows_per;
-  pl.gran = kSpTok;
-  pl.streams = 1;
-  pl.stream_rows = pl.rows_per;
-  pl.n_ctas = 2 * sms;
+  const int rows = B * G;
+  if (dtype == HC_F32) {
+    pl.rows_per = pl.stream_rows = sp_rows(rows);
+    pl.gran = kSpTok;
+    pl.streams = 1;
+    pl.n_ctas = 2 * sms;
+  } else {
+    pl.rows_per = rows > 128 ? 256 : 128;
+    pl.stream_rows = 128;
+    pl.gran = kTcTile;
+    pl.streams = 2;
+    pl.n_ctas = sms;
+  }
+  pl.n_groups = (rows + pl.rows_per - 1) / pl.rows_per;
   return pl;
 }
 
@@ -220,28 +631,24 @@ static size_t sp_bytes(const PrefixPlan& pl, int KV, size_t* ml_at) {
 }
 
 size_t shared_prefix_ws_bytes(int dtype, int B, int KV, int G) {
-  (void)dtype;
-  return sp_bytes(sp_plan(B, KV, G, device_sms(current_device())), KV, nullptr);
+  return sp_bytes(sp_plan(dtype, B, G, device_sms(current_device())), KV, nullptr);
 }
 
-template <typename T, int RPT>
-static int sp_launch(SPParams& p, cudaStream_t st) {
-  auto kern = shared_prefix_kernel<T, RPT>;
-  constexpr size_t smem = sp_smem<T>(16 * RPT);
-  static bool attr_set[kMaxDevices];
-  const int dev = current_device();
-  if (dev < 0) return HC_ERR_CUDA;
-  {
-    std::lock_guard<std::mutex> g(host_lock());
-    if (!attr_set[dev]) {
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-        return HC_ERR_CUDA;
-      attr_set[dev] = true;
-    }
-  }
+// Raises a kernel's dynamic shared-memory limit once per device.
+template <typename K>
+static bool sp_allow_smem(K kern, size_t bytes, bool (&done)[kMaxDevices], int dev) {
+  std::lock_guard<std::mutex> g(host_lock());
+  if (done[dev]) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+  done[dev] = true;
+  return true;
+}
+
+template <typename K, typename... Args>
+static int sp_pdl_launch(K kern, int grid, int threads, size_t smem, cudaStream_t st, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned int)p.plan.n_ctas);
-  cfg.blockDim = dim3(kSpThreads);
+  cfg.gridDim = dim3((unsigned int)grid);
+  cfg.blockDim = dim3((unsigned int)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -249,31 +656,47 @@ static int sp_launch(SPParams& p, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, (const SPParams)p) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+}
+
+template <int RPT>
+static int sp_launch_f32(const SPParams& p, int dev, cudaStream_t st) {
+  static bool done[kMaxDevices];
+  constexpr size_t smem = sp_smem<float>(16 * RPT);
+  if (!sp_allow_smem(shared_prefix_kernel<float, RPT>, smem, done, dev)) return HC_ERR_CUDA;
+  return sp_pdl_launch(shared_prefix_kernel<float, RPT>, p.plan.n_ctas, kSpThreads, smem, st, p);
 }
 
 template <typename T>
-static int sp_launch_rows(SPParams& p, cudaStream_t st) {
-  switch (p.plan.rows_per) {
-    case 16: return sp_launch<T, 1>(p, st);
-    case 32: return sp_launch<T, 2>(p, st);
-    default: return sp_launch<T, 4>(p, st);
-  }
+static int sp_launch_tc(const SPParams& p, int dtype, int dev, cudaStream_t st) {
+  static bool done[kMaxDevices];
+  CUtensorMap tmk, tmv;
+  const long long rows = (long long)p.n_blocks * kPage;
+  if (!pool_tensor_map(&tmk, p.kp, rows, dtype, kTcTile)) return HC_ERR_CUDA;
+  if (!pool_tensor_map(&tmv, p.vp, rows, dtype, kTcTile)) return HC_ERR_CUDA;
+  if (!sp_allow_smem(shared_prefix_tc_kernel<T>, kTcSmem, done, dev)) return HC_ERR_CUDA;
+  return sp_pdl_launch(shared_prefix_tc_kernel<T>, p.plan.n_ctas, kTcThreads, kTcSmem, st, p, tmk, tmv);
 }
 
 int shared_prefix_dispatch(int dtype, SPParams& p, void* ws, size_t ws_bytes, cudaStream_t st) {
   const int dev = current_device();
   if (dev < 0) return HC_ERR_CUDA;
-  p.plan = sp_plan(p.B, p.KV, p.G, device_sms(dev));
+  p.plan = sp_plan(dtype, p.B, p.G, device_sms(dev));
   size_t ml_at;
   if (!ws || ws_bytes < sp_bytes(p.plan, p.KV, &ml_at)) return HC_ERR_WORKSPACE;
   p.plan.part_o = reinterpret_cast<float*>(ws);
   p.plan.part_ml = reinterpret_cast<float2*>(reinterpret_cast<unsigned char*>(ws) + ml_at);
   p.wait_ns = wait_limit_ns(kMbarTimeoutNs);
+  p.stall = injected_stall();
   switch (dtype) {
-    case HC_F32: return sp_launch_rows<float>(p, st);
-    case HC_BF16: return sp_launch_rows<__nv_bfloat16>(p, st);
-    case HC_F16: return sp_launch_rows<__half>(p, st);
+    case HC_F32:
+      switch (p.plan.rows_per) {
+        case 16: return sp_launch_f32<1>(p, dev, st);
+        case 32: return sp_launch_f32<2>(p, dev, st);
+        default: return sp_launch_f32<4>(p, dev, st);
+      }
+    case HC_BF16: return sp_launch_tc<__nv_bfloat16>(p, dtype, dev, st);
+    case HC_F16: return sp_launch_tc<__half>(p, dtype, dev, st);
     default: return HC_ERR_DTYPE;
   }
 }
