@@ -705,60 +705,11 @@ __global__ void __launch_bounds__(kTThreads, 2)
 // to 131072 tokens at the decode grid's spans); the partial's (m, l) comes
 // with it (a broadcast load); then the block maximum, each thread rescales
 // its own partials, and the 32 groups' sums are added in shared memory.
-// FD_TAIL: where the prefix part's partials of one (row, query head) are.
-struct PrefixRow {
-  int n;          // partials
-  int per;        // partials a piece (a CTA's part of the segment) has for the row
-  int64_t first;  // the first partial's index
-  int64_t step;   // from one piece's to the next, and between a piece's streams
-  int64_t stream;
-  __device__ __forceinline__ size_t at(int c) const { return (size_t)(first + (c / per) * step + (c % per) * stream); }
-};
-
-// s: two ints of shared memory.  Called by all threads.
-__device__ __forceinline__ PrefixRow prefix_row(const FDParams& p, int r, int g, int* s) {
-  const int h = r % p.KV, i = (r / p.KV) * p.G + g;
-  const PrefixPlan& pl = p.pre;
-  auto tiles_of = [&](int k) { return (fd_tail_lo(p, k) + pl.gran - 1) / pl.gran; };  // k < KV: row k is head k's
-  if (threadIdx.x < 32) {
-    int before = 0, all = 0;
-    for (int k = threadIdx.x; k < p.KV; k += 32) {
-      const int t = tiles_of(k);
-      all += t;
-      before += k < h ? t : 0;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-      all += __shfl_xor_sync(0xffffffffu, all, o);
-    }
-    if (threadIdx.x == 0) {
-      s[0] = before;
-      s[1] = all;
-    }
-  }
-  __syncthreads();
-  const int tiles = tiles_of(h);
-  const int ng = i / pl.rows_per, ii = i % pl.rows_per;
-  const int span = (s[1] * pl.n_groups + pl.n_ctas - 1) / pl.n_ctas;
-  PrefixRow out = {0, 1, 0, 0, 0};
-  if (tiles == 0) return out;
-  const int beg = s[0] * pl.n_groups + ng * tiles;
-  const int c0 = beg / span, c1 = (beg + tiles - 1) / span;
-  const int set = pl.streams * pl.stream_rows;
-  out.per = set > pl.rows_per ? pl.streams : 1;  // the streams split the tokens, or the rows
-  out.n = (c1 - c0 + 1) * out.per;
-  out.first = (int64_t)(c0 + h * pl.n_groups + ng) * set + ii;
-  out.step = set;
-  out.stream = pl.stream_rows;
-  return out;
-}
-
 constexpr int kCThreads = 256;
 constexpr int kCSlices = 4;
 constexpr int kCSliceDims = kD / kCSlices;  // 32
 
-template <typename T, int kMode>
+template <typename T>
 __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, int nctas) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   int* s_start = reinterpret_cast<int*>(smem_raw);
@@ -769,7 +720,7 @@ __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, in
   __shared__ float s_red[NW], s_redl[NW];
   __shared__ float s_mrun;  // running maximum over the rounds of 128 partials
   __shared__ float4 s_acc[NG][kCSliceDims / 4];
-  const int total = row_prefix<kMode>(p, s_start, s_warp);
+  const int total = row_prefix<FD_ALL>(p, s_start, s_warp);
   const int span = span_of(total, nctas, p.gran);
   const int rg = blockIdx.x / kCSlices, sl = blockIdx.x % kCSlices;
   const int r = rg / p.G, g = rg % p.G;
@@ -818,17 +769,12 @@ __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, in
           reinterpret_cast<const T*>(p.v_new)[b * p.vn_sb + (int64_t)h * p.vn_sh + d0 + threadIdx.x]);
     __syncthreads();
   }
-  const int c0 = span ? rs / span : 0, n_own = re == rs || span == 0 ? 0 : (re - 1) / span - c0 + 1;
-  const size_t slot0 = (size_t)(c0 + r);
-  // FD_TAIL: the prefix part's partials of this row's query head follow
-  __shared__ int s_pre[2];
-  PrefixRow pre = {0, 1, 0, 0, 0};
-  if constexpr (kMode == FD_TAIL) pre = prefix_row(p, r, g, s_pre);
-  const int n = n_own + pre.n;
-  if (n == 0) {  // no pages: the new token alone, or nothing
+  if (re == rs || span == 0) {  // no pages: the new token alone, or nothing
     if (threadIdx.x < kCSliceDims) store(threadIdx.x, has_new ? v_new_d : 0.f);
     return;
   }
+  const int c0 = rs / span, n = (re - 1) / span - c0 + 1;
+  const size_t slot0 = (size_t)(c0 + r);
   // the partials are written by the decode kernel launched just before
   pdl_wait();
   pdl_trigger();  // the next kernel may get resident; it waits for this grid
@@ -841,16 +787,9 @@ __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, in
     for (int u = 0; u < DEPTH; ++u) {
       const int c = cb0 + (warp * GPW + sub) + u * NG;
       const bool ok = c < n;
-      const float* po = p.part_o;
-      const float2* pml = p.part_ml;
-      size_t at = (slot0 + c) * p.G + g;
-      if (kMode == FD_TAIL && c >= n_own) {
-        po = p.pre.part_o;
-        pml = p.pre.part_ml;
-        at = pre.at(c - n_own);
-      }
-      ml[u] = ok ? pml[at] : make_float2(-INFINITY, 0.f);
-      o[u] = ok ? *reinterpret_cast<const float4*>(po + at * kD + d0 + 4 * q4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      ml[u] = ok ? p.part_ml[(slot0 + c) * p.G + g] : make_float2(-INFINITY, 0.f);
+      o[u] = ok ? *reinterpret_cast<const float4*>(p.part_o + ((slot0 + c) * p.G + g) * kD + d0 + 4 * q4)
+                : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float mw = -INFINITY;
 #pragma unroll
@@ -899,6 +838,194 @@ __global__ void __launch_bounds__(kCThreads) flash_combine_kernel(FDParams p, in
     for (int k = 0; k < NG; ++k) O += reinterpret_cast<const float*>(&s_acc[k][d / 4])[d % 4];
     store(d, L > 0.f ? O / L : 0.f);
   }
+}
+
+// ---------------------------------------------------------------------------
+// FD_TAIL and FD_BLOCKS: the join of a (row, query head)'s partials.  A warp
+// takes a partial at a time, 4 dims a lane (one coalesced 512-byte row); W
+// warps share a head (8 / W heads a CTA), so that a batch of many heads has
+// no more CTAs than it needs and a small one still has every load in flight.
+// FD_TAIL: the prefix part's partials follow the row's own, then the step's
+// token that is not in the pages (k_new, v_new).
+constexpr int kJThreads = 256;
+constexpr int kJWarps = kJThreads / 32;
+
+// A head's partials of the prefix part: one of each of the segment's pieces.
+struct PrefixRow {
+  int n;
+  int64_t first;  // index of the set of rows in the first piece; the next piece's is `streams` further
+  int row;
+};
+
+// FD_TAIL: `before` and `all` prefix tiles of the KV heads in front of head h
+// and of all; PrefixPlan says how the launch has laid them out.
+__device__ __forceinline__ PrefixRow prefix_row(const FDParams& p, int h, int i, int before, int all) {
+  const PrefixPlan& pl = p.pre;
+  const int tiles = (fd_tail_lo(p, h) + pl.gran - 1) / pl.gran;
+  PrefixRow out = {0, 0, 0};
+  if (tiles == 0) return out;
+  const int ng = i / pl.rows_per, ii = i % pl.rows_per;
+  const int span = (all * pl.n_groups + pl.n_ctas - 1) / pl.n_ctas;
+  const int beg = before * pl.n_groups + ng * tiles;
+  const int c0 = beg / span, c1 = (beg + tiles - 1) / span;
+  out.n = c1 - c0 + 1;
+  out.first = (int64_t)(c0 + h * pl.n_groups + ng) * pl.streams + ii / pl.stream_rows;
+  out.row = ii % pl.stream_rows;
+  return out;
+}
+
+template <typename T, int kMode, int W>
+__global__ void __launch_bounds__(kJThreads) flash_join_kernel(FDParams p, int nctas) {
+  __shared__ int4 s_red[kJWarps];
+  __shared__ float2 s_ml[kJWarps];
+  __shared__ float4 s_o[kJWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = blockIdx.x * (kJWarps / W);  // the CTA's first (row, head)
+  const int r_first = first / p.G;
+  // tokens in front of the CTA's first row and in all; FD_TAIL: the prefix's
+  // tiles in all (those in front of the warp's KV head come later)
+  int before = 0, total = 0, tiles = 0;
+  for (int r = threadIdx.x; r < p.R; r += kJThreads) {
+    const int len = max(0, fd_row_len<kMode>(p, r));
+    const int pad = (len + p.gran - 1) / p.gran * p.gran;
+    total += pad;
+    before += r < r_first ? pad : 0;
+  }
+  if constexpr (kMode == FD_TAIL)
+    for (int k = threadIdx.x; k < p.KV; k += kJThreads) tiles += (fd_tail_lo(p, k) + p.pre.gran - 1) / p.pre.gran;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+  }
+  if (lane == 0) s_red[warp] = make_int4(before, total, tiles, 0);
+  __syncthreads();
+  before = total = tiles = 0;
+#pragma unroll
+  for (int w = 0; w < kJWarps; ++w) {
+    before += s_red[w].x;
+    total += s_red[w].y;
+    tiles += s_red[w].z;
+  }
+  const int rg = min(first + warp / W, p.R * p.G - 1);  // (the last CTA's spare warps repeat its last head)
+  const int w0 = warp % W;
+  const int r = rg / p.G, g = rg % p.G, b = r / p.KV, h = r % p.KV;
+  int rs = before;
+  for (int k = r_first; k < r; ++k) rs += (max(0, fd_row_len<kMode>(p, k)) + p.gran - 1) / p.gran * p.gran;
+  const int re = rs + (max(0, fd_row_len<kMode>(p, r)) + p.gran - 1) / p.gran * p.gran;
+  const int span = span_of(total, nctas, p.gran);
+  const int c0 = span ? rs / span : 0, n_own = re > rs ? (re - 1) / span - c0 + 1 : 0;
+  const int64_t own0 = (int64_t)(c0 + r) * p.G + g;
+  PrefixRow pre = {0, 0, 0};
+  if constexpr (kMode == FD_TAIL) {
+    int pb = 0;
+    for (int k = lane; k < h; k += 32) pb += (fd_tail_lo(p, k) + p.pre.gran - 1) / p.pre.gran;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) pb += __shfl_xor_sync(0xffffffffu, pb, o);
+    pre = prefix_row(p, h, b * p.G + g, pb, tiles);
+  }
+  const int n = n_own + pre.n;
+  // the step's token: its score (log2 domain), 4 dims a lane
+  float s_new = -INFINITY;
+  float4 v_new = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (kMode == FD_TAIL && p.k_new != nullptr && w0 == 0) {
+    const T* q = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + g) * p.qsh + 4 * lane;
+    const T* k = reinterpret_cast<const T*>(p.k_new) + b * p.kn_sb + h * p.kn_sh + 4 * lane;
+    const T* v = reinterpret_cast<const T*>(p.v_new) + b * p.vn_sb + h * p.vn_sh + 4 * lane;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dot = fmaf(Elem<T>::to_f(q[i]), Elem<T>::to_f(k[i]), dot);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    s_new = dot * p.scale_log2;
+    v_new = make_float4(Elem<T>::to_f(v[0]), Elem<T>::to_f(v[1]), Elem<T>::to_f(v[2]), Elem<T>::to_f(v[3]));
+  }
+  pdl_wait();
+  pdl_trigger();
+  float M = s_new, L = s_new == -INFINITY ? 0.f : 1.f;
+  float4 O = v_new;  // (zeros where there is no new token)
+  // partial c: where its maximum and sum are, and this lane's 4 outputs
+  auto ml_at = [&](int c) -> const float2* {
+    if (kMode != FD_TAIL || c < n_own) return p.part_ml + own0 + (int64_t)c * p.G;
+    return p.pre.part_ml + (pre.first + (int64_t)(c - n_own) * p.pre.streams) * p.pre.stream_rows + pre.row;
+  };
+  auto o_at = [&](int c) -> const float4* {
+    if (kMode != FD_TAIL || c < n_own)
+      return reinterpret_cast<const float4*>(p.part_o + (own0 + (int64_t)c * p.G) * kD) + lane;
+    const int64_t set = (pre.first + (int64_t)(c - n_own) * p.pre.streams) * p.pre.stream_rows;
+    // 8 dims of all rows, then the next 8
+    return reinterpret_cast<const float4*>(p.pre.part_o + set * kD +
+                                           ((int64_t)(lane >> 1) * p.pre.stream_rows + pre.row) * 8) +
+           (lane & 1);
+  };
+  for (int base = w0; base < n; base += 32 * W) {
+    // up to 32 partials: lane i holds the i-th's maximum and sum
+    const int cnt = min(32, (n - base + W - 1) / W);
+    float2 ml = lane < cnt ? *ml_at(base + lane * W) : make_float2(-INFINITY, 0.f);
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float mn = fmaxf(M, mx), ref = mn == -INFINITY ? 0.f : mn;
+    const float corr = exp2f(M - ref), f = exp2f(ml.x - ref);
+    M = mn;
+    float ls = f * ml.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
+    L = fmaf(L, corr, ls);
+    O.x *= corr;
+    O.y *= corr;
+    O.z *= corr;
+    O.w *= corr;
+    constexpr int U = 8;
+    for (int i = 0; i < cnt; i += U) {
+      float4 o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        o[u] = i + u < cnt ? *o_at(base + (i + u) * W) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float fu = __shfl_sync(0xffffffffu, f, (i + u) & 31);
+        O.x = fmaf(fu, o[u].x, O.x);
+        O.y = fmaf(fu, o[u].y, O.y);
+        O.z = fmaf(fu, o[u].z, O.z);
+        O.w = fmaf(fu, o[u].w, O.w);
+      }
+    }
+  }
+  if constexpr (W > 1) {
+    if (lane == 0) s_ml[warp] = make_float2(M, L);
+    s_o[warp][lane] = O;
+    __syncthreads();
+    if (w0 != 0) return;
+    float mn = M;
+#pragma unroll
+    for (int w = 1; w < W; ++w) mn = fmaxf(mn, s_ml[warp + w].x);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    float f = exp2f(M - ref);
+    L *= f;
+    O.x *= f;
+    O.y *= f;
+    O.z *= f;
+    O.w *= f;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      f = exp2f(s_ml[warp + w].x - ref);
+      const float4 o = s_o[warp + w][lane];
+      L = fmaf(f, s_ml[warp + w].y, L);
+      O.x = fmaf(f, o.x, O.x);
+      O.y = fmaf(f, o.y, O.y);
+      O.z = fmaf(f, o.z, O.z);
+      O.w = fmaf(f, o.w, O.w);
+    }
+  }
+  if (first + warp / W >= p.R * p.G) return;
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  T* out = reinterpret_cast<T*>(p.out) + (int64_t)rg * kD + 4 * lane;
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<float4*>(out) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+  else
+    *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::cvt2(O.x * inv, O.y * inv), Elem<T>::cvt2(O.z * inv, O.w * inv));
 }
 
 // ---------------------------------------------------------------------------
@@ -1030,25 +1157,6 @@ size_t flash_decode_ws_bytes(int R, int G) {
   return slots * G * kD * sizeof(float) + slots * G * sizeof(float2) + 256;
 }
 
-template <typename T, int kMode>
-static int fd_combine(FDParams& p, int grid, cudaStream_t st) {
-  // launched as a programmatic dependent of the decode kernel: its CTAs may
-  // start early and wait (griddepcontrol.wait) for the partials
-  const size_t csm = (((size_t)(p.R + 1) * sizeof(int) + 15) & ~(size_t)15);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.R * p.G * kCSlices);
-  cfg.blockDim = dim3(kCThreads);
-  cfg.dynamicSmemBytes = csm;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, flash_combine_kernel<T, kMode>, p, grid) != cudaSuccess) return HC_ERR_CUDA;
-  return HC_OK;
-}
-
 // Launch with programmatic stream serialization: the grid may start while the
 // previous kernel in the stream drains; every kernel launched this way
 // executes griddepcontrol.wait before it reads anything.
@@ -1066,6 +1174,40 @@ static cudaError_t pdl_launch(void (*kern)(KArgs...), int grid, int threads, siz
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// Warps a head of the join: the most of 8, 4, 2, 1 that leave at most 8
+// waves' worth of 4 CTAs an SM; few heads take more warps each, which shortens
+// the chain of loads.
+template <typename T, int kMode>
+static int fd_join(FDParams& p, int grid, cudaStream_t st) {
+  const int heads = p.R * p.G;
+  if (heads <= 148 * 4)
+    return pdl_launch(flash_join_kernel<T, kMode, 8>, heads, kJThreads, 0, st, p, grid) == cudaSuccess ? HC_OK
+                                                                                                      : HC_ERR_CUDA;
+  return pdl_launch(flash_join_kernel<T, kMode, 2>, (heads + 3) / 4, kJThreads, 0, st, p, grid) == cudaSuccess
+             ? HC_OK
+             : HC_ERR_CUDA;
+}
+
+template <typename T, int kMode>
+static int fd_combine(FDParams& p, int grid, cudaStream_t st) {
+  if constexpr (kMode != FD_ALL) return fd_join<T, kMode>(p, grid, st);
+  // launched as a programmatic dependent of the decode kernel: its CTAs may
+  // start early and wait (griddepcontrol.wait) for the partials
+  const size_t csm = (((size_t)(p.R + 1) * sizeof(int) + 15) & ~(size_t)15);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.R * p.G * kCSlices);
+  cfg.blockDim = dim3(kCThreads);
+  cfg.dynamicSmemBytes = csm;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, flash_combine_kernel<T>, p, grid) != cudaSuccess) return HC_ERR_CUDA;
+  return HC_OK;
 }
 
 // fp32 pools: the global-load kernel, rows padded to 16.

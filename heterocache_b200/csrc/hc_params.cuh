@@ -129,8 +129,9 @@ int score_dispatch(int dtype, ScoreParams& p, void* ws, size_t ws_bytes, cudaStr
 // segment h * NG + group holds tiles of `gran` tokens of the head's shared
 // tokens; all segments' tiles are laid end to end and cut into equal spans,
 // one a CTA.  A CTA's partials of a segment are at slot (cta + segment):
-// `streams` sets of `stream_rows` rows each (max in the log2 domain, sum,
-// 128 outputs).
+// `streams` sets of `stream_rows` rows each: part_ml [set][row] (maximum in
+// the log2 domain, sum), part_o [set][16][row][8] (8 outputs of every row,
+// then the next 8).
 struct PrefixPlan {
   int n_ctas, n_groups, rows_per, gran, streams, stream_rows;
   float* part_o;

@@ -189,11 +189,11 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
         for (int x = 8; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
         const int row = ty * RPT + i;
         if (ng * RT + row >= p.B * p.G) continue;
-        const int64_t at = slot * RT + row;
-        if (tx == 0) p.plan.part_ml[at] = make_float2(m[i], s);
-        *reinterpret_cast<float4*>(p.plan.part_o + at * kD + 4 * tx) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-        *reinterpret_cast<float4*>(p.plan.part_o + at * kD + 64 + 4 * tx) =
-            make_float4(o[i][4], o[i][5], o[i][6], o[i][7]);
+        if (tx == 0) p.plan.part_ml[slot * RT + row] = make_float2(m[i], s);
+        // dims 4 tx .. of each half: half an 8-dim group of the layout
+        float* dst = p.plan.part_o + slot * RT * kD + ((int64_t)(tx >> 1) * RT + row) * 8 + (tx & 1) * 4;
+        *reinterpret_cast<float4*>(dst) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        *reinterpret_cast<float4*>(dst + (int64_t)8 * RT * 8) = make_float4(o[i][4], o[i][5], o[i][6], o[i][7]);
       }
     }
   }
@@ -235,26 +235,66 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, u
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit_ns));
 }
 
-// One CTA's part of one segment.
+// Two fp32 values in one 64-bit register: a * b + c and a + b of both.
+__device__ __forceinline__ uint64_t pack_f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// One CTA's part of one segment: tiles t0 .. t1 - 1 of head h's `len` tokens.
 struct TcPiece {
-  int h, ng, t0, t1;
+  int h, ng, t0, t1, len;
 };
-// Walks the CTA's pieces in order.
+// Walks the CTA's pieces in order; called by whole warps (lane i holds the
+// shared length of the i-th of 32 heads).
 struct TcWalk {
-  int beg, end, start, h, ng;
+  int beg, end, start, h, ng, lens;
+  __device__ __forceinline__ void init(const SPParams& p) {
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    for (int k = lane; k < p.KV; k += 32) n += (sp_len(p, k) + kTcTile - 1) / kTcTile;
+    lens = lane < p.KV ? sp_len(p, lane) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    n *= p.plan.n_groups;
+    const int span = (n + (int)gridDim.x - 1) / (int)gridDim.x;
+    beg = (int)blockIdx.x * span;
+    end = min(n, beg + span);
+    start = h = ng = 0;
+  }
   __device__ __forceinline__ bool next(const SPParams& p, TcPiece& out) {
-    while (h < p.KV) {
-      const int tiles = (sp_len(p, h) + kTcTile - 1) / kTcTile;
-      if (start >= end) return false;
+    while (h < p.KV && start < end) {
+      const int len = __shfl_sync(0xffffffffu, lens, h & 31);
+      const int tiles = (len + kTcTile - 1) / kTcTile;
       const int t0 = max(beg, start) - start, t1 = min(end, start + tiles) - start;
       out.h = h;
       out.ng = ng;
       out.t0 = t0;
       out.t1 = t1;
+      out.len = len;
       start += tiles;
       if (++ng == p.plan.n_groups) {
         ng = 0;
-        ++h;
+        if ((++h & 31) == 0) {
+          const int k = h + (int)(threadIdx.x & 31);
+          lens = k < p.KV ? sp_len(p, k) : 0;
+        }
       }
       if (t0 < t1) return true;
     }
@@ -278,6 +318,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail, s_kissued, s_vissued;
   __shared__ int s_valid[kTcValidRing];  // tokens of the tile that count, by the CTA's tile number
+  __shared__ float s_m[2][128], s_l1[128];  // the streams' maxima, stream 1's sums (streams of the same rows)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -309,50 +350,58 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t tmem = s_tmem;
   pdl_wait();
   pdl_trigger();
-  const int total = sp_total(p);
-  const int span = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-  TcWalk walk = {(int)blockIdx.x * span, min(total, ((int)blockIdx.x + 1) * span), 0, 0, 0};
+  TcWalk walk;
+  walk.init(p);
   TcPiece pc;
 
   if (warp == 0 || warp == 2) {
-    // ---- producers
-    if (lane == 0) {
-      const bool keys = warp == 0;
-      const int NS = keys ? kTcK : vst;
-      uint64_t* full = keys ? k_full : v_full;
-      uint64_t* empty = keys ? k_empty : v_empty;
-      unsigned char* ring = keys ? sk : sv;
-      const CUtensorMap* map = keys ? &tmk : &tmv;
-      const uint64_t pol = l2_evict_first_policy();
-      int n = 0;
-      bool ok = true;
-      while (ok && walk.next(p, pc)) {
-        const int len = sp_len(p, pc.h);
-        const int32_t* bt = p.bt + (int64_t)pc.h * p.max_blocks;
-        // an injected stall (hc_set_wait_limits) loads no key tile: every wait
-        // on one runs out, for tests of the timeout path
-        for (int t = keys && p.stall ? pc.t1 : pc.t0; t < pc.t1; ++t, ++n) {
+    // ---- producers (lane 0 issues)
+    const bool keys = warp == 0;
+    const int NS = keys ? kTcK : vst;
+    uint64_t* full = keys ? k_full : v_full;
+    uint64_t* empty = keys ? k_empty : v_empty;
+    unsigned char* ring = keys ? sk : sv;
+    const CUtensorMap* map = keys ? &tmk : &tmv;
+    const uint64_t pol = l2_evict_first_policy();
+    int n = 0;
+    bool ok = true;
+    while (ok && walk.next(p, pc)) {
+      const int32_t* bt = p.bt + (int64_t)pc.h * p.max_blocks;
+      // an injected stall (hc_set_wait_limits) loads no key tile: every wait
+      // on one runs out, for tests of the timeout path
+      if (keys && p.stall) continue;
+      // lane i holds the page of the i-th of 32 pages
+      int page0 = pc.t0 >> 1;
+      int pages = page0 + lane < p.max_blocks ? bt[page0 + lane] : -1;
+      for (int t = pc.t0; t < pc.t1; ++t, ++n) {
+        if ((t >> 1) - page0 == 32) {
+          page0 += 32;
+          pages = page0 + lane < p.max_blocks ? bt[page0 + lane] : -1;
+        }
+        const int blk = __shfl_sync(0xffffffffu, pages, (t >> 1) - page0);
+        if (lane == 0) {
           const int pos = t * kTcTile;
-          int blk = bt[pos >> 8];
           const bool in = blk >= 0 && blk < p.n_blocks;
           const int s = n % NS;
           if (!mbar_wait_sleep(&empty[s], ((n / NS) & 1) ^ 1, p.wait_ns)) {
             atomicExch(&s_fail, 1);
             ok = false;
-            break;
+          } else {
+            if (keys) {
+              if (!in) set_err(p.err, HC_ERR_RANGE);
+              s_valid[n % kTcValidRing] = in ? min(kTcTile, pc.len - pos) : 0;
+            }
+            unsigned char* dst = ring + (size_t)s * kTcTileBytes;
+            const int y = (in ? blk : 0) * kPage + (pos & (kPage - 1));
+            mbar_arrive_expect_tx(&full[s], (uint32_t)kTcTileBytes);
+            tma_load_2d(dst, map, 0, y, &full[s], pol);
+            tma_load_2d(dst + kTcBox, map, 64, y, &full[s], pol);
+            if (keys) s_kissued = n + 1;
+            else s_vissued = n + 1;
           }
-          if (keys) {
-            if (!in) set_err(p.err, HC_ERR_RANGE);
-            s_valid[n % kTcValidRing] = in ? min(kTcTile, len - pos) : 0;
-          }
-          unsigned char* dst = ring + (size_t)s * kTcTileBytes;
-          const int y = (in ? blk : 0) * kPage + (pos & (kPage - 1));
-          mbar_arrive_expect_tx(&full[s], (uint32_t)kTcTileBytes);
-          tma_load_2d(dst, map, 0, y, &full[s], pol);
-          tma_load_2d(dst + kTcBox, map, 64, y, &full[s], pol);
-          if (keys) s_kissued = n + 1;
-          else s_vissued = n + 1;
         }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+        if (!ok) break;
       }
     }
   } else if (warp == 1) {
@@ -456,6 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t co = tmem + lane_off + kTcColO + (uint32_t)(128 * x);
     const float sl2 = p.scale_log2;
     const int tid = threadIdx.x - 128;  // of 256
+    const int gq = 16 % p.G, gb = 16 / p.G;
     int kbase = 0, steps = 0;
     bool dead = false;
     while (walk.next(p, pc)) {
@@ -464,16 +514,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int grows = min(p.plan.rows_per, p.B * p.G - g0);       // its rows
       const int srows = min(128, grows - (wide ? 128 * x : 0));     // this stream's rows (may be <= 0)
       const int n = wide ? (srows > 0 ? nt : 0) : (nt + 1 - x) >> 1;
-      // the queries, 128-byte swizzled; the MMAs that read the old ones have completed
+      // the queries, 128-byte swizzled; the MMAs that read the old ones, and
+      // the loads of the old accumulators, have completed
       named_bar_sync(1, 256);
-      for (int i = tid; i < nq * 128 * 16; i += 256) {
-        const int r = i >> 4, c = i & 15;
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (r < grows) {
-          const int qi = g0 + r, b = qi / p.G, g = qi % p.G;
-          w = ldg128(reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(pc.h * p.G + g) * p.qsh + c * 8);
+      {
+        const int c = tid & 15;
+        int b = (g0 + (tid >> 4)) / p.G, g = (g0 + (tid >> 4)) % p.G;
+        const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)pc.h * p.G * p.qsh + c * 8;
+        unsigned char* dst = sq + (c >> 3) * kTcBox;
+#pragma unroll 8
+        for (int r = tid >> 4; r < nq * 128; r += 16) {
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (r < grows) w = ldg128(q + b * p.qsb + g * p.qsh);
+          *reinterpret_cast<uint4*>(dst + (r >> 7) * kTcTileBytes + swz128(r & 127, c & 7)) = w;
+          g += gq;
+          b += gb;
+          if (g >= p.G) {
+            g -= p.G;
+            ++b;
+          }
         }
-        *reinterpret_cast<uint4*>(sq + (r >> 7) * kTcTileBytes + (c >> 3) * kTcBox + swz128(r & 127, c & 7)) = w;
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -488,24 +548,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after();
         if (active) {
           const int valid = s_valid[(kbase + (wide ? j : 2 * j + x)) % kTcValidRing];
-          const bool part = valid < kTcTile;
-          float mx = -INFINITY;
+          uint32_t v[128];
+          tmem_ld32(cs, v);
+          tmem_ld32(cs + 32u, v + 32);
+          tmem_ld32(cs + 64u, v + 64);
+          tmem_ld32(cs + 96u, v + 96);
+          tmem_ld_wait();
+          if (valid < kTcTile) {
 #pragma unroll
-          for (int c2 = 0; c2 < 2; ++c2) {
-            uint32_t v[64];
-            tmem_ld32(cs + (uint32_t)(64 * c2), v);
-            tmem_ld32(cs + (uint32_t)(64 * c2 + 32), v + 32);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              const float s = (part && 64 * c2 + i >= valid) ? -INFINITY : __uint_as_float(v[i]);
-              mx = fmaxf(mx, s);
-            }
+            for (int i = 0; i < 128; ++i)
+              if (i >= valid) v[i] = 0xff800000u;  // -infinity
           }
-          const float m_new = fmaxf(m_used, mx * sl2);  // log2 domain (scale > 0)
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(v[i]);
+#pragma unroll
+          for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+          // log2 domain (scale > 0)
+          const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
           const bool resc = j > 0 && m_new > m_used + 8.f;
           if (j == 0) m_used = m_new;
           if (__any_sync(0xffffffffu, resc)) {
+            // P stays below 2^8: O and l are rescaled only when the maximum
+            // has grown by more since they last were
             if (!mbar_wait_warp(&o_done[x], (steps + j - 1) & 1, p.wait_ns)) {
               dead = true;
               break;
@@ -513,13 +578,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_after();
             const float alpha = resc ? exp2_approx(m_used - m_new) : 1.f;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t v[32];
-              tmem_ld32(co + (uint32_t)(32 * c), v);
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(co + (uint32_t)(16 * c), o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-              tmem_st32(co + (uint32_t)(32 * c), v);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(co + (uint32_t)(16 * c), o);
             }
             if (resc) {
               l *= alpha;
@@ -527,55 +592,73 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
           const float nm = m_used == -INFINITY ? 0.f : -m_used;  // (no token so far: every P is 0)
-          float ps = 0.f;
+          const uint64_t sl22 = pack_f2(sl2, sl2), nm2 = pack_f2(nm, nm);
+          uint64_t ps[2] = {0ull, 0ull};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_ld32(cs + (uint32_t)(32 * c), v);
-            tmem_ld_wait();
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int k0 = 32 * c + 2 * i;
-              const float s0 = (part && k0 >= valid) ? -INFINITY : __uint_as_float(v[2 * i]);
-              const float s1 = (part && k0 + 1 >= valid) ? -INFINITY : __uint_as_float(v[2 * i + 1]);
-              const float e0 = exp2_approx(fmaf(s0, sl2, nm));
-              const float e1 = exp2_approx(fmaf(s1, sl2, nm));
-              ps += e0 + e1;
+              const float2 t = unpack_f2(fma_f2(
+                  pack_f2(__uint_as_float(v[32 * c + 2 * i]), __uint_as_float(v[32 * c + 2 * i + 1])), sl22, nm2));
+              const float e0 = exp2_approx(t.x), e1 = exp2_approx(t.y);
+              ps[i & 1] = add_f2(ps[i & 1], pack_f2(e0, e1));
               w[i] = Elem<T>::cvt2(e0, e1);
             }
             tmem_st16(cs + (uint32_t)(16 * c), w);
           }
-          l += ps;
+          const float2 sum = unpack_f2(add_f2(ps[0], ps[1]));
+          l += sum.x + sum.y;
           tmem_st_wait();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[x]);
       }
-      // the piece's partials: O relative to m_used, not divided by the sum
+      // the piece's partials: O relative to the maximum, not divided by the sum
       if (n > 0 && !dead && !mbar_wait_warp(&o_done[x], (steps + n - 1) & 1, p.wait_ns)) dead = true;
+      const int64_t slot = (int64_t)blockIdx.x + pc.h * p.plan.n_groups + pc.ng;
+      float f0 = 1.f, f1 = 0.f;
+      if (!wide) {
+        // both streams hold the row: joined here, each warp half of the dims
+        // (either stream's accumulator is in the warp's own lanes)
+        s_m[x][row] = m_used;
+        if (x == 1) s_l1[row] = l;
+        tc_fence_after();
+        tc_fence_before();
+        named_bar_sync(1, 256);
+        const float m0 = s_m[0][row], m1 = s_m[1][row];
+        m_used = fmaxf(m0, m1);
+        const float ref = m_used == -INFINITY ? 0.f : m_used;
+        f0 = exp2_approx(m0 - ref);
+        f1 = exp2_approx(m1 - ref);
+        l = f0 * l + f1 * s_l1[row];  // (stream 0 stores it)
+      }
       if (active && !dead) {
         tc_fence_after();
-        const int64_t slot = (int64_t)blockIdx.x + pc.h * p.plan.n_groups + pc.ng;
-        const int64_t at = (slot * 2 + x) * 128 + row;
-        float* dst = p.plan.part_o + at * kD;
-        if (row < srows) p.plan.part_ml[at] = make_float2(m_used, l);
+        const int64_t set = wide ? (slot * 2 + x) * 128 : slot * 128;
+        // 8 dims of all rows, then the next 8: a warp's stores are 1 KB in a piece
+        float* dst = p.plan.part_o + set * kD + row * 8;
+        if (row < srows && (wide || x == 0)) p.plan.part_ml[set + row] = make_float2(m_used, l);
+        const bool both = !wide && nt > 1;  // (one tile: stream 1 has no accumulator)
+        const uint32_t ca = tmem + lane_off + kTcColO + (wide ? (uint32_t)(128 * x) : 0u);
+        const int c0 = wide ? 0 : 4 * x, c1 = wide ? 8 : 4 * x + 4;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          if (n > 0) {
-            tmem_ld32(co + (uint32_t)(32 * c), v);
-            tmem_ld_wait();
-          } else {  // a stream without a tile in this piece
+        for (int c = c0; c < c1; ++c) {
+          uint32_t v[16], u[16];
+          tmem_ld16(ca + (uint32_t)(16 * c), v);
+          if (both) tmem_ld16(ca + (uint32_t)(128 + 16 * c), u);
+          tmem_ld_wait();
+          if (!wide) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0u;
+            for (int i = 0; i < 16; ++i)
+              v[i] = __float_as_uint(__uint_as_float(v[i]) * f0 + (both ? __uint_as_float(u[i]) * f1 : 0.f));
           }
           if (row < srows)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(dst + 32 * c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2],
-                                                                          v[4 * i + 3]);
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(dst + (2 * c + (i >> 1)) * 128 * 8 + (i & 1) * 4) =
+                  make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
         tc_fence_before();
       }
@@ -617,7 +700,7 @@ static PrefixPlan sp_plan(int dtype, int B, int G, int sms) {
     pl.rows_per = rows > 128 ? 256 : 128;
     pl.stream_rows = 128;
     pl.gran = kTcTile;
-    pl.streams = 2;
+    pl.streams = pl.rows_per / 128;
     pl.n_ctas = sms;
   }
   pl.n_groups = (rows + pl.rows_per - 1) / pl.rows_per;
