@@ -256,12 +256,15 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gid = lane >> 2, tig = lane & 3;
-  pdl_wait();  // as in the TMA kernel
+  if constexpr (kMode != FD_TAIL) pdl_wait();  // as in the TMA kernel
   pdl_trigger();
   const int total = row_prefix<kMode>(p, s_start, s_warp);
   const int span = span_of(total, gridDim.x, p.gran);
   const int beg = blockIdx.x * span;
-  if (beg >= total) return;
+  if (beg >= total) {
+    if constexpr (kMode == FD_TAIL) pdl_wait();
+    return;
+  }
   const int end = min(total, beg + span);
   // first row with s_start[r+1] > beg
   int lo = 0, hi = p.R - 1;
@@ -363,6 +366,7 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
     }
     __syncthreads();
   }
+  if constexpr (kMode == FD_TAIL) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -541,8 +545,12 @@ __global__ void __launch_bounds__(kTThreads, 2)
   const int gid = lane >> 2, tig = lane & 3;
   // programmatic dependent launch: wait for the kernel before (the page
   // append) to finish, then let the combine get resident; it reads row
-  // lengths before its own wait and waits for this grid's partials
-  pdl_wait();
+  // lengths before its own wait and waits for this grid's partials.
+  // FD_TAIL: the kernel before is the prefix part, whose CTAs let this grid
+  // start only after what came before them was complete, and whose results
+  // this grid does not read: it waits for them at its end, so that the join,
+  // which waits for this grid, finds both.
+  if constexpr (kMode != FD_TAIL) pdl_wait();
   pdl_trigger();
   const int total = row_prefix<kMode>(p, s_start, s_warp, s_len);
   const int span = span_of(total, gridDim.x, kTTile);
@@ -555,7 +563,10 @@ __global__ void __launch_bounds__(kTThreads, 2)
     fence_mbar_init();
   }
   __syncthreads();
-  if (beg >= total) return;
+  if (beg >= total) {
+    if constexpr (kMode == FD_TAIL) pdl_wait();
+    return;
+  }
   const int end = min(total, beg + span);
   const int ntiles = (end - beg) / kTTile;
   int r0 = 0, hi = p.R - 1;  // first row with s_start[r+1] > beg
@@ -695,6 +706,7 @@ __global__ void __launch_bounds__(kTThreads, 2)
     }
   }
   if (cur >= 0) flush(cur);
+  if constexpr (kMode == FD_TAIL) pdl_wait();
 }
 
 // Merge of one (row, query head, 32-dim slice of the output): four CTAs per
@@ -960,9 +972,18 @@ __global__ void __launch_bounds__(kJThreads) flash_join_kernel(FDParams p, int n
            (lane & 1);
   };
   for (int base = w0; base < n; base += 32 * W) {
-    // up to 32 partials: lane i holds the i-th's maximum and sum
+    // up to 32 partials: lane i holds the i-th's maximum and sum; the first
+    // outputs are in flight with them
+    constexpr int U = 8;
     const int cnt = min(32, (n - base + W - 1) / W);
-    float2 ml = lane < cnt ? *ml_at(base + lane * W) : make_float2(-INFINITY, 0.f);
+    const float2 ml = lane < cnt ? *ml_at(base + lane * W) : make_float2(-INFINITY, 0.f);
+    float4 o[U];
+    auto load = [&](int i) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        o[u] = i + u < cnt ? *o_at(base + (i + u) * W) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    load(0);
     float mx = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -977,12 +998,8 @@ __global__ void __launch_bounds__(kJThreads) flash_join_kernel(FDParams p, int n
     O.y *= corr;
     O.z *= corr;
     O.w *= corr;
-    constexpr int U = 8;
     for (int i = 0; i < cnt; i += U) {
-      float4 o[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        o[u] = i + u < cnt ? *o_at(base + (i + u) * W) : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i > 0) load(i);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float fu = __shfl_sync(0xffffffffu, f, (i + u) & 31);

@@ -203,9 +203,13 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
 // Tensor-core form (16-bit types): one CTA per SM, tiles of 128 tokens.
 //   S = Q K^T  (M = 128 query rows on the TMEM lanes, N = 128 tokens)
 //   O += P V   (A = P from tensor memory, B = V as loaded, MN-major)
-// Two streams X = 0, 1, each with its own S (P is written over its first 64
-// columns) and O accumulators, so that the tensor core works on one while
-// the softmax warps work on the other.  With at most 128 query rows a group
+// Two streams X = 0, 1, each with its own O accumulator, so that the tensor
+// core works on one while the softmax warps work on the other.  A stream
+// takes its tiles in halves of 64 tokens, with two S accumulators in turn (P
+// is written over the first 32 columns of its S): the scores of a half are
+// computed while the softmax of the one before runs, which halved the time a
+// softmax warp waits (128 tokens a step, one S a stream: 4800 clocks a step,
+// 2700 of them waiting for S).  With at most 128 query rows a group
 // both streams hold the same rows and take the tiles in turn (X takes tiles
 // X, X + 2, ...): two independent splits of the tokens.  With up to 256 the
 // streams hold 128 rows each and every tile serves both.
@@ -228,6 +232,8 @@ constexpr int kTcTiles = 7;              // tile buffers: queries, keys, values
 constexpr size_t kTcSmem = 1024 + (size_t)kTcTiles * kTcTileBytes;
 constexpr int kTcK = 3;                  // key stages; values have the rest
 constexpr int kTcValidRing = 8;          // tiles whose valid counts are kept
+constexpr int kTcHalf = 64;              // tokens of a step
+// tensor-memory columns: S of stream X, buffer i at 128 X + 64 i, O at 256 + 128 X
 constexpr uint32_t kTcColS = 0, kTcColO = 256;
 
 // The same answer for the whole warp (each lane polls for itself).
@@ -255,6 +261,15 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// One lane of the (converged) warp.  A branch on it tells the compiler that
+// one thread is active, so that it need not serialise the instructions whose
+// operands are uniform registers (MMAs, commits).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(is));
+  return is != 0;
 }
 
 // One CTA's part of one segment: tiles t0 .. t1 - 1 of head h's `len` tokens.
@@ -302,6 +317,131 @@ struct TcWalk {
   }
 };
 
+// What an MMA issuer needs of the CTA's shared memory.
+struct TcSmem {
+  unsigned char *sq, *sk, *sv;
+  int vst;
+  uint64_t *q_full, *k_full, *k_empty, *v_full, *v_empty;
+  uint64_t (*s_full)[2];
+  uint64_t (*p_ready)[2];
+  uint64_t* o_done;
+  const int* s_valid;
+};
+
+// The MMAs of both streams, called by a whole warp: all lanes wait, one issues
+// (the same one throughout: MMAs of one thread execute in order, so a half's
+// S may follow the O step that reads the P it overwrites).  Half h of a tile
+// has S buffer h.
+template <typename T>
+__device__ __forceinline__ bool tc_issue(const SPParams& p, const TcSmem& sm, TcWalk& walk, uint32_t tmem, bool wide) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  const uint32_t id_s = idesc_f16_m128(kBf16, kTcHalf);
+  const uint32_t id_o = idesc_f16_m128(kBf16, 128) | kIdescBMajorMN;
+  const int lane = threadIdx.x & 31;
+  int kbase = 0, piece = 0;   // the piece's first tile, pieces
+  int done[2] = {0, 0};       // tiles of earlier pieces per stream
+  int kw = -1, vw = -1;       // last key / value tile waited for
+  TcPiece pc;
+  auto wait_k = [&](int n) {
+    if (n <= kw) return true;
+    if (!mbar_wait_warp(&sm.k_full[n % kTcK], (n / kTcK) & 1, p.wait_ns)) return false;
+    kw = n;
+    tc_fence_after();
+    return true;
+  };
+  // the value tile, the tokens that do not count zeroed
+  auto wait_v = [&](int n) {
+    if (n <= vw) return true;
+    if (!mbar_wait_warp(&sm.v_full[n % sm.vst], (n / sm.vst) & 1, p.wait_ns)) return false;
+    vw = n;
+    const int valid = sm.s_valid[n % kTcValidRing];
+    if (valid < kTcTile) {
+      unsigned char* vt = sm.sv + (size_t)(n % sm.vst) * kTcTileBytes;
+      for (int c = valid * 8 + lane; c < kTcTile * 8; c += 32) {
+        *reinterpret_cast<uint4*>(vt + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(vt + kTcBox + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
+    return true;
+  };
+  // S of half h of tile n for stream x; free_k: the tile's last
+  auto issue_s = [&](int x, int n, int h, bool free_k) {
+    if (elect_one()) {
+      const uint64_t dq = smem_desc_sw128(smem_u32(sm.sq + (wide ? x : 0) * kTcTileBytes));
+      const uint64_t dk = smem_desc_sw128(smem_u32(sm.sk + (size_t)(n % kTcK) * kTcTileBytes) + h * kTcHalf * 128);
+      const uint32_t d = tmem + kTcColS + (uint32_t)(128 * x + 64 * h);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const uint64_t off = (uint64_t)(((kk >> 2) * kTcBox + (kk & 3) * 32) >> 4);
+        umma_f16(d, dq + off, dk + off, id_s, kk > 0 ? 1u : 0u);
+      }
+      umma_commit(&sm.s_full[x][h]);
+      if (free_k) umma_commit(&sm.k_empty[n % kTcK]);
+    }
+    __syncwarp();
+  };
+  auto issue_pv = [&](int x, int n, int h, bool first, bool free_v) {
+    if (elect_one()) {
+      const uint64_t dv = smem_desc_sw128_mn(
+          smem_u32(sm.sv + (size_t)(n % sm.vst) * kTcTileBytes) + h * kTcHalf * 128, kTcBox);
+      const uint32_t d = tmem + kTcColO + (uint32_t)(128 * x);
+      const uint32_t pa = tmem + kTcColS + (uint32_t)(128 * x + 64 * h);
+#pragma unroll
+      for (int kk = 0; kk < kTcHalf / 16; ++kk)
+        umma_f16_ts(d, pa + (uint32_t)(8 * kk), dv + (uint64_t)((kk * 16 * 128) >> 4), id_o,
+                    (!first || kk > 0) ? 1u : 0u);
+      umma_commit(&sm.o_done[x]);
+      if (free_v) umma_commit(&sm.v_empty[n % sm.vst]);
+    }
+    __syncwarp();
+  };
+  bool ok = true;
+  while (ok && walk.next(p, pc)) {
+    const int nt = pc.t1 - pc.t0;
+    // each stream's tiles: first, first + step, ..
+    const int step = wide ? 1 : 2;
+    const bool both = !wide || p.B * p.G - pc.ng * 256 > 128;  // (wide: stream 1 has rows)
+    const int n0 = wide ? nt : (nt + 1) >> 1, n1 = !both ? 0 : wide ? nt : nt >> 1;
+    const int f0 = kbase, f1 = kbase + (wide ? 0 : 1);
+    // a tile's stage is free once the last stream that reads it has
+    const bool last0 = !wide || !both;
+    kbase += nt;
+    ok = mbar_wait_warp(sm.q_full, piece++ & 1, p.wait_ns) && wait_k(f0);
+    if (!ok) break;
+    for (int h = 0; h < 2; ++h) {
+      issue_s(0, f0, h, last0 && h);
+      if (n1 > 0) {
+        ok = ok && wait_k(f1);
+        if (ok) issue_s(1, f1, h, h);
+      }
+    }
+    for (int i = 0; ok && i < n0; ++i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int n = (x ? f1 : f0) + i * step, nx = x ? n1 : n0;
+          if (!ok || i >= nx) continue;
+          ok = wait_v(n) && mbar_wait_warp(&sm.p_ready[x][h], (done[x] + i) & 1, p.wait_ns);
+          if (!ok) continue;
+          tc_fence_after();
+          const bool last = x == 1 || last0;
+          issue_pv(x, n, h, i == 0 && h == 0, last && h);
+          if (i + 1 < nx) {
+            ok = wait_k(n + step);
+            if (ok) issue_s(x, n + step, h, last && h);
+          }
+        }
+      }
+    }
+    done[0] += n0;
+    done[1] += n1;
+  }
+  return ok;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kTcThreads, 1)
     shared_prefix_tc_kernel(const SPParams p, const __grid_constant__ CUtensorMap tmk,
@@ -314,7 +454,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   unsigned char* sk = sq + nq * kTcTileBytes;
   unsigned char* sv = sk + kTcK * kTcTileBytes;
   __shared__ __align__(8) uint64_t q_full, k_full[kTcK], k_empty[kTcK], v_full[kTcTiles - kTcK],
-      v_empty[kTcTiles - kTcK], s_full[2], p_ready[2], o_done[2];
+      v_empty[kTcTiles - kTcK], s_full[2][2], p_ready[2][2], o_done[2], all_done;
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail, s_kissued, s_vissued;
   __shared__ int s_valid[kTcValidRing];  // tokens of the tile that count, by the CTA's tile number
@@ -332,10 +472,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&v_empty[i], 1);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_full[x], 1);
-      mbar_init(&p_ready[x], 4);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[x][i], 1);
+        mbar_init(&p_ready[x][i], 4);
+      }
       mbar_init(&o_done[x], 1);
     }
+    mbar_init(&all_done, 1);
     s_fail = 0;
     s_kissued = s_vissued = 0;
     fence_mbar_init();
@@ -404,104 +547,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!ok) break;
       }
     }
-  } else if (warp == 1) {
-    // ---- MMA issuer: all lanes wait, lane 0 issues
-    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-    const uint32_t id_s = idesc_f16_m128(kBf16, 128);
-    const uint32_t id_o = idesc_f16_m128(kBf16, 128) | kIdescBMajorMN;
-    int kbase = 0;                 // the piece's first tile's number
-    int ns[2] = {0, 0};            // S and O MMAs issued per stream
-    int nv[2] = {0, 0};
-    int piece = 0;
-    bool ok = true;
-    int kw = -1, vw = -1;          // last key / value tile waited for
-    while (ok && walk.next(p, pc)) {
-      const int nt = pc.t1 - pc.t0;
-      // steps of each stream: its tiles of the piece
-      const int n0 = wide ? nt : (nt + 1) >> 1;
-      const int n1 = wide ? (p.B * p.G - pc.ng * 256 > 128 ? nt : 0) : nt >> 1;
-      auto tile_of = [&](int x, int j) { return kbase + (wide ? j : 2 * j + x); };
-      auto issue_s = [&](int x, int j) -> bool {
-        const int n = tile_of(x, j);
-        if (n > kw) {
-          if (!mbar_wait_warp(&k_full[n % kTcK], (n / kTcK) & 1, p.wait_ns)) return false;
-          kw = n;
-        }
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t aq = smem_u32(sq + (wide ? x : 0) * kTcTileBytes);
-          const uint32_t bk = smem_u32(sk + (size_t)(n % kTcK) * kTcTileBytes);
-          const uint32_t d = tmem + kTcColS + (uint32_t)(128 * x);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint32_t off = (uint32_t)((kk >> 2) * kTcBox + (kk & 3) * 32);
-            umma_f16(d, smem_desc_sw128(aq + off), smem_desc_sw128(bk + off), id_s, kk > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[x]);
-          // the key stage is free once the last stream that reads it has
-          if (!wide || x == 1 || n1 == 0) umma_commit(&k_empty[n % kTcK]);
-        }
-        __syncwarp();
-        ++ns[x];
-        return true;
-      };
-      auto issue_pv = [&](int x, int j) -> bool {
-        const int n = tile_of(x, j);
-        unsigned char* vt = sv + (size_t)(n % vst) * kTcTileBytes;
-        if (n > vw) {
-          if (!mbar_wait_warp(&v_full[n % vst], (n / vst) & 1, p.wait_ns)) return false;
-          vw = n;
-          const int valid = s_valid[n % kTcValidRing];
-          if (valid < kTcTile) {  // zero the other tokens' values
-            for (int i = valid * 8 + lane; i < kTcTile * 8; i += 32) {
-              *reinterpret_cast<uint4*>(vt + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(vt + kTcBox + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-        }
-        if (!mbar_wait_warp(&p_ready[x], nv[x] & 1, p.wait_ns)) return false;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t bv = smem_u32(vt);
-          const uint32_t d = tmem + kTcColO + (uint32_t)(128 * x);
-          const uint32_t pa = tmem + kTcColS + (uint32_t)(128 * x);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_f16_ts(d, pa + (uint32_t)(8 * kk), smem_desc_sw128_mn(bv + (uint32_t)(kk * 16 * 128), kTcBox), id_o,
-                        (j > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&o_done[x]);
-          if (!wide || x == 1 || n1 == 0) umma_commit(&v_empty[n % vst]);
-        }
-        __syncwarp();
-        ++nv[x];
-        return true;
-      };
-      ok = mbar_wait_warp(&q_full, piece & 1, p.wait_ns);
-      if (ok && n0 > 0) ok = issue_s(0, 0);
-      if (ok && n1 > 0) ok = issue_s(1, 0);
-      for (int j = 0; ok && j < n0; ++j) {
-        ok = issue_pv(0, j);
-        if (ok && j + 1 < n0) ok = issue_s(0, j + 1);
-        if (ok && j < n1) ok = issue_pv(1, j);
-        if (ok && j + 1 < n1) ok = issue_s(1, j + 1);
+    // the last stages' releases (asynchronous arrivals) have landed before
+    // the CTA gives up its shared memory
+    for (int i = max(0, n - NS); ok && i < n; ++i)
+      if (!mbar_wait_warp(&empty[i % NS], (i / NS) & 1, p.wait_ns)) {
+        if (lane == 0) atomicExch(&s_fail, 1);
+        ok = false;
       }
-      kbase += nt;
-      ++piece;
-    }
+  } else if (warp == 1) {
+    // ---- MMA issuer
+    const TcSmem sm = {sq, sk, sv, vst, &q_full, k_full, k_empty, v_full, v_empty, s_full, p_ready, o_done, s_valid};
+    const bool ok = tc_issue<T>(p, sm, walk, tmem, wide);
     if (!ok && lane == 0) atomicExch(&s_fail, 1);
     // every MMA issued has completed before the tensor memory is released
-    for (int x = 0; x < 2; ++x) {
-      if (ns[x]) (void)mbar_wait_sleep(&s_full[x], (ns[x] - 1) & 1, p.wait_ns);
-      if (nv[x]) (void)mbar_wait_sleep(&o_done[x], (nv[x] - 1) & 1, p.wait_ns);
-    }
+    if (elect_one()) umma_commit(&all_done);
+    __syncwarp();
+    (void)mbar_wait_warp(&all_done, 0, p.wait_ns);
+    __syncwarp();
   } else if (warp >= 4) {
     // ---- softmax: one query row per thread (TMEM lane)
     const int x = (warp - 4) >> 2;
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t cs = tmem + lane_off + kTcColS + (uint32_t)(128 * x);
+    const uint32_t cs0 = tmem + lane_off + kTcColS + (uint32_t)(128 * x);
     const uint32_t co = tmem + lane_off + kTcColO + (uint32_t)(128 * x);
     const float sl2 = p.scale_log2;
     const int tid = threadIdx.x - 128;  // of 256
@@ -513,7 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int g0 = pc.ng * p.plan.rows_per;                       // the group's first query row
       const int grows = min(p.plan.rows_per, p.B * p.G - g0);       // its rows
       const int srows = min(128, grows - (wide ? 128 * x : 0));     // this stream's rows (may be <= 0)
-      const int n = wide ? (srows > 0 ? nt : 0) : (nt + 1 - x) >> 1;
+      const int n = 2 * (wide ? (srows > 0 ? nt : 0) : (nt + 1 - x) >> 1);  // steps
       // the queries, 128-byte swizzled; the MMAs that read the old ones, and
       // the loads of the old accumulators, have completed
       named_bar_sync(1, 256);
@@ -522,17 +590,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int b = (g0 + (tid >> 4)) / p.G, g = (g0 + (tid >> 4)) % p.G;
         const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)pc.h * p.G * p.qsh + c * 8;
         unsigned char* dst = sq + (c >> 3) * kTcBox;
-#pragma unroll 8
-        for (int r = tid >> 4; r < nq * 128; r += 16) {
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (r < grows) w = ldg128(q + b * p.qsb + g * p.qsh);
-          *reinterpret_cast<uint4*>(dst + (r >> 7) * kTcTileBytes + swz128(r & 127, c & 7)) = w;
-          g += gq;
-          b += gb;
-          if (g >= p.G) {
-            g -= p.G;
-            ++b;
+        for (int r0 = tid >> 4; r0 < nq * 128; r0 += 128) {
+          uint4 w[8];  // eight loads in flight
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            w[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r0 + 16 * i < grows) w[i] = ldg128(q + b * p.qsb + g * p.qsh);
+            g += gq;
+            b += gb;
+            if (g >= p.G) {
+              g -= p.G;
+              ++b;
+            }
           }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(dst + (r0 >> 7) * kTcTileBytes + swz128((r0 + 16 * i) & 127, c & 7)) = w[i];
         }
       }
       fence_proxy_async_smem();
@@ -541,29 +614,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool active = 32 * (warp & 3) < srows;  // the warp's lanes hold query rows
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n && !dead; ++j) {
-        if (!mbar_wait_warp(&s_full[x], (steps + j) & 1, p.wait_ns)) {
+        const int i = steps + j, buf = i & 1;
+        const uint32_t cs = cs0 + (uint32_t)(64 * buf);
+        if (!mbar_wait_warp(&s_full[x][buf], (i >> 1) & 1, p.wait_ns)) {
           dead = true;
           break;
         }
         tc_fence_after();
         if (active) {
-          const int valid = s_valid[(kbase + (wide ? j : 2 * j + x)) % kTcValidRing];
-          uint32_t v[128];
+          const int valid =
+              s_valid[(kbase + (wide ? j >> 1 : (j & ~1) + x)) % kTcValidRing] - (j & 1) * kTcHalf;
+          uint32_t v[kTcHalf];
           tmem_ld32(cs, v);
           tmem_ld32(cs + 32u, v + 32);
-          tmem_ld32(cs + 64u, v + 64);
-          tmem_ld32(cs + 96u, v + 96);
           tmem_ld_wait();
-          if (valid < kTcTile) {
+          if (valid < kTcHalf) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i >= valid) v[i] = 0xff800000u;  // -infinity
+            for (int k = 0; k < kTcHalf; ++k)
+              if (k >= valid) v[k] = 0xff800000u;  // -infinity
           }
           float mx[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(v[i]);
+          for (int k = 0; k < 4; ++k) mx[k] = __uint_as_float(v[k]);
 #pragma unroll
-          for (int i = 4; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+          for (int k = 4; k < kTcHalf; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(v[k]));
           // log2 domain (scale > 0)
           const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
           const bool resc = j > 0 && m_new > m_used + 8.f;
@@ -571,7 +645,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (__any_sync(0xffffffffu, resc)) {
             // P stays below 2^8: O and l are rescaled only when the maximum
             // has grown by more since they last were
-            if (!mbar_wait_warp(&o_done[x], (steps + j - 1) & 1, p.wait_ns)) {
+            // (S of this step was issued after the O step before last, so at
+            // most the last one is open)
+            if (!mbar_wait_warp(&o_done[x], (i - 1) & 1, p.wait_ns)) {
               dead = true;
               break;
             }
@@ -583,7 +659,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tmem_ld16(co + (uint32_t)(16 * c), o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
               tmem_st16(co + (uint32_t)(16 * c), o);
             }
             if (resc) {
@@ -595,15 +671,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const uint64_t sl22 = pack_f2(sl2, sl2), nm2 = pack_f2(nm, nm);
           uint64_t ps[2] = {0ull, 0ull};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int k = 0; k < 16; ++k) {
               const float2 t = unpack_f2(fma_f2(
-                  pack_f2(__uint_as_float(v[32 * c + 2 * i]), __uint_as_float(v[32 * c + 2 * i + 1])), sl22, nm2));
+                  pack_f2(__uint_as_float(v[32 * c + 2 * k]), __uint_as_float(v[32 * c + 2 * k + 1])), sl22, nm2));
               const float e0 = exp2_approx(t.x), e1 = exp2_approx(t.y);
-              ps[i & 1] = add_f2(ps[i & 1], pack_f2(e0, e1));
-              w[i] = Elem<T>::cvt2(e0, e1);
+              ps[k & 1] = add_f2(ps[k & 1], pack_f2(e0, e1));
+              w[k] = Elem<T>::cvt2(e0, e1);
             }
             tmem_st16(cs + (uint32_t)(16 * c), w);
           }
@@ -613,10 +689,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[x]);
+        if (lane == 0) mbar_arrive(&p_ready[x][buf]);
       }
       // the piece's partials: O relative to the maximum, not divided by the sum
-      if (n > 0 && !dead && !mbar_wait_warp(&o_done[x], (steps + n - 1) & 1, p.wait_ns)) dead = true;
+      // (the last two O steps may both be open: one phase after the other, a
+      // parity tells only neighbouring phases apart)
+      for (int k = 2; k > 0; --k)
+        if (n > 0 && !dead && !mbar_wait_warp(&o_done[x], (steps + n - k) & 1, p.wait_ns)) dead = true;
       const int64_t slot = (int64_t)blockIdx.x + pc.h * p.plan.n_groups + pc.ng;
       float f0 = 1.f, f1 = 0.f;
       if (!wide) {
@@ -679,6 +758,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   __syncthreads();
   if (warp == 1) {
+    __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512u);
   }
