@@ -66,6 +66,10 @@ SIGNATURES = {
     "hc_flash_decode_blocks": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p,
                        c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p,
                        c_void_p, c_size_t, c_void_p, c_void_p]),
+    "hc_flash_decode_sparse_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "hc_flash_decode_sparse": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p,
+                       c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p,
+                       c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "hc_flash_decode_shared_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "hc_flash_decode_shared": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p,
                        c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,

@@ -96,21 +96,22 @@ int block_bounds_dispatch(int dtype, const BBParams& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// Scores: one warp per (row, block), 4 channels a lane.
+// Scores.  A warp takes 16 blocks, two for each 4 lanes: lane p of the four
+// holds the 16-byte chunks p, p + 4, .. of the blocks' least and greatest
+// keys (a load of the warp is eight 64-byte pieces), as 64-bit values, and
+// multiplies them with the query heads, which lie in shared memory split into
+// their positive and negative parts:
+//   max(q lo, q hi) = max(q, 0) hi + min(q, 0) lo   for lo <= hi,
+// one of the two products being zero.  Bounds the wrong way round are swapped
+// first.  A sum that is not finite (an infinite or NaN bound or query) is
+// taken again from the formula as it stands.
+// The queries' layout puts the four lanes' values side by side: with [dim]
+// rows the four read the same banks, which took 130 us at 128 rows x 820
+// blocks (80% of the shared-memory pipe, the 64-bit units at 6%).
 constexpr int kBsThreads = 256;
 constexpr int kBsWarps = kBsThreads / 32;
-
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&f)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 w = *reinterpret_cast<const float4*>(p);
-    f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
-  } else {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
-  }
-}
+constexpr int kBsTwo = 2;                           // blocks a lane has in hand
+constexpr int kBsCta = kBsWarps * 8 * kBsTwo;       // blocks of a CTA
 
 // Blocks of a row, its length clamped to the page table.
 __device__ __forceinline__ int bs_blocks(const BSParams& p, int r) {
@@ -118,48 +119,156 @@ __device__ __forceinline__ int bs_blocks(const BSParams& p, int r) {
   return (len + HC_SPARSE_BLOCK - 1) / HC_SPARSE_BLOCK;
 }
 
+// E elements of 16 bytes as fp32.
+template <typename T, int E>
+__device__ __forceinline__ void bs_unpack(const uint4& w, float (&f)[E]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(w.x);
+    f[1] = __uint_as_float(w.y);
+    f[2] = __uint_as_float(w.z);
+    f[3] = __uint_as_float(w.w);
+  } else {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = unpack2<T>(u[i]);
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  }
+}
+
+// The score's definition, for one lane: sums of max(q lo, q hi), NaN as the
+// highest, the greatest over the heads.
 template <typename T>
-__global__ void __launch_bounds__(kBsThreads) block_score_kernel(const BSParams p) {
+__device__ __noinline__ double bs_plain_score(const BSParams& p, int r, const T* lim) {
+  const int b = r / p.KV, h = r % p.KV;
+  double best = -INFINITY;
+#pragma unroll 1
+  for (int g = 0; g < p.G; ++g) {
+    const T* q = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + g) * p.qsh;
+    double s = 0.0;
+#pragma unroll 1
+    for (int d = 0; d < kD; ++d) {
+      const double x = (double)Elem<T>::to_f(q[d]) * (double)Elem<T>::to_f(lim[d]);
+      const double y = (double)Elem<T>::to_f(q[d]) * (double)Elem<T>::to_f(lim[kD + d]);
+      s += x > y || isnan(x) ? x : y;
+    }
+    best = fmax(best, isnan(s) ? (double)INFINITY : s);
+  }
+  return best;
+}
+
+template <typename T, int kG>
+__global__ void __launch_bounds__(kBsThreads, 2) block_score_kernel(const BSParams p) {
+  constexpr int E = 16 / (int)sizeof(T), CH = kD / E, MINE = CH / 4;  // chunks of a row, of a lane
+  constexpr int STEP = MINE < 4 ? MINE : 4;                           // chunks loaded at a time
+  constexpr int GP = (kG + 1) / 2;                                    // pairs of heads
+  // [lane's chunk][element][sign][head pair][lane of the four] of two heads
+  extern __shared__ __align__(16) double2 s_q[];
   pdl_wait();
   pdl_trigger();
   const int r = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = bs_blocks(p, r);
-  if (n <= p.n_select) return;  // every block is listed
-  const int blk = blockIdx.x * kBsWarps + warp;
-  if (blk >= n) return;
+  if (n <= p.n_select || (int)blockIdx.x * kBsCta >= n) return;  // (n <= n_select: every block is listed)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = r / p.KV, h = r % p.KV;
-  const int phys = p.bt[(int64_t)r * p.max_blocks + blk / kBlkPerPage];
-  double* out = p.scores + (int64_t)r * p.max_blocks * kBlkPerPage + blk;
-  if (phys < 0 || phys >= p.n_blocks) {
-    if (lane == 0) {
-      set_err(p.err, HC_ERR_RANGE);
-      *out = -INFINITY;
-    }
-    return;
+  for (int i = threadIdx.x; i < 2 * GP * kD; i += kBsThreads) {
+    const int g = i / kD, d = i % kD, chunk = d / E;
+    const double q = g < p.G ? (double)Elem<T>::to_f(reinterpret_cast<const T*>(
+                                   p.q)[b * p.qsb + (int64_t)(h * p.G + g) * p.qsh + d])
+                             : 0.0;
+    double* at = reinterpret_cast<double*>(
+        s_q + ((((chunk >> 2) * E + d % E) * 2) * GP + (g >> 1)) * 4 + (chunk & 3)) + (g & 1);
+    at[0] = q < 0.0 ? 0.0 : q;  // (a NaN stays one)
+    at[GP * 4 * 2] = q < 0.0 ? q : 0.0;
   }
-  const T* lim = reinterpret_cast<const T*>(p.bounds) +
-                 ((int64_t)phys * kBlkPerPage + (blk & (kBlkPerPage - 1))) * 2 * kD + 4 * lane;
-  float lo[4], hi[4];
-  load4<T>(lim, lo);
-  load4<T>(lim + kD, hi);
-  double best = -INFINITY;
-  for (int g = 0; g < p.G; ++g) {
-    float q[4];
-    load4<T>(reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + g) * p.qsh + 4 * lane, q);
-    double s = 0.0;
+  __syncthreads();
+  const int part = lane & 3;
+  double* scores = p.scores + (int64_t)r * p.max_blocks * kBlkPerPage;
+#pragma unroll 1
+  for (int first = blockIdx.x * kBsCta; first < n; first += gridDim.x * kBsCta) {
+    if (first + warp * kBsTwo * 8 >= n) break;
+    const T* lim[kBsTwo];
+    int blk[kBsTwo];
+    bool ok[kBsTwo];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // (a product of two 32-bit values is exact in 64 bits)
-      const double x = (double)q[i] * (double)lo[i], y = (double)q[i] * (double)hi[i];
-      s += x > y || isnan(x) ? x : y;
+    for (int t = 0; t < kBsTwo; ++t) {
+      blk[t] = first + (warp * kBsTwo + t) * 8 + (lane >> 2);
+      int phys = blk[t] < n ? p.bt[(int64_t)r * p.max_blocks + blk[t] / kBlkPerPage] : -1;
+      ok[t] = phys >= 0 && phys < p.n_blocks;
+      if (blk[t] < n && !ok[t] && part == 0) set_err(p.err, HC_ERR_RANGE);
+      if (!ok[t]) phys = 0;
+      lim[t] = reinterpret_cast<const T*>(p.bounds) +
+               ((int64_t)phys * kBlkPerPage + (blk[t] & (kBlkPerPage - 1))) * 2 * kD;
+    }
+    double acc[kBsTwo][2 * GP];
+#pragma unroll
+    for (int t = 0; t < kBsTwo; ++t)
+#pragma unroll
+      for (int g = 0; g < 2 * GP; ++g) acc[t][g] = 0.0;
+#pragma unroll
+    for (int c0 = 0; c0 < MINE; c0 += STEP) {
+      uint4 wl[kBsTwo][STEP], wh[kBsTwo][STEP];
+#pragma unroll
+      for (int t = 0; t < kBsTwo; ++t)
+#pragma unroll
+        for (int c = 0; c < STEP; ++c) {
+          wl[t][c] = wh[t][c] = make_uint4(0u, 0u, 0u, 0u);
+          if (ok[t]) {
+            wl[t][c] = ld_stream128(lim[t] + (4 * (c0 + c) + part) * E);
+            wh[t][c] = ld_stream128(lim[t] + kD + (4 * (c0 + c) + part) * E);
+          }
+        }
+#pragma unroll
+      for (int c = 0; c < STEP; ++c) {
+        float lo[kBsTwo][E], hi[kBsTwo][E];
+#pragma unroll
+        for (int t = 0; t < kBsTwo; ++t) {
+          bs_unpack<T, E>(wl[t][c], lo[t]);
+          bs_unpack<T, E>(wh[t][c], hi[t]);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          double x[kBsTwo], y[kBsTwo];
+#pragma unroll
+          for (int t = 0; t < kBsTwo; ++t) {
+            x[t] = bb_max(lo[t][e], hi[t][e]);
+            y[t] = bb_min(lo[t][e], hi[t][e]);
+          }
+          const double2* q = s_q + (((c0 + c) * E + e) * 2) * GP * 4 + part;
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const double2 up = q[g * 4], down = q[(GP + g) * 4];
+#pragma unroll
+            for (int t = 0; t < kBsTwo; ++t) {
+              acc[t][2 * g] = fma(down.x, y[t], fma(up.x, x[t], acc[t][2 * g]));
+              acc[t][2 * g + 1] = fma(down.y, y[t], fma(up.y, x[t], acc[t][2 * g + 1]));
+            }
+          }
+        }
+      }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (isnan(s)) s = INFINITY;
-    best = fmax(best, s);
+    for (int t = 0; t < kBsTwo; ++t) {
+      double best = -INFINITY;
+      bool odd = false;
+#pragma unroll
+      for (int g = 0; g < 2 * GP; ++g) {
+        acc[t][g] += __shfl_xor_sync(0xffffffffu, acc[t][g], 1);
+        acc[t][g] += __shfl_xor_sync(0xffffffffu, acc[t][g], 2);
+        if (g < p.G) {
+          odd |= !isfinite(acc[t][g]);
+          best = fmax(best, acc[t][g]);
+        }
+      }
+      if (part == 0 && blk[t] < n) {
+        if (!ok[t]) best = -INFINITY;
+        else if (odd) best = bs_plain_score<T>(p, r, lim[t]);
+        scores[blk[t]] = best;
+      }
+    }
   }
-  if (lane == 0) *out = best;
 }
 
 // Order-preserving 64-bit key of a score (-0 as +0).
@@ -169,16 +278,22 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 }
 
 // ---------------------------------------------------------------------------
-// Selection: one CTA per row.  Radix select of the n_select-th greatest key,
-// 8 bits a round from the top, then one pass in block order.
-template <int kThreads>
-__global__ void __launch_bounds__(kThreads) block_select_kernel(const BSParams p) {
+// Selection: one CTA per row.  The sink and recent blocks are in; of the rest
+// a radix select finds the key of the last that is, 8 bits a round from the
+// highest bit in which the row's keys differ, until a digit's keys are all in
+// (three rounds or so).  Then one scan in block order lists them.
+constexpr int kSelThreads = 512;
+constexpr int kSelKeys = 4096;  // keys held in shared memory (rows of up to 262144 tokens)
+
+__global__ void __launch_bounds__(kSelThreads) block_select_kernel(const BSParams p) {
+  __shared__ unsigned long long s_key[kSelKeys];
   __shared__ unsigned int s_hist[256];
+  __shared__ unsigned long long s_min[kSelThreads / 32], s_max[kSelThreads / 32];
   __shared__ int s_warp[32];
-  __shared__ int s_digit, s_left;
+  __shared__ int s_digit, s_left, s_all;
   pdl_wait();
   pdl_trigger();
-  const int r = blockIdx.x;
+  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = bs_blocks(p, r);
   int32_t* list = p.blocks + (int64_t)r * p.n_select;
   const int count = min(n, p.n_select);
@@ -187,50 +302,105 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(const BSParams p
     const int len = p.heads_len[r];
     if (len < 0 || len > p.max_blocks * kPage) set_err(p.err, HC_ERR_RANGE);
   }
-  for (int i = count + threadIdx.x; i < p.n_select; i += kThreads) list[i] = -1;
+  for (int i = count + threadIdx.x; i < p.n_select; i += kSelThreads) list[i] = -1;
   if (n <= p.n_select) {
-    for (int i = threadIdx.x; i < n; i += kThreads) list[i] = i;
+    for (int i = threadIdx.x; i < n; i += kSelThreads) list[i] = i;
     return;
   }
+  // blocks lo .. hi - 1 compete for `left` places (sink + recent <= n_select < n)
+  const int lo = p.sink, hi = n - p.recent;
   const double* sc = p.scores + (int64_t)r * p.max_blocks * kBlkPerPage;
-  auto key = [&](int j) -> unsigned long long {
-    return (j < p.sink || j >= n - p.recent) ? ~0ull : score_key(sc[j]);
-  };
-  unsigned long long prefix = 0, mask = 0;
-  int left = count;  // how many of the keys that match the prefix are taken
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kThreads) s_hist[i] = 0;
+  const bool held = n <= kSelKeys;
+  auto key = [&](int j) -> unsigned long long { return held ? s_key[j] : score_key(sc[j]); };
+  unsigned long long kmin = ~0ull, kmax = 0ull;
+  for (int j = lo + threadIdx.x; j < hi; j += kSelThreads) {
+    const unsigned long long k = score_key(sc[j]);
+    if (held) s_key[j] = k;
+    kmin = min(kmin, k);
+    kmax = max(kmax, k);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    kmin = min(kmin, __shfl_xor_sync(0xffffffffu, kmin, o));
+    kmax = max(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
+  }
+  if (lane == 0) {
+    s_min[warp] = kmin;
+    s_max[warp] = kmax;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelThreads / 32; ++w) {
+    kmin = min(kmin, s_min[w]);
+    kmax = max(kmax, s_max[w]);
+  }
+  int left = count - lo - (n - hi);  // places among the keys that match the prefix
+  int top = kmin == kmax ? 0 : 64 - __clzll((long long)(kmin ^ kmax));  // bits still open
+  unsigned long long prefix = top < 64 ? kmax >> top << top : 0ull;
+  unsigned long long mask = top < 64 ? ~0ull >> top << top : 0ull;
+  bool all = left == 0;  // every key that matches the prefix is in (or none: left == 0)
+  while (top > 0 && !all) {
+    const int shift = max(top - 8, 0), bits = top - shift;
+    for (int i = threadIdx.x; i < 256; i += kSelThreads) s_hist[i] = 0;
     __syncthreads();
-    for (int j = threadIdx.x; j < n; j += kThreads) {
+    for (int j = lo + threadIdx.x; j < hi; j += kSelThreads) {
       const unsigned long long k = key(j);
-      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255], 1u);
+      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1u)], 1u);
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      int run = 0, d = 255;
-      while (d > 0 && run + (int)s_hist[d] < left) run += (int)s_hist[d--];
-      s_digit = d;
-      s_left = left - run;
+    if (warp == 0) {
+      // lane i holds digits 255 - 8 i .. 248 - 8 i: the greatest first
+      int c[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += c[i] = (int)s_hist[255 - 8 * lane - i];
+      int run = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += y;
+      }
+      run -= sum;  // keys of greater digits
+      if (run < left && run + sum >= left) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (run < left && run + c[i] >= left) {
+            s_digit = 255 - 8 * lane - i;
+            s_left = left - run;
+            s_all = left - run == c[i];
+          }
+          run += c[i];
+        }
+      }
     }
     __syncthreads();
-    left = s_left;
     prefix |= (unsigned long long)s_digit << shift;
-    mask |= 255ull << shift;
+    mask |= ((1ull << bits) - 1ull) << shift;
+    left = s_left;
+    all = s_all;
+    top = shift;
     __syncthreads();
   }
-  // prefix is the n_select-th greatest key; `left` of the blocks that have it are in
-  int taken = 0, ties = 0;
-  for (int j0 = 0; j0 < n; j0 += kThreads) {
-    const int j = j0 + threadIdx.x;
-    const unsigned long long k = j < n ? key(j) : 0ull;
-    const int eq = j < n && k == prefix;
-    int tot;
-    const int rank = ties + block_exclusive_scan(eq, s_warp, tot);
-    ties += tot;
-    const int in = j < n && (k > prefix || (eq && rank < left));
-    const int at = taken + block_exclusive_scan(in, s_warp, tot);
-    taken += tot;
-    if (in) list[at] = j;
+  // keys above the prefix are in, and the first `left` that match it; each
+  // thread lists a run of blocks
+  const int per = (n + kSelThreads - 1) / kSelThreads;
+  const int j0 = min(threadIdx.x * per, n), j1 = min(j0 + per, n);
+  int above = 0, equal = 0;
+  for (int j = j0; j < j1; ++j) {
+    const bool must = j < lo || j >= hi;
+    const unsigned long long k = must ? 0ull : key(j) & mask;
+    above += must || k > prefix;
+    equal += !must && k == prefix;
+  }
+  int tot;
+  int a = block_exclusive_scan(above, s_warp, tot);
+  int e = block_exclusive_scan(equal, s_warp, tot);
+  for (int j = j0; j < j1; ++j) {
+    const bool must = j < lo || j >= hi;
+    const unsigned long long k = must ? 0ull : key(j) & mask;
+    const bool in = must || k > prefix, eq = !must && k == prefix;
+    if (in || (eq && e < left)) list[a + min(e, left)] = j;
+    a += in;
+    e += eq;
   }
 }
 
@@ -238,10 +408,20 @@ size_t block_select_ws_bytes(int R, int max_blocks) {
   return (size_t)R * max_blocks * kBlkPerPage * sizeof(double) + 256;
 }
 
+template <typename T, int kG>
+static cudaError_t bs_launch_scores(const BSParams& p, cudaLaunchConfig_t& cfg) {
+  cfg.dynamicSmemBytes = (size_t)kD * 2 * ((kG + 1) / 2) * sizeof(double2);
+  return cudaLaunchKernelEx(&cfg, block_score_kernel<T, kG>, p);
+}
+
 template <typename T>
 static int bs_launch(BSParams& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned int)((p.max_blocks * kBlkPerPage + kBsWarps - 1) / kBsWarps), (unsigned int)p.R);
+  // CTAs of a row: enough for every SM to have its two; more would only load
+  // the queries more often
+  const int tiles = (p.max_blocks * kBlkPerPage + kBsCta - 1) / kBsCta;
+  const int want = (2 * device_sms(current_device()) + p.R - 1) / p.R;
+  cfg.gridDim = dim3((unsigned int)(tiles < want ? tiles : want), (unsigned int)p.R);
   cfg.blockDim = dim3(kBsThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -249,10 +429,13 @@ static int bs_launch(BSParams& p, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, block_score_kernel<T>, (const BSParams)p) != cudaSuccess) return HC_ERR_CUDA;
+  const cudaError_t e = p.G <= 1 ? bs_launch_scores<T, 1>(p, cfg) : p.G <= 2 ? bs_launch_scores<T, 2>(p, cfg)
+                        : p.G <= 4 ? bs_launch_scores<T, 4>(p, cfg) : bs_launch_scores<T, 8>(p, cfg);
+  if (e != cudaSuccess) return HC_ERR_CUDA;
   cfg.gridDim = dim3((unsigned int)p.R);
-  cfg.blockDim = dim3(512);
-  return cudaLaunchKernelEx(&cfg, block_select_kernel<512>, (const BSParams)p) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, block_select_kernel, (const BSParams)p) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
 }
 
 int block_select_dispatch(int dtype, BSParams& p, void* ws, size_t ws_bytes, cudaStream_t st) {

@@ -977,6 +977,36 @@ int hc_flash_decode_blocks(int dtype, int bsz, int num_kv_heads, int groups, int
       hc::flash_decode_dispatch(dtype, p, workspace, workspace_bytes, (cudaStream_t)stream, hc::FD_BLOCKS));
 }
 
+size_t hc_flash_decode_sparse_workspace_size(int bsz, int num_kv_heads, int groups, int head_dim, int max_blocks) {
+  (void)head_dim;
+  if (bsz <= 0 || num_kv_heads <= 0 || groups <= 0 || max_blocks <= 0) return 0;
+  return std::max(hc::block_select_ws_bytes(bsz * num_kv_heads, max_blocks),
+                  hc::flash_decode_ws_bytes(bsz * num_kv_heads, groups));
+}
+
+int hc_flash_decode_sparse(int dtype, int bsz, int num_kv_heads, int groups, int head_dim, const void* q, int64_t qsb,
+                           int64_t qsh, const void* k_pool, const void* v_pool, int n_pool_blocks,
+                           const int32_t* block_table, int max_blocks, const int32_t* heads_len, const void* bounds,
+                           int n_select, int sink, int recent, float scale, void* out, int32_t* blocks,
+                           int32_t* counts, void* workspace, size_t workspace_bytes, int32_t* err_flag,
+                           void* stream) {
+  // nothing is launched unless both parts can be
+  if (!valid_dtype(dtype)) return HC_ERR_DTYPE;
+  if (bsz <= 0 || num_kv_heads <= 0 || max_blocks <= 0 || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out))
+    return HC_ERR_INVALID;
+  if ((int64_t)bsz * num_kv_heads * n_select * HC_SPARSE_BLOCK > 0x7fffffffLL) return HC_ERR_UNSUPPORTED;
+  if (workspace_bytes < hc_flash_decode_sparse_workspace_size(bsz, num_kv_heads, groups, head_dim, max_blocks))
+    return HC_ERR_WORKSPACE;
+  // the scores of the selection are dead when the attention's partials come
+  const int rc = hc_block_select(dtype, bsz, num_kv_heads, groups, head_dim, q, qsb, qsh, bounds, n_pool_blocks,
+                                 block_table, max_blocks, heads_len, n_select, sink, recent, blocks, counts,
+                                 workspace, workspace_bytes, err_flag, stream);
+  if (rc != HC_OK) return rc;
+  return hc_flash_decode_blocks(dtype, bsz, num_kv_heads, groups, head_dim, q, qsb, qsh, k_pool, v_pool,
+                                n_pool_blocks, block_table, max_blocks, heads_len, blocks, counts, n_select, scale,
+                                out, workspace, workspace_bytes, err_flag, stream);
+}
+
 size_t hc_flash_decode_shared_workspace_size(int dtype, int bsz, int num_kv_heads, int groups, int head_dim) {
   (void)head_dim;
   if (!valid_dtype(dtype) || bsz <= 0 || num_kv_heads <= 0 || groups <= 0) return 0;

@@ -347,34 +347,70 @@ def flash_decode(q, k_pool, v_pool, block_table, heads_len, *, num_kv_heads, out
 _HERE = contextlib.nullcontext()
 
 
+def _refuse(what: str):
+    raise ValueError(f"heterocache_b200: {what}")
+
+
 def _same_device(*ts: Optional[torch.Tensor]):
     """All tensors on one CUDA device; a context in which that device is the
     current one (the library launches on the current device)."""
-    dev = ts[0].device
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"heterocache_b200: tensors on different devices ({dev} and {t.device})")
-    if dev.type != "cuda":
-        raise ValueError("heterocache_b200: tensors must live on a CUDA device")
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if t is not None and t.get_device() != dev:
+            _refuse(f"tensors on different devices ({ts[0].device} and {t.device})")
+    if dev < 0:
+        for t in ts:
+            if t is not None and t.device != ts[0].device:
+                _refuse(f"tensors on different devices ({ts[0].device} and {t.device})")
+        _refuse("tensors must live on a CUDA device")
+    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _pool(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
-    _need(t.dim() == 4 and t.shape[1:] == (PAGE, 1, HEAD_DIM) and t.is_contiguous(),
-          f"{name} must be a contiguous [n_blocks, {PAGE}, 1, {HEAD_DIM}] pool")
-    _need(t.dtype == like.dtype, f"{name} must have the dtype of the other operands")
+def _raw_stream(t: torch.Tensor) -> int:
+    """``_stream`` without building a stream object (a microsecond of a call's host time)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
-def _cache_rows(block_table, heads_len, rows: int) -> None:
-    _i32(block_table, "block_table"), _i32(heads_len, "heads_len")
-    _need(block_table.dim() == 2 and block_table.shape[0] >= rows and heads_len.numel() >= rows,
-          "block_table and heads_len need a row per (batch row, KV head)")
+def _ints(t: torch.Tensor, name: str, n: int, what: str) -> None:
+    """A contiguous int32 tensor of at least n entries."""
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        _refuse(f"{name} must be a contiguous int32 tensor")
+    if t.numel() < n:
+        _refuse(what)
 
 
-def _bounds(bounds, n_blocks: int, like: torch.Tensor) -> None:
-    _need(bounds.dtype == like.dtype and bounds.is_contiguous()
-          and tuple(bounds.shape) == (n_blocks, PAGE // BLOCK, 2, HEAD_DIM),
-          f"bounds must be a contiguous [n_blocks, {PAGE // BLOCK}, 2, {HEAD_DIM}] tensor in the pool dtype")
+def _pool(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
+    """A page pool; returns its number of pages."""
+    s = t.shape
+    if len(s) != 4 or s[1] != PAGE or s[2] != 1 or s[3] != HEAD_DIM or not t.is_contiguous():
+        _refuse(f"{name} must be a contiguous [n_blocks, {PAGE}, 1, {HEAD_DIM}] pool")
+    if t.dtype != dtype:
+        _refuse(f"{name} must have the dtype of the other operands")
+    return s[0]
+
+
+def _pools(k_pool, v_pool, dtype: torch.dtype) -> int:
+    n = _pool(k_pool, "k_pool", dtype)
+    if _pool(v_pool, "v_pool", dtype) != n:
+        _refuse("k_pool and v_pool must have the same shape")
+    return n
+
+
+def _cache_rows(block_table, heads_len, rows: int) -> int:
+    """The page table's and the lengths' rows; returns the table's width."""
+    s = block_table.shape
+    what = "block_table and heads_len need a row per (batch row, KV head)"
+    _ints(block_table, "block_table", 0, what)
+    if len(s) != 2 or s[0] < rows:
+        _refuse(what)
+    _ints(heads_len, "heads_len", rows, what)
+    return s[1]
+
+
+def _bounds(bounds, n_blocks: int, dtype: torch.dtype) -> None:
+    if (bounds.dtype != dtype or tuple(bounds.shape) != (n_blocks, PAGE // BLOCK, 2, HEAD_DIM)
+            or not bounds.is_contiguous()):
+        _refuse(f"bounds must be a contiguous [n_blocks, {PAGE // BLOCK}, 2, {HEAD_DIM}] tensor in the pool dtype")
 
 
 def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_blocks, free_ptr, err, *,
@@ -396,74 +432,92 @@ def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_
     cache as it was.  ``workspace`` holds a counter; calls that may overlap
     need a workspace each."""
     _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
-    _same_shape(k, v)
-    _need(q.dim() == 4 and k.dim() == 4, "q, k, v need [bsz, heads, tokens, D]")
+    if q.dim() != 4 or k.dim() != 4:
+        _refuse("q, k, v need [bsz, heads, tokens, D]")
     bsz, H, T, D = q.shape
-    KV = k.shape[1]
+    shape = k.shape
+    KV, dtype = shape[1], q.dtype
     dt = dtype_code(q)
-    _need(k.shape[0] == bsz and k.shape[2] == T and k.dtype == q.dtype, "q, k and v must share batch, tokens and dtype")
-    _need(bsz > 0 and KV > 0 and H > 0, "q, k and v need at least one sequence and one head")
-    _pool(k_pool, "k_pool", q), _pool(v_pool, "v_pool", q)
-    _need(k_pool.shape == v_pool.shape, "k_pool and v_pool must have the same shape")
-    _cache_rows(block_table, heads_len, bsz * KV)
-    _i32(free_blocks, "free_blocks"), _i32(free_ptr, "free_ptr"), _i32(err, "err")
-    _need(free_ptr.numel() >= 1 and err.numel() >= 1, "free_ptr and err need an entry")
-    trig = []
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        _rows(t, name)
-        t = t.unsqueeze(0) if t.dim() == 2 else t
-        _need(t.dim() == 3 and t.shape[0] in (1, bsz) and t.shape[1] == T, f"{name} needs [bsz or 1, tokens, D]")
-        _need(t.dtype in (q.dtype, torch.float32) and t.dtype == cos.dtype,
-              "cos and sin must share a dtype: the queries', or float32")
-        trig += [0 if t.shape[0] == 1 else t.stride(0), t.stride(1)]
+    if shape != v.shape or k.dtype != v.dtype:
+        _refuse("k and v must have the same shape and dtype")
+    if shape[0] != bsz or shape[2] != T or k.dtype != dtype:
+        _refuse("q, k and v must share batch, tokens and dtype")
+    R = bsz * KV
+    if R <= 0 or H <= 0:
+        _refuse("q, k and v need at least one sequence and one head")
+    n_pages = _pools(k_pool, v_pool, dtype)
+    width = _cache_rows(block_table, heads_len, R)
+    _ints(free_blocks, "free_blocks", 0, "")
+    _ints(free_ptr, "free_ptr", 1, "free_ptr and err need an entry")
+    _ints(err, "err", 1, "free_ptr and err need an entry")
+    trig = cos.dtype
+    cb, ct = _trig_strides(cos, "cos", bsz, T, dtype, trig)
+    sb, st = _trig_strides(sin, "sin", bsz, T, dtype, trig)
     if counts is not None:
-        _i32(counts, "counts")
-        _need(counts.numel() >= bsz, "counts needs an entry per sequence")
+        _ints(counts, "counts", bsz, "counts needs an entry per sequence")
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
     else:
         _rows(q_out, "q_out")
-        _need(q_out.shape == q.shape and q_out.dtype == q.dtype, "q_out must have the queries' shape and dtype")
+        if q_out.shape != q.shape or q_out.dtype != dtype:
+            _refuse("q_out must have the queries' shape and dtype")
     if heads_len_out is None:
         heads_len_out = heads_len
     else:
-        _i32(heads_len_out, "heads_len_out")
-        _need(heads_len_out.numel() >= bsz * KV, "heads_len_out needs a row per (batch row, KV head)")
+        _ints(heads_len_out, "heads_len_out", R, "heads_len_out needs a row per (batch row, KV head)")
     if bounds is not None:
-        _bounds(bounds, k_pool.shape[0], q)
+        _bounds(bounds, n_pages, dtype)
     counter = workspace.counter
-    (qb, qh, qt, _), (kb, kh, kt, _), (vb, vh, vt, _), (ob, oh, ot, _) = (q.stride(), k.stride(), v.stride(),
-                                                                          q_out.stride())
+    qb, qh, qt, _ = q.stride()
+    kb, kh, kt, _ = k.stride()
+    vb, vh, vt, _ = v.stride()
+    ob, oh, ot, _ = q_out.stride()
     with _same_device(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, heads_len_out, free_blocks, free_ptr,
                       err, counts, q_out, bounds, counter):
-        rc = lib().hc_rope_append(dt, DTYPES[cos.dtype], bsz, H, KV, T, D, q.data_ptr(), qb, qh, qt, k.data_ptr(), kb,
-                                  kh, kt, v.data_ptr(), vb, vh, vt, cos.data_ptr(), trig[0], trig[1], sin.data_ptr(),
-                                  trig[2], trig[3], q_out.data_ptr(), ob, oh, ot, _ptr(counts), k_pool.data_ptr(),
-                                  v_pool.data_ptr(), k_pool.shape[0], block_table.data_ptr(), block_table.shape[1],
-                                  heads_len.data_ptr(), heads_len_out.data_ptr(), free_blocks.data_ptr(),
-                                  free_blocks.numel(), free_ptr.data_ptr(), _ptr(bounds), counter.data_ptr(),
-                                  err.data_ptr(), _stream(q))
-    check("hc_rope_append", rc)
+        rc = lib().hc_rope_append(dt, DTYPES[trig], bsz, H, KV, T, D, q.data_ptr(), qb, qh, qt, k.data_ptr(), kb, kh,
+                                  kt, v.data_ptr(), vb, vh, vt, cos.data_ptr(), cb, ct, sin.data_ptr(), sb, st,
+                                  q_out.data_ptr(), ob, oh, ot, _ptr(counts), k_pool.data_ptr(), v_pool.data_ptr(),
+                                  n_pages, block_table.data_ptr(), width, heads_len.data_ptr(),
+                                  heads_len_out.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(),
+                                  free_ptr.data_ptr(), _ptr(bounds), counter.data_ptr(), err.data_ptr(),
+                                  _raw_stream(q))
+    if rc:
+        check("hc_rope_append", rc)
     LAUNCHES[0] += 1
     return q_out
 
 
-def _decode_operands(q, k_pool, v_pool, block_table, heads_len, num_kv_heads, out):
-    """Checks that the decode attentions below share; returns (out, bsz, G)."""
+def _trig_strides(t, name: str, bsz: int, T: int, dtype, trig) -> Tuple[int, int]:
+    """Batch and token stride of cos or sin, [bsz or 1, T, D] or [T, D]."""
+    _rows(t, name)
+    s = t.shape
+    if len(s) == 2:
+        s = (1,) + tuple(s)
+    if len(s) != 3 or (s[0] != 1 and s[0] != bsz) or s[1] != T:
+        _refuse(f"{name} needs [bsz or 1, tokens, D]")
+    if t.dtype != trig or (trig != dtype and trig != torch.float32):
+        _refuse("cos and sin must share a dtype: the queries', or float32")
+    return (0 if s[0] == 1 else t.stride(0)), t.stride(-2)
+
+
+def _decode_query(q, num_kv_heads: int, name: str) -> Tuple[int, int]:
+    """(bsz, query heads per KV head) of a decode step's query."""
     _rows(q, "q")
-    _need(q.dim() == 4 and q.shape[2] == 1, "decode attention takes one query position, [bsz, H, 1, D]")
-    bsz, H = q.shape[0], q.shape[1]
-    _need(bsz > 0 and num_kv_heads > 0 and H > 0 and H % num_kv_heads == 0,
-          f"the {H} query heads do not split evenly over {num_kv_heads} KV heads")
-    _pool(k_pool, "k_pool", q), _pool(v_pool, "v_pool", q)
-    _need(k_pool.shape == v_pool.shape, "k_pool and v_pool must have the same shape")
-    _cache_rows(block_table, heads_len, bsz * num_kv_heads)
+    s = q.shape
+    if len(s) != 4 or s[2] != 1:
+        _refuse(f"{name} takes one query position, [bsz, H, 1, D]")
+    if s[0] <= 0 or num_kv_heads <= 0 or s[1] <= 0 or s[1] % num_kv_heads:
+        _refuse(f"the {s[1]} query heads do not split evenly over {num_kv_heads} KV heads")
+    return s[0], s[1] // num_kv_heads
+
+
+def _decode_out(out, q, bsz: int) -> torch.Tensor:
+    H = q.shape[1]
     if out is None:
-        out = torch.empty(bsz, H, HEAD_DIM, dtype=q.dtype, device=q.device)
-    else:
-        _need(out.is_contiguous() and out.numel() == bsz * H * HEAD_DIM and out.dtype == q.dtype,
-              "out must be a contiguous [bsz, H, D] buffer in the query dtype")
-    return out, bsz, H // num_kv_heads
+        return torch.empty((bsz, H, HEAD_DIM), dtype=q.dtype, device=q.device)
+    if not out.is_contiguous() or out.numel() != bsz * H * HEAD_DIM or out.dtype != q.dtype:
+        _refuse("out must be a contiguous [bsz, H, D] buffer in the query dtype")
+    return out
 
 
 def flash_decode_shared(q, k_pool, v_pool, block_table, heads_len, shared_len, *, num_kv_heads, out=None,
@@ -474,27 +528,33 @@ def flash_decode_shared(q, k_pool, v_pool, block_table, heads_len, shared_len, *
     the first sequence's rows of the page table.  Each row's own tokens follow
     from position shared_len[h] to heads_len[r] - 1; with k_new / v_new [bsz,
     KV, 1, D] one more token a row, not in the pages."""
-    out, bsz, G = _decode_operands(q, k_pool, v_pool, block_table, heads_len, num_kv_heads, out)
-    _i32(shared_len, "shared_len"), _i32(err, "err")
-    _need(shared_len.numel() >= num_kv_heads, "shared_len needs an entry per KV head")
-    _need((k_new is None) == (v_new is None), "k_new and v_new come together")
+    bsz, G = _decode_query(q, num_kv_heads, "decode attention")
+    n_pages = _pools(k_pool, v_pool, q.dtype)
+    width = _cache_rows(block_table, heads_len, bsz * num_kv_heads)
+    out = _decode_out(out, q, bsz)
+    _ints(shared_len, "shared_len", num_kv_heads, "shared_len needs an entry per KV head")
+    _ints(err, "err", 1, "err needs an entry")
+    if (k_new is None) != (v_new is None):
+        _refuse("k_new and v_new come together")
     kn = vn = (0, 0)
     if k_new is not None:
         _rows(k_new, "k_new"), _rows(v_new, "v_new")
         _same_shape(k_new, v_new)
-        _need(tuple(k_new.shape) == (bsz, num_kv_heads, 1, HEAD_DIM) and k_new.dtype == q.dtype,
-              "k_new/v_new must be [bsz, KV, 1, D] in the query dtype")
+        if tuple(k_new.shape) != (bsz, num_kv_heads, 1, HEAD_DIM) or k_new.dtype != q.dtype:
+            _refuse("k_new/v_new must be [bsz, KV, 1, D] in the query dtype")
         kn, vn = k_new.stride(), v_new.stride()
     dt = dtype_code(q)
+    L = lib()
     with _same_device(q, k_pool, v_pool, block_table, heads_len, shared_len, out, err, k_new, v_new):
-        ws = workspace.get(lib().hc_flash_decode_shared_workspace_size(dt, bsz, num_kv_heads, G, HEAD_DIM))
-        rc = lib().hc_flash_decode_shared(dt, bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), q.stride(0), q.stride(1),
-                                          k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0],
-                                          block_table.data_ptr(), block_table.shape[1], heads_len.data_ptr(),
-                                          shared_len.data_ptr(), _ptr(k_new), _ptr(v_new), kn[0], kn[1], vn[0], vn[1],
-                                          float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr(),
-                                          _stream(q))
-    check("hc_flash_decode_shared", rc)
+        ws = workspace.get(L.hc_flash_decode_shared_workspace_size(dt, bsz, num_kv_heads, G, HEAD_DIM))
+        qs = q.stride()
+        rc = L.hc_flash_decode_shared(dt, bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1],
+                                      k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
+                                      heads_len.data_ptr(), shared_len.data_ptr(), _ptr(k_new), _ptr(v_new), kn[0],
+                                      kn[1], vn[0], vn[1], float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                      err.data_ptr(), _raw_stream(q))
+    if rc:
+        check("hc_flash_decode_shared", rc)
     LAUNCHES[0] += 3
     return out
 
@@ -504,22 +564,42 @@ def block_bounds(k_pool, block_table, heads_len, bounds, err, *, rows=None, last
     into ``bounds`` [n_blocks, 4, 2, D]: of every row, or of those listed in
     ``rows`` (int32); of all its blocks, or of those that hold its last
     ``last`` tokens."""
-    _pool(k_pool, "k_pool", k_pool)
+    n_pages = _pool(k_pool, "k_pool", k_pool.dtype)
     n = block_table.shape[0]
-    _cache_rows(block_table, heads_len, n)
-    _bounds(bounds, k_pool.shape[0], k_pool)
-    _i32(err, "err")
-    _need(last >= 0, "last must not be negative")
+    width = _cache_rows(block_table, heads_len, n)
+    _bounds(bounds, n_pages, k_pool.dtype)
+    _ints(err, "err", 1, "err needs an entry")
+    if last < 0:
+        _refuse("last must not be negative")
     if rows is not None:
-        _i32(rows, "rows")
+        _ints(rows, "rows", 0, "")
     with _same_device(k_pool, block_table, heads_len, bounds, err, rows):
-        rc = lib().hc_block_bounds(dtype_code(k_pool), n, HEAD_DIM, k_pool.data_ptr(), k_pool.shape[0],
-                                   block_table.data_ptr(), block_table.shape[1], heads_len.data_ptr(), _ptr(rows),
+        rc = lib().hc_block_bounds(dtype_code(k_pool), n, HEAD_DIM, k_pool.data_ptr(), n_pages,
+                                   block_table.data_ptr(), width, heads_len.data_ptr(), _ptr(rows),
                                    0 if rows is None else rows.numel(), int(last), bounds.data_ptr(), err.data_ptr(),
-                                   _stream(k_pool))
-    check("hc_block_bounds", rc)
+                                   _raw_stream(k_pool))
+    if rc:
+        check("hc_block_bounds", rc)
     LAUNCHES[0] += 1
     return bounds
+
+
+def _select_lists(q, bounds, R: int, n_select: int, sink: int, recent: int, blocks, counts):
+    """Checks of the selection's own operands; returns (blocks, counts)."""
+    if n_select < 1 or sink < 0 or recent < 0 or sink + recent > n_select:
+        _refuse("sink + recent blocks must not be more than n_select, which must be at least 1")
+    what = "blocks needs [rows, n_select] and counts an entry per row"
+    if blocks is None:
+        blocks = torch.empty((R, n_select), dtype=torch.int32, device=q.device)
+    else:
+        _ints(blocks, "blocks", 0, what)
+        if tuple(blocks.shape) != (R, n_select):
+            _refuse(what)
+    if counts is None:
+        counts = torch.empty((R,), dtype=torch.int32, device=q.device)
+    else:
+        _ints(counts, "counts", R, what)
+    return blocks, counts
 
 
 def block_select(q, bounds, block_table, heads_len, *, num_kv_heads, n_select: int, sink: int = 1, recent: int = 1,
@@ -528,33 +608,23 @@ def block_select(q, bounds, block_table, heads_len, *, num_kv_heads, n_select: i
     each row the first ``sink``, the last ``recent`` and those of the highest
     bound on their scores, n_select in all.  Returns (blocks [rows, n_select]
     int32 ascending, -1 behind; counts [rows] int32)."""
-    _rows(q, "q")
-    _need(q.dim() == 4 and q.shape[2] == 1, "block_select takes one query position, [bsz, H, 1, D]")
-    bsz, H = q.shape[0], q.shape[1]
-    _need(bsz > 0 and num_kv_heads > 0 and H > 0 and H % num_kv_heads == 0,
-          f"the {H} query heads do not split evenly over {num_kv_heads} KV heads")
-    _need(n_select >= 1 and sink >= 0 and recent >= 0 and sink + recent <= n_select,
-          "sink + recent blocks must not be more than n_select, which must be at least 1")
+    bsz, G = _decode_query(q, num_kv_heads, "block_select")
     R = bsz * num_kv_heads
-    _cache_rows(block_table, heads_len, R)
-    _bounds(bounds, bounds.shape[0], q)
-    _i32(err, "err")
-    if blocks is None:
-        blocks = torch.empty(R, n_select, dtype=torch.int32, device=q.device)
-    if counts is None:
-        counts = torch.empty(R, dtype=torch.int32, device=q.device)
-    _i32(blocks, "blocks"), _i32(counts, "counts")
-    _need(tuple(blocks.shape) == (R, n_select) and counts.numel() >= R,
-          "blocks needs [rows, n_select] and counts an entry per row")
-    G = H // num_kv_heads
+    width = _cache_rows(block_table, heads_len, R)
+    n_pages = bounds.shape[0]
+    _bounds(bounds, n_pages, q.dtype)
+    _ints(err, "err", 1, "err needs an entry")
+    blocks, counts = _select_lists(q, bounds, R, n_select, sink, recent, blocks, counts)
+    L = lib()
     with _same_device(q, bounds, block_table, heads_len, err, blocks, counts):
-        ws = workspace.get(lib().hc_block_select_workspace_size(bsz, num_kv_heads, block_table.shape[1]))
-        rc = lib().hc_block_select(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), q.stride(0),
-                                   q.stride(1), bounds.data_ptr(), bounds.shape[0], block_table.data_ptr(),
-                                   block_table.shape[1], heads_len.data_ptr(), int(n_select), int(sink), int(recent),
-                                   blocks.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr(),
-                                   _stream(q))
-    check("hc_block_select", rc)
+        ws = workspace.get(L.hc_block_select_workspace_size(bsz, num_kv_heads, width))
+        qs = q.stride()
+        rc = L.hc_block_select(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1],
+                               bounds.data_ptr(), n_pages, block_table.data_ptr(), width, heads_len.data_ptr(),
+                               int(n_select), int(sink), int(recent), blocks.data_ptr(), counts.data_ptr(),
+                               ws.data_ptr(), ws.numel(), err.data_ptr(), _raw_stream(q))
+    if rc:
+        check("hc_block_select", rc)
     LAUNCHES[0] += 2
     return blocks, counts
 
@@ -564,19 +634,28 @@ def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, count
     """Decode attention over each row's listed 64-token blocks alone
     (hc_flash_decode_blocks): blocks [rows, n] int32 ascending, the first
     counts[row] of them used."""
-    out, bsz, G = _decode_operands(q, k_pool, v_pool, block_table, heads_len, num_kv_heads, out)
+    bsz, G = _decode_query(q, num_kv_heads, "decode attention")
+    n_pages = _pools(k_pool, v_pool, q.dtype)
     R = bsz * num_kv_heads
-    _i32(blocks, "blocks"), _i32(counts, "counts"), _i32(err, "err")
-    _need(blocks.dim() == 2 and blocks.shape[0] >= R and blocks.shape[1] >= 1 and counts.numel() >= R,
-          "blocks needs [rows, n] and counts an entry per row")
+    width = _cache_rows(block_table, heads_len, R)
+    out = _decode_out(out, q, bsz)
+    what = "blocks needs [rows, n] and counts an entry per row"
+    _ints(blocks, "blocks", 1, what)
+    _ints(counts, "counts", R, what)
+    _ints(err, "err", 1, "err needs an entry")
+    if blocks.dim() != 2 or blocks.shape[0] < R:
+        _refuse(what)
+    L = lib()
     with _same_device(q, k_pool, v_pool, block_table, heads_len, blocks, counts, out, err):
-        ws = workspace.get(lib().hc_flash_decode_workspace_size(bsz, num_kv_heads, G, HEAD_DIM))
-        rc = lib().hc_flash_decode_blocks(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), q.stride(0),
-                                          q.stride(1), k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0],
-                                          block_table.data_ptr(), block_table.shape[1], heads_len.data_ptr(),
-                                          blocks.data_ptr(), counts.data_ptr(), blocks.shape[1], float(scale),
-                                          out.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr(), _stream(q))
-    check("hc_flash_decode_blocks", rc)
+        ws = workspace.get(L.hc_flash_decode_workspace_size(bsz, num_kv_heads, G, HEAD_DIM))
+        qs = q.stride()
+        rc = L.hc_flash_decode_blocks(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1],
+                                      k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
+                                      heads_len.data_ptr(), blocks.data_ptr(), counts.data_ptr(), blocks.shape[1],
+                                      float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr(),
+                                      _raw_stream(q))
+    if rc:
+        check("hc_flash_decode_blocks", rc)
     LAUNCHES[0] += 2
     return out
 
@@ -584,12 +663,29 @@ def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, count
 def flash_decode_sparse(q, k_pool, v_pool, block_table, heads_len, bounds, *, num_kv_heads, n_select: int,
                         sink: int = 1, recent: int = 1, out=None, scale: float = 0.0, workspace: Workspace, err,
                         blocks=None, counts=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Block-sparse decode attention: ``block_select``, then ``flash_decode_blocks``
-    over what it lists.  Returns (out [bsz, H, D], blocks, counts)."""
-    blocks, counts = block_select(q, bounds, block_table, heads_len, num_kv_heads=num_kv_heads, n_select=n_select,
-                                  sink=sink, recent=recent, workspace=workspace, err=err, blocks=blocks, counts=counts)
-    out = flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, counts, num_kv_heads=num_kv_heads,
-                              out=out, scale=scale, workspace=workspace, err=err)
+    """Block-sparse decode attention (hc_flash_decode_sparse): what
+    ``block_select`` and then ``flash_decode_blocks`` over its lists give.
+    Returns (out [bsz, H, D], blocks [rows, n_select], counts [rows])."""
+    bsz, G = _decode_query(q, num_kv_heads, "decode attention")
+    n_pages = _pools(k_pool, v_pool, q.dtype)
+    R = bsz * num_kv_heads
+    width = _cache_rows(block_table, heads_len, R)
+    out = _decode_out(out, q, bsz)
+    _bounds(bounds, n_pages, q.dtype)
+    _ints(err, "err", 1, "err needs an entry")
+    blocks, counts = _select_lists(q, bounds, R, n_select, sink, recent, blocks, counts)
+    L = lib()
+    with _same_device(q, k_pool, v_pool, block_table, heads_len, bounds, blocks, counts, out, err):
+        ws = workspace.get(L.hc_flash_decode_sparse_workspace_size(bsz, num_kv_heads, G, HEAD_DIM, width))
+        qs = q.stride()
+        rc = L.hc_flash_decode_sparse(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1],
+                                      k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
+                                      heads_len.data_ptr(), bounds.data_ptr(), int(n_select), int(sink), int(recent),
+                                      float(scale), out.data_ptr(), blocks.data_ptr(), counts.data_ptr(),
+                                      ws.data_ptr(), ws.numel(), err.data_ptr(), _raw_stream(q))
+    if rc:
+        check("hc_flash_decode_sparse", rc)
+    LAUNCHES[0] += 4
     return out, blocks, counts
 
 

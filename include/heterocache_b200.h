@@ -298,6 +298,9 @@ int hc_rope_append(int dtype, int trig_dtype, int bsz, int num_heads, int num_kv
  *
  * hc_flash_decode_blocks: hc_flash_decode over the listed blocks of each row
  * alone (a row with none gives zeros); workspace as hc_flash_decode's.
+ *
+ * hc_flash_decode_sparse: the selection, then the attention over what it
+ * lists, in one call.
  */
 #define HC_SPARSE_BLOCK 64
 int hc_block_bounds(int dtype, int rows_total, int head_dim, const void* k_pool, int n_pool_blocks,
@@ -313,6 +316,13 @@ int hc_flash_decode_blocks(int dtype, int bsz, int num_kv_heads, int groups, int
                            const int32_t* block_table, int max_blocks, const int32_t* heads_len,
                            const int32_t* blocks, const int32_t* counts, int n_select, float scale, void* out,
                            void* workspace, size_t workspace_bytes, int32_t* err_flag, void* stream);
+size_t hc_flash_decode_sparse_workspace_size(int bsz, int num_kv_heads, int groups, int head_dim, int max_blocks);
+int hc_flash_decode_sparse(int dtype, int bsz, int num_kv_heads, int groups, int head_dim, const void* q, int64_t qsb,
+                           int64_t qsh, const void* k_pool, const void* v_pool, int n_pool_blocks,
+                           const int32_t* block_table, int max_blocks, const int32_t* heads_len, const void* bounds,
+                           int n_select, int sink, int recent, float scale, void* out, int32_t* blocks,
+                           int32_t* counts, void* workspace, size_t workspace_bytes, int32_t* err_flag,
+                           void* stream);
 
 /* ---------------------------------------------------------------------------
  * Decode attention of a batch that shares a long prefix: continuations of
