@@ -10,6 +10,8 @@
 // on the order of a 32-bit sum, and the products of 16-bit values and their
 // sums are then exact for all but extreme exponents.  A score that is not a
 // number counts as the highest, so that NaN keys are attended to, not hidden.
+#include <algorithm>
+
 #include "hc_host.cuh"
 #include "hc_params.cuh"
 
@@ -96,7 +98,7 @@ int block_bounds_dispatch(int dtype, const BBParams& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// Scores.  A warp takes 16 blocks, two for each 4 lanes: lane p of the four
+// Scores.  A warp takes 8 kHand blocks, kHand for each 4 lanes: lane p of them
 // holds the 16-byte chunks p, p + 4, .. of the blocks' least and greatest
 // keys (a load of the warp is eight 64-byte pieces), as 64-bit values, and
 // multiplies them with the query heads, which lie in shared memory split into
@@ -108,10 +110,10 @@ int block_bounds_dispatch(int dtype, const BBParams& p, cudaStream_t st) {
 // The queries' layout puts the four lanes' values side by side: with [dim]
 // rows the four read the same banks, which took 130 us at 128 rows x 820
 // blocks (80% of the shared-memory pipe, the 64-bit units at 6%).
-constexpr int kBsThreads = 256;
+constexpr int kBsThreads = 128;
 constexpr int kBsWarps = kBsThreads / 32;
-constexpr int kBsTwo = 2;                           // blocks a lane has in hand
-constexpr int kBsCta = kBsWarps * 8 * kBsTwo;       // blocks of a CTA
+// Blocks of a CTA whose lanes have kHand of them in hand.
+__host__ __device__ constexpr int bs_cta(int hand) { return kBsWarps * 8 * hand; }
 
 // Blocks of a row, its length clamped to the page table.
 __device__ __forceinline__ int bs_blocks(const BSParams& p, int r) {
@@ -159,10 +161,11 @@ __device__ __noinline__ double bs_plain_score(const BSParams& p, int r, const T*
   return best;
 }
 
-template <typename T, int kG>
-__global__ void __launch_bounds__(kBsThreads, 2) block_score_kernel(const BSParams p) {
+template <typename T, int kG, int kHand>
+__global__ void __launch_bounds__(kBsThreads, 4) block_score_kernel(const BSParams p) {
+  constexpr int kBsCta = bs_cta(kHand);
   constexpr int E = 16 / (int)sizeof(T), CH = kD / E, MINE = CH / 4;  // chunks of a row, of a lane
-  constexpr int STEP = MINE < 4 ? MINE : 4;                           // chunks loaded at a time
+  constexpr int STEP = 8 / kHand;                                     // chunks loaded at a time
   constexpr int GP = (kG + 1) / 2;                                    // pairs of heads
   // [lane's chunk][element][sign][head pair][lane of the four] of two heads
   extern __shared__ __align__(16) double2 s_q[];
@@ -188,13 +191,13 @@ __global__ void __launch_bounds__(kBsThreads, 2) block_score_kernel(const BSPara
   double* scores = p.scores + (int64_t)r * p.max_blocks * kBlkPerPage;
 #pragma unroll 1
   for (int first = blockIdx.x * kBsCta; first < n; first += gridDim.x * kBsCta) {
-    if (first + warp * kBsTwo * 8 >= n) break;
-    const T* lim[kBsTwo];
-    int blk[kBsTwo];
-    bool ok[kBsTwo];
+    if (first + warp * kHand * 8 >= n) break;
+    const T* lim[kHand];
+    int blk[kHand];
+    bool ok[kHand];
 #pragma unroll
-    for (int t = 0; t < kBsTwo; ++t) {
-      blk[t] = first + (warp * kBsTwo + t) * 8 + (lane >> 2);
+    for (int t = 0; t < kHand; ++t) {
+      blk[t] = first + (warp * kHand + t) * 8 + (lane >> 2);
       int phys = blk[t] < n ? p.bt[(int64_t)r * p.max_blocks + blk[t] / kBlkPerPage] : -1;
       ok[t] = phys >= 0 && phys < p.n_blocks;
       if (blk[t] < n && !ok[t] && part == 0) set_err(p.err, HC_ERR_RANGE);
@@ -202,16 +205,16 @@ __global__ void __launch_bounds__(kBsThreads, 2) block_score_kernel(const BSPara
       lim[t] = reinterpret_cast<const T*>(p.bounds) +
                ((int64_t)phys * kBlkPerPage + (blk[t] & (kBlkPerPage - 1))) * 2 * kD;
     }
-    double acc[kBsTwo][2 * GP];
+    double acc[kHand][2 * GP];
 #pragma unroll
-    for (int t = 0; t < kBsTwo; ++t)
+    for (int t = 0; t < kHand; ++t)
 #pragma unroll
       for (int g = 0; g < 2 * GP; ++g) acc[t][g] = 0.0;
 #pragma unroll
     for (int c0 = 0; c0 < MINE; c0 += STEP) {
-      uint4 wl[kBsTwo][STEP], wh[kBsTwo][STEP];
+      uint4 wl[kHand][STEP], wh[kHand][STEP];
 #pragma unroll
-      for (int t = 0; t < kBsTwo; ++t)
+      for (int t = 0; t < kHand; ++t)
 #pragma unroll
         for (int c = 0; c < STEP; ++c) {
           wl[t][c] = wh[t][c] = make_uint4(0u, 0u, 0u, 0u);
@@ -222,17 +225,17 @@ __global__ void __launch_bounds__(kBsThreads, 2) block_score_kernel(const BSPara
         }
 #pragma unroll
       for (int c = 0; c < STEP; ++c) {
-        float lo[kBsTwo][E], hi[kBsTwo][E];
+        float lo[kHand][E], hi[kHand][E];
 #pragma unroll
-        for (int t = 0; t < kBsTwo; ++t) {
+        for (int t = 0; t < kHand; ++t) {
           bs_unpack<T, E>(wl[t][c], lo[t]);
           bs_unpack<T, E>(wh[t][c], hi[t]);
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          double x[kBsTwo], y[kBsTwo];
+          double x[kHand], y[kHand];
 #pragma unroll
-          for (int t = 0; t < kBsTwo; ++t) {
+          for (int t = 0; t < kHand; ++t) {
             x[t] = bb_max(lo[t][e], hi[t][e]);
             y[t] = bb_min(lo[t][e], hi[t][e]);
           }
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kBsThreads, 2) block_score_kernel(const BSPara
           for (int g = 0; g < GP; ++g) {
             const double2 up = q[g * 4], down = q[(GP + g) * 4];
 #pragma unroll
-            for (int t = 0; t < kBsTwo; ++t) {
+            for (int t = 0; t < kHand; ++t) {
               acc[t][2 * g] = fma(down.x, y[t], fma(up.x, x[t], acc[t][2 * g]));
               acc[t][2 * g + 1] = fma(down.y, y[t], fma(up.y, x[t], acc[t][2 * g + 1]));
             }
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(kBsThreads, 2) block_score_kernel(const BSPara
       }
     }
 #pragma unroll
-    for (int t = 0; t < kBsTwo; ++t) {
+    for (int t = 0; t < kHand; ++t) {
       double best = -INFINITY;
       bool odd = false;
 #pragma unroll
@@ -408,20 +411,20 @@ size_t block_select_ws_bytes(int R, int max_blocks) {
   return (size_t)R * max_blocks * kBlkPerPage * sizeof(double) + 256;
 }
 
-template <typename T, int kG>
-static cudaError_t bs_launch_scores(const BSParams& p, cudaLaunchConfig_t& cfg) {
+template <typename T, int kG, int kHand>
+static cudaError_t bs_launch_scores(const BSParams& p, cudaLaunchConfig_t& cfg, int sms) {
+  // CTAs of a row: no more than fit on the SMs at a time (4 each), so that
+  // none waits for a second turn
+  const int tiles = (p.max_blocks * kBlkPerPage + bs_cta(kHand) - 1) / bs_cta(kHand);
+  cfg.gridDim = dim3((unsigned int)std::min(tiles, std::max(1, 4 * sms / p.R)), (unsigned int)p.R);
   cfg.dynamicSmemBytes = (size_t)kD * 2 * ((kG + 1) / 2) * sizeof(double2);
-  return cudaLaunchKernelEx(&cfg, block_score_kernel<T, kG>, p);
+  return cudaLaunchKernelEx(&cfg, block_score_kernel<T, kG, kHand>, p);
 }
 
 template <typename T>
 static int bs_launch(BSParams& p, cudaStream_t st) {
+  const int sms = device_sms(current_device());
   cudaLaunchConfig_t cfg = {};
-  // CTAs of a row: enough for every SM to have its two; more would only load
-  // the queries more often
-  const int tiles = (p.max_blocks * kBlkPerPage + kBsCta - 1) / kBsCta;
-  const int want = (2 * device_sms(current_device()) + p.R - 1) / p.R;
-  cfg.gridDim = dim3((unsigned int)(tiles < want ? tiles : want), (unsigned int)p.R);
   cfg.blockDim = dim3(kBsThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -429,8 +432,16 @@ static int bs_launch(BSParams& p, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = p.G <= 1 ? bs_launch_scores<T, 1>(p, cfg) : p.G <= 2 ? bs_launch_scores<T, 2>(p, cfg)
-                        : p.G <= 4 ? bs_launch_scores<T, 4>(p, cfg) : bs_launch_scores<T, 8>(p, cfg);
+  // Four blocks a lane read the queries from shared memory half as often as
+  // two; two make twice the CTAs, for few rows.  (Bounds of 128 rows x 820
+  // blocks: 28 us with four, 37 with two; 8 rows x 1640: 11 and 9.)  More
+  // than four heads leave registers for two.
+  const bool four = (int64_t)p.R * p.max_blocks * kBlkPerPage >= (int64_t)2 * sms * bs_cta(4);
+  cudaError_t e;
+  if (p.G > 4) e = bs_launch_scores<T, 8, 2>(p, cfg, sms);
+  else if (p.G > 2) e = four ? bs_launch_scores<T, 4, 4>(p, cfg, sms) : bs_launch_scores<T, 4, 2>(p, cfg, sms);
+  else if (p.G > 1) e = four ? bs_launch_scores<T, 2, 4>(p, cfg, sms) : bs_launch_scores<T, 2, 2>(p, cfg, sms);
+  else e = four ? bs_launch_scores<T, 1, 4>(p, cfg, sms) : bs_launch_scores<T, 1, 2>(p, cfg, sms);
   if (e != cudaSuccess) return HC_ERR_CUDA;
   cfg.gridDim = dim3((unsigned int)p.R);
   cfg.blockDim = dim3(kSelThreads);
