@@ -255,7 +255,7 @@ struct RAParams {
   void* bounds;  // block bounds to keep up to date, or null
   unsigned int* done;  // zero before and after a launch
   int B, H, KV, T;
-  int units, kv_ctas;  // 64-token blocks a row may touch; key/value CTAs (set at launch)
+  int units, run, kv_ctas;  // 64-token blocks a row may touch, a CTA's; key/value CTAs (set at launch)
   int32_t* err;
 };
 int rope_append_dispatch(int dtype, RAParams& p, cudaStream_t st);

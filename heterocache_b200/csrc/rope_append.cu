@@ -15,9 +15,12 @@
 // Work is split into units of one aligned 64-token block of one row (so a
 // block's bounds are reduced inside one CTA, without atomics) and into query
 // units of 32 tokens x up to 4 heads (the cosines and sines are loaded once
-// for the 4 heads).  Every key/value CTA derives the page allocation for
+// for the 4 heads).  Registers are kept to three CTAs an SM, two tokens (four
+// heads) of a thread in flight: 16 x 4096 tokens of 32 + 8 heads, 1.36 GB,
+// take 238 us (88% of the copy rate; with fp32 minima and one token in
+// flight at 111 registers, 441 us).  Every key/value CTA derives the page allocation for
 // itself from the state the call found; the last of them to finish (a
-// counter in the workspace) writes the page table, the lengths and the
+// counter) writes the page table, the lengths and the
 // free-list pointer, so nothing is written while another CTA still reads.
 #include "hc_host.cuh"
 #include "hc_params.cuh"
@@ -33,6 +36,8 @@ template <typename T> struct RaRow {
   static constexpr int CH2 = kD / 2 / E;            // chunks of half a row
 };
 
+// Least / greatest of two values, or of two 16-bit pairs at a time; NaN if
+// either is.
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
@@ -43,6 +48,42 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+template <typename T> struct Word;  // 32 bits of T
+template <> struct Word<float> {
+  __device__ __forceinline__ static uint32_t min(uint32_t a, uint32_t b) {
+    return __float_as_uint(min_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
+  __device__ __forceinline__ static uint32_t max(uint32_t a, uint32_t b) {
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static constexpr uint32_t kInf = 0x7f800000u, kNegInf = 0xff800000u;
+};
+template <> struct Word<__nv_bfloat16> {
+  __device__ __forceinline__ static uint32_t min(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ static uint32_t max(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static constexpr uint32_t kInf = 0x7f807f80u, kNegInf = 0xff80ff80u;
+};
+template <> struct Word<__half> {
+  __device__ __forceinline__ static uint32_t min(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ static uint32_t max(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static constexpr uint32_t kInf = 0x7c007c00u, kNegInf = 0xfc00fc00u;
+};
 
 template <typename T, int E>
 __device__ __forceinline__ void unpack_chunk(const uint4& w, float (&f)[E]) {
@@ -70,44 +111,51 @@ __device__ __forceinline__ uint4 pack_chunk(const float (&f)[E]) {
                       Elem<T>::cvt2(f[6], f[7]));
   }
 }
-// E elements of a cosine / sine row: in the cache type or in fp32
-template <typename T, int E>
-__device__ __forceinline__ void load_trig(const void* base, int64_t off, bool f32, float (&f)[E]) {
-  if (sizeof(T) != 4 && f32) {
-    const float* p = reinterpret_cast<const float*>(base) + off;
-#pragma unroll
-    for (int i = 0; i < E; i += 4) {
-      const uint4 w = ldg128(p + i);
-      f[i] = __uint_as_float(w.x);
-      f[i + 1] = __uint_as_float(w.y);
-      f[i + 2] = __uint_as_float(w.z);
-      f[i + 3] = __uint_as_float(w.w);
-    }
-  } else {
-    unpack_chunk<T, E>(ldg128(reinterpret_cast<const T*>(base) + off), f);
-  }
-}
-
-// The rotation's factors for one chunk of each half.
-template <int E> struct Trig {
-  float c1[E], s1[E], c2[E], s2[E];
+// The rotation's factors for one chunk of each half, as loaded: of type TT,
+// the cache's or fp32.
+template <typename TT, int E> struct Trig {
+  static constexpr int N = E * (int)sizeof(TT) / 16;
+  uint4 c1[N], s1[N], c2[N], s2[N];
 };
-template <typename T, int E>
-__device__ __forceinline__ void load_rotation(const RAParams& p, int b, int t, int d0, Trig<E>& g) {
-  const int64_t c = b * p.csb + t * p.cst + d0, s = b * p.ssb + t * p.sst + d0;
-  load_trig<T, E>(p.cos, c, p.trig_f32, g.c1);
-  load_trig<T, E>(p.cos, c + kD / 2, p.trig_f32, g.c2);
-  load_trig<T, E>(p.sin, s, p.trig_f32, g.s1);
-  load_trig<T, E>(p.sin, s + kD / 2, p.trig_f32, g.s2);
-}
-template <int E>
-__device__ __forceinline__ void rotate(const Trig<E>& g, float (&x1)[E], float (&x2)[E]) {
+template <typename TT, int E>
+__device__ __forceinline__ void load_rotation(const RAParams& p, int b, int t, int d0, Trig<TT, E>& g) {
+  const TT* c = reinterpret_cast<const TT*>(p.cos) + b * p.csb + t * p.cst + d0;
+  const TT* s = reinterpret_cast<const TT*>(p.sin) + b * p.ssb + t * p.sst + d0;
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const float a = x1[i], z = x2[i];
-    x1[i] = fmaf(a, g.c1[i], -(z * g.s1[i]));
-    x2[i] = fmaf(z, g.c2[i], a * g.s2[i]);
+  for (int i = 0; i < Trig<TT, E>::N; ++i) {
+    g.c1[i] = ldg128(reinterpret_cast<const uint4*>(c) + i);
+    g.s1[i] = ldg128(reinterpret_cast<const uint4*>(s) + i);
+    g.c2[i] = ldg128(reinterpret_cast<const uint4*>(c + kD / 2) + i);
+    g.s2[i] = ldg128(reinterpret_cast<const uint4*>(s + kD / 2) + i);
   }
+}
+template <typename TT, int E>
+__device__ __forceinline__ void unpack_trig(const uint4 (&w)[Trig<TT, E>::N], float (&f)[E]) {
+  constexpr int PER = 16 / (int)sizeof(TT);
+#pragma unroll
+  for (int i = 0; i < Trig<TT, E>::N; ++i) {
+    float part[PER];
+    unpack_chunk<TT, PER>(w[i], part);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) f[i * PER + j] = part[j];
+  }
+}
+// y1 = x1 c1 - x2 s1, y2 = x2 c2 + x1 s2: two roundings in fp32, then one to T.
+template <typename T, typename TT, int E>
+__device__ __forceinline__ void rotate(const Trig<TT, E>& g, uint4& w1, uint4& w2) {
+  float x1[E], x2[E], c[E], s[E], y[E];
+  unpack_chunk<T, E>(w1, x1);
+  unpack_chunk<T, E>(w2, x2);
+  unpack_trig<TT, E>(g.c1, c);
+  unpack_trig<TT, E>(g.s1, s);
+#pragma unroll
+  for (int i = 0; i < E; ++i) y[i] = fmaf(x1[i], c[i], -(x2[i] * s[i]));
+  w1 = pack_chunk<T, E>(y);
+  unpack_trig<TT, E>(g.c2, c);
+  unpack_trig<TT, E>(g.s2, s);
+#pragma unroll
+  for (int i = 0; i < E; ++i) y[i] = fmaf(x2[i], c[i], x1[i] * s[i]);
+  w2 = pack_chunk<T, E>(y);
 }
 
 __device__ __forceinline__ int ra_count(const RAParams& p, int b) {
@@ -236,7 +284,7 @@ __device__ __forceinline__ void ra_finish(const RAParams& p, int status, int bas
 }
 
 // Rotated queries: 32 tokens (of all sequences, end to end) x kRaHeads heads.
-template <typename T>
+template <typename T, typename TT>
 __device__ __forceinline__ void ra_query_unit(const RAParams& p, int unit) {
   constexpr int E = RaRow<T>::E, CH2 = RaRow<T>::CH2, TOK = kRaThreads / CH2;
   const int nh = (p.H + kRaHeads - 1) / kRaHeads;
@@ -256,25 +304,25 @@ __device__ __forceinline__ void ra_query_unit(const RAParams& p, int unit) {
       w1[i] = *reinterpret_cast<const uint4*>(src + (h0 + i) * p.qsh);
       w2[i] = *reinterpret_cast<const uint4*>(src + (h0 + i) * p.qsh + kD / 2);
     }
-  Trig<E> g;
-  load_rotation<T, E>(p, b, t, d0, g);
+  Trig<TT, E> g;
+  load_rotation<TT, E>(p, b, t, d0, g);
 #pragma unroll
   for (int i = 0; i < kRaHeads; ++i)
     if (h0 + i < p.H) {
-      float x1[E], x2[E];
-      unpack_chunk<T, E>(w1[i], x1);
-      unpack_chunk<T, E>(w2[i], x2);
-      rotate<E>(g, x1, x2);
-      *reinterpret_cast<uint4*>(dst + (h0 + i) * p.osh) = pack_chunk<T, E>(x1);
-      *reinterpret_cast<uint4*>(dst + (h0 + i) * p.osh + kD / 2) = pack_chunk<T, E>(x2);
+      rotate<T, TT, E>(g, w1[i], w2[i]);
+      *reinterpret_cast<uint4*>(dst + (h0 + i) * p.osh) = w1[i];
+      *reinterpret_cast<uint4*>(dst + (h0 + i) * p.osh + kD / 2) = w2[i];
     }
 }
 
 // One aligned 64-token block of one row: threads c < CH2 of a token take
-// chunk c of both halves of the key, the other CH2 those of the value.
-template <typename T>
-__device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int cnt, int blk, int take, float* s_mm) {
+// chunk c of both halves of the key, the other CH2 those of the value; two
+// tokens a thread are in flight.
+template <typename T, typename TT>
+__device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int cnt, int blk, int take,
+                                         uint32_t* s_mm) {
   constexpr int E = RaRow<T>::E, CH2 = RaRow<T>::CH2, PER = 2 * CH2, TOK = kRaThreads / PER;
+  constexpr int RW = kD * (int)sizeof(T) / 4;  // 32-bit words of a row
   const int b = r / p.KV, h = r % p.KV;
   const int beg = max(blk * HC_SPARSE_BLOCK, len), end = min((blk + 1) * HC_SPARSE_BLOCK, len + cnt);
   const int phys = ra_page(p, r, len, beg >> 8, take);
@@ -285,39 +333,42 @@ __device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int 
                      : reinterpret_cast<const T*>(p.v) + b * p.vsb + h * p.vsh + d0;
   const int64_t sst = key ? p.kst : p.vst;
   T* pool = reinterpret_cast<T*>(key ? p.kp : p.vp) + (int64_t)phys * kPage * kD + d0;
-  float mn1[E], mn2[E], mx1[E], mx2[E];
+  uint32_t mn[8], mx[8];  // of the two chunks
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    mn1[i] = mn2[i] = INFINITY;
-    mx1[i] = mx2[i] = -INFINITY;
+  for (int i = 0; i < 8; ++i) {
+    mn[i] = Word<T>::kInf;
+    mx[i] = Word<T>::kNegInf;
   }
-  for (int pos = beg + (int)threadIdx.x / PER; pos < end; pos += TOK) {
-    const int t = pos - len;
-    uint4 w1 = ldg128(src + t * sst), w2 = ldg128(src + t * sst + kD / 2);
-    if (key) {
-      Trig<E> g;
-      load_rotation<T, E>(p, b, t, d0, g);
-      float x1[E], x2[E];
-      unpack_chunk<T, E>(w1, x1);
-      unpack_chunk<T, E>(w2, x2);
-      rotate<E>(g, x1, x2);
-      w1 = pack_chunk<T, E>(x1);
-      w2 = pack_chunk<T, E>(x2);
-      if (p.bounds) {  // of the rounded keys: what the pages hold
-        unpack_chunk<T, E>(w1, x1);
-        unpack_chunk<T, E>(w2, x2);
+  for (int pos0 = beg + (int)threadIdx.x / PER; pos0 < end; pos0 += 2 * TOK) {
+    uint4 w1[2], w2[2];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          mn1[i] = min_nan(mn1[i], x1[i]);
-          mn2[i] = min_nan(mn2[i], x2[i]);
-          mx1[i] = max_nan(mx1[i], x1[i]);
-          mx2[i] = max_nan(mx2[i], x2[i]);
+    for (int u = 0; u < 2; ++u)
+      if (pos0 + u * TOK < end) {
+        const T* x = src + (pos0 + u * TOK - len) * sst;
+        w1[u] = ldg128(x);
+        w2[u] = ldg128(x + kD / 2);
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int pos = pos0 + u * TOK;
+      if (pos >= end) continue;
+      if (key) {
+        Trig<TT, E> g;
+        load_rotation<TT, E>(p, b, pos - len, d0, g);
+        rotate<T, TT, E>(g, w1[u], w2[u]);
+        if (p.bounds) {  // of the rounded keys: what the pages hold
+          const uint32_t x[8] = {w1[u].x, w1[u].y, w1[u].z, w1[u].w, w2[u].x, w2[u].y, w2[u].z, w2[u].w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            mn[i] = Word<T>::min(mn[i], x[i]);
+            mx[i] = Word<T>::max(mx[i], x[i]);
+          }
         }
       }
+      T* dst = pool + (int64_t)(pos & (kPage - 1)) * kD;
+      *reinterpret_cast<uint4*>(dst) = w1[u];
+      *reinterpret_cast<uint4*>(dst + kD / 2) = w2[u];
     }
-    T* dst = pool + (int64_t)(pos & (kPage - 1)) * kD;
-    *reinterpret_cast<uint4*>(dst) = w1;
-    *reinterpret_cast<uint4*>(dst + kD / 2) = w2;
   }
   if (!p.bounds) return;
   // over the tokens of a warp (lanes PER apart), then over the warps
@@ -325,67 +376,134 @@ __device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int 
 #pragma unroll
   for (int o = PER; o < 32; o <<= 1)
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      mn1[i] = min_nan(mn1[i], __shfl_xor_sync(0xffffffffu, mn1[i], o));
-      mn2[i] = min_nan(mn2[i], __shfl_xor_sync(0xffffffffu, mn2[i], o));
-      mx1[i] = max_nan(mx1[i], __shfl_xor_sync(0xffffffffu, mx1[i], o));
-      mx2[i] = max_nan(mx2[i], __shfl_xor_sync(0xffffffffu, mx2[i], o));
+    for (int i = 0; i < 8; ++i) {
+      mn[i] = Word<T>::min(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
+      mx[i] = Word<T>::max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
     }
   __syncthreads();
   if (lane < CH2) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      s_mm[(warp * 2) * kD + d0 + i] = mn1[i];
-      s_mm[(warp * 2) * kD + kD / 2 + d0 + i] = mn2[i];
-      s_mm[(warp * 2 + 1) * kD + d0 + i] = mx1[i];
-      s_mm[(warp * 2 + 1) * kD + kD / 2 + d0 + i] = mx2[i];
+    for (int i = 0; i < 4; ++i) {
+      s_mm[(warp * 2) * RW + lane * 4 + i] = mn[i];
+      s_mm[(warp * 2) * RW + RW / 2 + lane * 4 + i] = mn[4 + i];
+      s_mm[(warp * 2 + 1) * RW + lane * 4 + i] = mx[i];
+      s_mm[(warp * 2 + 1) * RW + RW / 2 + lane * 4 + i] = mx[4 + i];
     }
   }
   __syncthreads();
-  const int which = threadIdx.x / kD, d = threadIdx.x % kD;  // 0: min, 1: max
-  T* out = reinterpret_cast<T*>(p.bounds) + (((int64_t)phys * (kPage / HC_SPARSE_BLOCK) + (blk & 3)) * 2 + which) * kD + d;
-  float x = s_mm[which * kD + d];
+  const int which = threadIdx.x / RW, d = threadIdx.x % RW;  // 0: least, 1: greatest
+  if (which > 1) return;
+  uint32_t* out = reinterpret_cast<uint32_t*>(p.bounds) +
+                  (((int64_t)phys * (kPage / HC_SPARSE_BLOCK) + (blk & (kPage / HC_SPARSE_BLOCK - 1))) * 2 + which) * RW +
+                  d;
+  uint32_t x = s_mm[which * RW + d];
 #pragma unroll
   for (int w = 1; w < kRaWarps; ++w) {
-    const float y = s_mm[(w * 2 + which) * kD + d];
-    x = which ? max_nan(x, y) : min_nan(x, y);
+    const uint32_t y = s_mm[(w * 2 + which) * RW + d];
+    x = which ? Word<T>::max(x, y) : Word<T>::min(x, y);
   }
   if (blk * HC_SPARSE_BLOCK < len) {  // the block held tokens before
-    const float y = Elem<T>::to_f(*out);
-    x = which ? max_nan(x, y) : min_nan(x, y);
+    const uint32_t y = *out;
+    x = which ? Word<T>::max(x, y) : Word<T>::min(x, y);
   }
-  *out = Elem<T>::from_f(x);
+  *out = x;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRaThreads) rope_append_kernel(const RAParams p) {
+__host__ __device__ constexpr int ra_rows() {
+  return kRaThreads / (2 * RaRow<T>::CH2);
+}
+
+// One token a sequence: a row's token takes as many threads as a token of
+// ra_block, and a CTA a run of rows from r0 on (16 of a 16-bit cache), so
+// that few CTAs go through all rows for the allocation.  `take`: the free
+// list's index of row r0's first free page.
+template <typename T, typename TT>
+__device__ __forceinline__ void ra_token(const RAParams& p, int r0, int take) {
+  constexpr int E = RaRow<T>::E, CH2 = RaRow<T>::CH2, PER = 2 * CH2;
+  constexpr int RW = kD * (int)sizeof(T) / 4;
+  const int r = r0 + (int)threadIdx.x / PER;
+  if (r >= p.B * p.KV) return;
+  const int b = r / p.KV, h = r % p.KV;
+  if (ra_count(p, b) == 0) return;
+  const int pos = p.heads_len[r];
+  int phys = p.bt[(int64_t)r * p.max_blocks + (pos >> 8)];
+  if (phys == -1) {
+    bool bad = false;
+    for (int k = r0; k < r; ++k) take += ra_need(p, k, bad);
+    phys = p.free_blocks[take];
+  }
+  const int c = threadIdx.x % PER;
+  const bool key = c < CH2;
+  const int d0 = (key ? c : c - CH2) * E;
+  const T* src = key ? reinterpret_cast<const T*>(p.k) + b * p.ksb + h * p.ksh + d0
+                     : reinterpret_cast<const T*>(p.v) + b * p.vsb + h * p.vsh + d0;
+  uint4 w1 = ldg128(src), w2 = ldg128(src + kD / 2);
+  if (key) {
+    Trig<TT, E> g;
+    load_rotation<TT, E>(p, b, 0, d0, g);
+    rotate<T, TT, E>(g, w1, w2);
+  }
+  T* dst = reinterpret_cast<T*>(key ? p.kp : p.vp) + ((int64_t)phys * kPage + (pos & (kPage - 1))) * kD + d0;
+  *reinterpret_cast<uint4*>(dst) = w1;
+  *reinterpret_cast<uint4*>(dst + kD / 2) = w2;
+  if (!key || !p.bounds) return;
+  uint32_t* lim = reinterpret_cast<uint32_t*>(p.bounds) +
+                  ((int64_t)phys * (kPage / HC_SPARSE_BLOCK) + ((pos & (kPage - 1)) / HC_SPARSE_BLOCK)) * 2 * RW + c * 4;
+  const bool more = (pos & (HC_SPARSE_BLOCK - 1)) != 0;  // the block held tokens before
+  auto merge = [&](uint32_t* at, const uint4& w) {
+    uint4 lo = w, hi = w;
+    if (more) {
+      const uint4 a = *reinterpret_cast<const uint4*>(at), z = *reinterpret_cast<const uint4*>(at + RW);
+      lo = make_uint4(Word<T>::min(a.x, w.x), Word<T>::min(a.y, w.y), Word<T>::min(a.z, w.z), Word<T>::min(a.w, w.w));
+      hi = make_uint4(Word<T>::max(z.x, w.x), Word<T>::max(z.y, w.y), Word<T>::max(z.z, w.z), Word<T>::max(z.w, w.w));
+    }
+    *reinterpret_cast<uint4*>(at) = lo;
+    *reinterpret_cast<uint4*>(at + RW) = hi;
+  };
+  merge(lim, w1);
+  merge(lim + RW / 2, w2);
+}
+
+template <typename T, typename TT>
+__global__ void __launch_bounds__(kRaThreads, 3) rope_append_kernel(const RAParams p) {
   __shared__ int2 s_red[kRaWarps];
   __shared__ int s_warp[32];
-  __shared__ float s_mm[kRaWarps * 2 * kD];
+  __shared__ uint32_t s_mm[kRaWarps * 2 * kD * sizeof(T) / 4];
   pdl_wait();
   pdl_trigger();
   if ((int)blockIdx.x >= p.kv_ctas) {
-    ra_query_unit<T>(p, (int)blockIdx.x - p.kv_ctas);
+    ra_query_unit<T, TT>(p, (int)blockIdx.x - p.kv_ctas);
     return;
   }
-  const int r = blockIdx.x / p.units, u = blockIdx.x % p.units;
+  const int per_row = (p.units + p.run - 1) / p.run;
+  const bool single = p.T == 1;
+  const int r = single ? (int)blockIdx.x * ra_rows<T>() : (int)blockIdx.x / per_row;
+  const int u0 = (blockIdx.x % per_row) * p.run;
   const int base = *p.free_ptr;
   int before, total;
   const int status = ra_plan(p, r, base, s_red, before, total);
-  if (!status) {
+  if (!status && single) {
+    ra_token<T, TT>(p, r, base + before);
+  } else if (!status) {
     const int len = p.heads_len[r], cnt = ra_count(p, r / p.KV);
-    const int blk = len / HC_SPARSE_BLOCK + u;
-    if (cnt > 0 && blk * HC_SPARSE_BLOCK < len + cnt) ra_block<T>(p, r, len, cnt, blk, base + before, s_mm);
+    for (int u = u0; u < min(u0 + p.run, p.units); ++u) {
+      const int blk = len / HC_SPARSE_BLOCK + u;
+      if (cnt > 0 && blk * HC_SPARSE_BLOCK < len + cnt) ra_block<T, TT>(p, r, len, cnt, blk, base + before, s_mm);
+    }
   }
   ra_finish(p, status, base, total, s_warp);
 }
 
-template <typename T>
+template <typename T, typename TT>
 static int ra_launch(RAParams& p, cudaStream_t st) {
   constexpr int TOK = kRaThreads / RaRow<T>::CH2;
   const int64_t R = (int64_t)p.B * p.KV;
   p.units = (p.T + HC_SPARSE_BLOCK - 2) / HC_SPARSE_BLOCK + 1;  // blocks that T tokens can touch
-  const int64_t kv = R * p.units;
+  // a CTA finds the allocation once for a run of 4 blocks, where there are
+  // still CTAs enough to fill the GPU
+  p.run = R * p.units >= 4 * 8 * (int64_t)device_sms(current_device()) ? 4 : 1;
+  const int64_t kv = p.T == 1 ? (R + ra_rows<T>() - 1) / ra_rows<T>() : R * ((p.units + p.run - 1) / p.run);
   const int64_t q = (((int64_t)p.B * p.T + TOK - 1) / TOK) * ((p.H + kRaHeads - 1) / kRaHeads);
   if (kv + q > 0x7fffffffLL) return HC_ERR_UNSUPPORTED;
   p.kv_ctas = (int)kv;
@@ -398,14 +516,15 @@ static int ra_launch(RAParams& p, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, rope_append_kernel<T>, (const RAParams)p) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, rope_append_kernel<T, TT>, (const RAParams)p) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
 }
 
 int rope_append_dispatch(int dtype, RAParams& p, cudaStream_t st) {
   switch (dtype) {
-    case HC_F32: return ra_launch<float>(p, st);
-    case HC_BF16: return ra_launch<__nv_bfloat16>(p, st);
-    case HC_F16: return ra_launch<__half>(p, st);
+    case HC_F32: return ra_launch<float, float>(p, st);
+    case HC_BF16:
+      return p.trig_f32 ? ra_launch<__nv_bfloat16, float>(p, st) : ra_launch<__nv_bfloat16, __nv_bfloat16>(p, st);
+    case HC_F16: return p.trig_f32 ? ra_launch<__half, float>(p, st) : ra_launch<__half, __half>(p, st);
     default: return HC_ERR_DTYPE;
   }
 }
