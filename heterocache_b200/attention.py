@@ -101,8 +101,10 @@ class _HeteroAttention(nn.Module):
         k = self.k_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         v = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         cos, sin = position_embeddings
-        q, k = apply_rotary_pos_emb(q, k, cos, sin)
         cache = past_key_values
+        if q_len == 1 and getattr(cache, "fused_rope", False):
+            return self._decode_fused(cache, q, k, v, cos, sin), None
+        q, k = apply_rotary_pos_emb(q, k, cos, sin)
         if cache is not None and not hasattr(cache, "prefill_select"):
             # another transformers cache (e.g. the DynamicCache a model builds by
             # default): plain causal attention over what it returns
@@ -133,6 +135,18 @@ class _HeteroAttention(nn.Module):
             else:
                 cache.decode_select(q, self.layer_idx)
         return self.o_proj(out.reshape(bsz, 1, -1)), None
+
+
+    def _decode_fused(self, cache, q, k, v, cos, sin) -> torch.Tensor:
+        """A decode step with the rotation inside the page append
+        (``HeteroCache.update_rope``): the query comes back rotated."""
+        q = cache.update_rope(q, k, v, cos, sin, self.layer_idx)
+        if self.decode_select_before_attention:
+            cache.decode_select(q, self.layer_idx)
+        out = cache.attention(q, self.layer_idx, scale=self.scaling)
+        if not self.decode_select_before_attention:
+            cache.decode_select(q, self.layer_idx, defer=cache.defer_checks)
+        return self.o_proj(out.reshape(q.shape[0], 1, -1))
 
 
 class LlamaAttention(_HeteroAttention):

@@ -57,6 +57,16 @@ class HeteroCacheConfig:
     ``total_kv_heads`` (default: layers x KV heads) is the model-wide KV head
     count of the budget formula; a cache that holds only some of a layer's
     heads (the head-sharded mode) sets it to the whole model's count.
+
+    ``fused_rope`` (default off): the patched attention classes hand a decode
+    step's unrotated query, key and value to ``HeteroCache.update_rope``, which
+    rotates and appends in one launch (rounded once; the model's own rotation
+    rounds each product, so results differ in the last bit).
+
+    ``sparse_blocks`` (default 0: off): decode attention reads at most that
+    many 64-token blocks of each row -- its first ``sparse_sink``, its last
+    ``sparse_recent`` and those whose keys' bounds promise the highest scores
+    (``ops.flash_decode_sparse``) -- in place of the whole row.
     """
 
     def __init__(self, data: Optional[Dict], compression_ratio: Optional[float] = 0.5,
@@ -65,7 +75,12 @@ class HeteroCacheConfig:
                  pooling: Optional[str] = "avgpool", kernel_size: Optional[int] = 5,
                  num_attn_heads: Optional[int] = 32, num_kv_heads: Optional[int] = 8,
                  num_layers: Optional[int] = 32, window_size: int = 1,
-                 total_kv_heads: Optional[int] = None):
+                 total_kv_heads: Optional[int] = None, fused_rope: bool = False, sparse_blocks: int = 0,
+                 sparse_sink: int = 1, sparse_recent: int = 2):
+        if sparse_blocks and not 0 <= sparse_sink + sparse_recent <= sparse_blocks:
+            raise ValueError("sparse_sink + sparse_recent must not be more than sparse_blocks")
+        self.fused_rope = fused_rope
+        self.sparse_blocks, self.sparse_sink, self.sparse_recent = sparse_blocks, sparse_sink, sparse_recent
         self.data = data
         self.stable_threshold = stable_threshold
         self.compression_ratio = compression_ratio
@@ -216,6 +231,14 @@ class HeteroCache(_CacheBase):
                                          not getattr(cache_config, "real_offload", False)))
         self._deferred: List[int] = []
         self._batch_arrays: Dict = {}
+        # rotation and append of a decode step in one launch (the patched
+        # attention classes look here); block-sparse decode attention, with
+        # each layer's block bounds (made before its first decode step)
+        self.fused_rope = bool(getattr(cache_config, "fused_rope", False))
+        self.sparse_blocks = int(getattr(cache_config, "sparse_blocks", 0))
+        self.sparse_sink = int(getattr(cache_config, "sparse_sink", 1))
+        self.sparse_recent = int(getattr(cache_config, "sparse_recent", 2))
+        self._bounds: List[Optional[torch.Tensor]] = [None] * n
         # checks per batch launch (0: the library's choice)
         self.drift_batch_per_launch = int(getattr(cache_config, "drift_batch_per_launch", 0))
         self.check_log: List[Dict] = []
@@ -415,7 +438,7 @@ class HeteroCache(_CacheBase):
         q = kw.get("query_states") if self.bsz == 1 else None
         if q is not None:
             self._ensure_decode_state(layer_idx, q)
-        if kw.get("defer_append"):
+        if kw.get("defer_append") and not self.sparse_blocks:
             # attention() attends over the pages plus this token, then appends
             # it on the side stream, off the attention's critical path
             # [k, v, q (None once stored), query slot, decode_select of this step already ran]
@@ -428,7 +451,56 @@ class HeteroCache(_CacheBase):
                           self.block_tables[layer_idx], self.heads_len[layer_idx], self.free_blocks[layer_idx],
                           self._free_ptr[layer_idx], self._err, q=q, q_stage=q_stage)
         self._q_staged[layer_idx] = q_stage is not None
+        if self.sparse_blocks:
+            self._refresh_bounds(layer_idx, last=1)
         return key_states, value_states
+
+    def update_rope(self, query_states, key_states, value_states, cos, sin, layer_idx):
+        """A decode step's ``update`` from unrotated q [bsz, H, 1, D] and k, v
+        [bsz, KV, 1, D]: rotation (cos, sin [bsz or 1, 1, D], as the model's
+        rotary embedding gives them) and page append in one launch
+        (``ops.rope_append``).  Returns the rotated query, which ``attention``
+        and ``decode_select`` take; with batch size 1 it lies in the drift
+        check's query buffer already."""
+        if key_states.shape[-2] != 1:
+            raise ValueError("update_rope: one token per sequence (prefill goes through update)")
+        if self.key_pools[layer_idx] is None:
+            raise RuntimeError("update_rope: the layer has no pages yet (prefill first)")
+        if self._deferred and layer_idx in self._deferred:
+            self.flush_checks()
+        self._append_bookkeeping(layer_idx)
+        if layer_idx == 0:
+            self._seen_tokens += 1
+        self._wait_retrieval(layer_idx)
+        self._wait_append(layer_idx)
+        q_out = None
+        if self.bsz == 1:
+            self._ensure_decode_state(layer_idx, query_states)
+            q_out = self._qbuf[layer_idx][self._qcount[layer_idx]].view(1, self.num_attn_heads, 1, self.head_dim)
+        if self.sparse_blocks:
+            self._ensure_bounds(layer_idx)
+        q_out = ops.rope_append(query_states, key_states, value_states, cos, sin, self.key_pools[layer_idx],
+                                self.value_pools[layer_idx], self.block_tables[layer_idx], self.heads_len[layer_idx],
+                                self.free_blocks[layer_idx], self._free_ptr[layer_idx], self._err,
+                                workspace=self._ws_fd, q_out=q_out, bounds=self._bounds[layer_idx])
+        self._q_staged[layer_idx] = self.bsz == 1
+        return q_out
+
+    def _ensure_bounds(self, layer_idx) -> None:
+        """The layer's block bounds, from its pages (once, before its first
+        sparse decode step; appends and retrievals keep them up to date)."""
+        if self._bounds[layer_idx] is None:
+            kp = self.key_pools[layer_idx]
+            self._bounds[layer_idx] = torch.zeros(kp.shape[0], PAGE // ops.BLOCK, 2, self.head_dim, dtype=kp.dtype,
+                                                  device=kp.device)
+            self._refresh_bounds(layer_idx)
+
+    def _refresh_bounds(self, layer_idx, rows=None, last: int = 0) -> None:
+        """Block bounds of some rows (default: all), or of every row's last tokens."""
+        if self._bounds[layer_idx] is None:
+            return  # made from the pages when they are first needed
+        ops.block_bounds(self.key_pools[layer_idx], self.block_tables[layer_idx], self.heads_len[layer_idx],
+                         self._bounds[layer_idx], self._err, rows=rows, last=last)
 
     def _append_bookkeeping(self, layer_idx: int) -> None:
         """Host side of a decode append: the free-list check of
@@ -595,6 +667,11 @@ class HeteroCache(_CacheBase):
         of all these layers and for each layer's own check."""
         for l in layers:
             self._ensure_decode_state(l, query_example)
+            if self.sparse_blocks:
+                self._ensure_bounds(l)
+                self._ws_fd.get(ops.lib().hc_flash_decode_sparse_workspace_size(
+                    self.bsz, self.num_kv_heads, self.num_key_value_groups, ops.HEAD_DIM,
+                    self.block_tables[l].shape[1]))
         n = sum(self._jobs[l].n_jobs for l in layers if self._jobs[l] is not None)
         if n and self._ws_score is not None:
             dt = ops.DTYPES[query_example.dtype]
@@ -767,6 +844,8 @@ class HeteroCache(_CacheBase):
                              k_pool=self.key_pools[layer_idx], v_pool=self.value_pools[layer_idx],
                              block_table=self.block_tables[layer_idx], num_kv_heads=self.num_kv_heads,
                              err=self._err, stream=side, tier_first_head=first)
+            with torch.cuda.stream(side):
+                self._refresh_bounds(layer_idx, rows=jobs.member_head)
             ev = torch.cuda.Event()
             ev.record(side)
             self._retrieve_done[layer_idx] = ev
@@ -777,6 +856,7 @@ class HeteroCache(_CacheBase):
                          k_pool=self.key_pools[layer_idx], v_pool=self.value_pools[layer_idx],
                          block_table=self.block_tables[layer_idx], num_kv_heads=self.num_kv_heads,
                          err=self._err, tier_first_head=first)
+            self._refresh_bounds(layer_idx, rows=jobs.member_head)
 
     def full_tier(self, layer_idx):
         """(k, v, first_head): the layer's full KV tier and the head id of its
@@ -796,11 +876,22 @@ class HeteroCache(_CacheBase):
         on the side stream; the layer's next use waits for that append.
         ``mirrors`` (device addresses) each receive a copy of the output (see
         ``ops.flash_decode``): the head-sharded mode's gathered outputs on
-        every GPU."""
+        every GPU.  With ``sparse_blocks`` set, over the selected blocks of
+        each row (no mirrors)."""
         if self._deferred and layer_idx in self._deferred:
             self.flush_checks()
         self._wait_retrieval(layer_idx)
         self._wait_append(layer_idx)
+        if self.sparse_blocks:
+            if mirrors:
+                raise NotImplementedError("block-sparse decode attention has no output mirrors")
+            self._ensure_bounds(layer_idx)
+            return ops.flash_decode_sparse(query_states, self.key_pools[layer_idx], self.value_pools[layer_idx],
+                                           self.block_tables[layer_idx], self.heads_len[layer_idx],
+                                           self._bounds[layer_idx], num_kv_heads=self.num_kv_heads,
+                                           n_select=self.sparse_blocks, sink=self.sparse_sink,
+                                           recent=self.sparse_recent, scale=scale, out=out, workspace=self._ws_fd,
+                                           err=self._err)[0]
         total = int(self._hlen[layer_idx].sum())
         pend = self._pending[layer_idx]
         if pend is None:
@@ -840,6 +931,83 @@ class HeteroCache(_CacheBase):
         if q is not None and not selected:
             self._q_staged[layer_idx] = True  # decode_select of this step comes next
         return out
+
+
+    # ------------------------------------------------------------------
+    def fork(self, n: int) -> "CacheGroup":
+        """``n`` continuations of this cache's prompt (samples, beams): a
+        ``CacheGroup`` of caches in the state this one is in after its prefill.
+        This cache is left as it is.
+
+        The heads whose prompt pages never change again (all but the
+        satellites, whose pages each continuation's retrievals rewrite) keep one
+        copy of them for the whole group: ``attention_together`` reads them
+        once for all members (``ops.flash_decode_shared``).  Each member has
+        pages of its own for the satellites, for the last, partly filled
+        page of the other heads, and for the tokens it decodes."""
+        if n < 1:
+            raise ValueError("fork: at least one continuation")
+        if self.bsz != 1:
+            raise NotImplementedError("fork: batch size 1 (a prompt)")
+        if self._group is not None or self.sparse_blocks:
+            raise NotImplementedError("fork: a cache of its own, without block-sparse attention")
+        if any(self._qcount) or any(p is not None for p in self._pending) or self._deferred \
+                or any(e is not None for e in self._append_done):
+            raise RuntimeError("fork: continue a prompt right after its prefill")
+        members = [HeteroCache(self.config) for _ in range(n)]
+        group = CacheGroup(members)
+        for m in members:
+            m.bsz, m.head_dim, m.prefill_len, m._seen_tokens = 1, self.head_dim, self.prefill_len, self._seen_tokens
+            m.base_compress_len = self.base_compress_len
+            m.record_checks, m.defer_checks = self.record_checks, self.defer_checks
+            m.drift_batch_per_launch = self.drift_batch_per_launch
+            m._ensure_device(self._dev)
+            m.key_cache_cpu, m.value_cache_cpu = list(self.key_cache_cpu), list(self.value_cache_cpu)
+            m.prefill_topk_set = [t.clone() if torch.is_tensor(t) else list(t) for t in self.prefill_topk_set]
+            m._ref_bitmap = [None if t is None else t.clone() for t in self._ref_bitmap]
+            m._kept, m._tier_first = list(self._kept), list(self._tier_first)
+            m.layer_head_capacities = list(self.layer_head_capacities)
+            m.prefill_boundary_blocks = list(self.prefill_boundary_blocks)
+        if self._side_stream is not None:  # the prompt's full tier is written there
+            torch.cuda.current_stream(self._dev).wait_stream(self._side_stream)
+        for l in range(self.num_layers):
+            if self.key_pools[l] is not None:
+                group._fork_layer(self, l)
+        return group
+
+
+def fork_pages(block_table, lens, gen: int, width: int, private, n: int):
+    """Page tables of ``n`` continuations of one prompt, on the host.
+
+    ``block_table`` [KV, >= pages] (the prompt's, whose pages are contiguous
+    ids from 0 on), ``lens`` [KV] its tokens a head, ``gen`` the tokens a
+    member may append, ``private`` the heads whose pages each member has for
+    itself.  Returns (tables [n, KV, width], shared [KV] tokens a head whose
+    pages all members share, copies [(from, to)] of page ids, free [n] lists of
+    each member's spare ids, pages in all)."""
+    KV = len(lens)
+    used = int(max([int(block_table[h, (int(lens[h]) + PAGE - 1) // PAGE - 1]) + 1 for h in range(KV) if lens[h]]
+                   or [0]))
+    tables = np.full((n, KV, width), -1, dtype=np.int32)
+    shared = np.zeros(KV, dtype=np.int32)
+    copies, free, nxt = [], [], used
+    for h in range(KV):
+        shared[h] = 0 if h in private else int(lens[h]) // PAGE * PAGE
+    for i in range(n):
+        spare = 0
+        for h in range(KV):
+            L = int(lens[h])
+            pages, first = (L + PAGE - 1) // PAGE, int(shared[h]) // PAGE
+            tables[i, h, :pages] = block_table[h, :pages]
+            if i > 0:  # the first member keeps the prompt's own
+                for p in range(first, pages):
+                    copies.append((int(block_table[h, p]), nxt))
+                    tables[i, h, p] = nxt
+                    nxt += 1
+            spare += (L + gen + PAGE - 1) // PAGE - pages
+        free.append(list(range(nxt, nxt + spare)))
+        nxt += spare
+    return tables, shared, copies, free, nxt
 
 
 def flush_checks_together(caches) -> None:
@@ -910,6 +1078,40 @@ class CacheGroup:
         self._layers: Dict[int, dict] = {}
         self._qbufs: Dict[int, torch.Tensor] = {}
         self._ws: Optional[Workspace] = None
+        # a fork's layers: tokens of each head whose pages all members share
+        self.shared_len: Dict[int, torch.Tensor] = {}
+
+    def _fork_layer(self, cache, layer) -> None:
+        """The layer's pool of a fork: ``cache``'s pages, the members' copies of
+        those they do not share, and their spare pages."""
+        kp, vp, dev = cache.key_pools[layer], cache.value_pools[layer], cache._dev
+        members = cache.data["leader_member_relations"][layer].values()
+        private = {int(h) for m in members for h in m}
+        lens, n, KV = cache._hlen[layer], len(self.members), cache.num_kv_heads
+        bt = cache.block_tables[layer].cpu().numpy()
+        tables, shared, copies, free, total = fork_pages(bt, lens, cache.config.max_gen_len, bt.shape[1], private, n)
+        pools = []
+        for old in (kp, vp):
+            new = torch.zeros(total, *old.shape[1:], dtype=old.dtype, device=dev)
+            used = min(total, old.shape[0])
+            new[:used].copy_(old[:used])
+            if copies:
+                src, dst = torch.tensor(copies, device=dev).t()
+                new[dst] = old[src]
+            pools.append(new)
+        st = dict(slot=total, rows=KV, mb=bt.shape[1], dtype=kp.dtype, device=dev, kp=pools[0], vp=pools[1],
+                  bt=torch.from_numpy(tables.reshape(n * KV, -1)).to(dev),
+                  hl=cache.heads_len[layer].repeat(n))
+        self._layers[layer] = st
+        self.shared_len[layer] = torch.from_numpy(shared).to(dev)
+        for i, m in enumerate(self.members):
+            rows = slice(i * KV, (i + 1) * KV)
+            m.key_pools[layer], m.value_pools[layer] = pools
+            m.block_tables[layer], m.heads_len[layer] = st["bt"][rows], st["hl"][rows]
+            m.free_blocks[layer] = torch.tensor(free[i], dtype=torch.int32, device=dev)
+            m._free_ptr[layer] = torch.zeros(1, dtype=torch.int32, device=dev)
+            m._hlen[layer] = lens.copy()
+            m._mapped[layer] = (tables[i] >= 0).sum(1).astype(np.int64)
 
     def _query_buffer(self, cache, layer, S, H, D, dtype, device):
         """Member's drift-check query buffer [S, H, D]: row ``cache._gidx`` of
@@ -984,10 +1186,19 @@ def attention_together(group: CacheGroup, query_states, layer_idx, scale: float 
     c0 = members[0]
     if query_states.shape[0] != len(members):
         raise ValueError("attention_together: one query row per member")
+    if any(c.sparse_blocks for c in members):
+        raise NotImplementedError("attention_together: block-sparse members attend for themselves")
+    shared = group.shared_len.get(layer_idx)
+    if shared is not None and mirrors:
+        raise NotImplementedError("attention_together: a fork's attention has no output mirrors")
     ws = group._workspace(c0._dev)
     total = sum(int(c._hlen[layer_idx].sum()) for c in members)
     pends = [c._pending[layer_idx] for c in members]
     if all(p is None for p in pends):
+        if shared is not None:
+            return ops.flash_decode_shared(query_states, st["kp"], st["vp"], st["bt"], st["hl"], shared,
+                                           num_kv_heads=c0.num_kv_heads, scale=scale, out=out, workspace=ws,
+                                           err=c0._err)
         return ops.flash_decode(query_states, st["kp"], st["vp"], st["bt"], st["hl"], num_kv_heads=c0.num_kv_heads,
                                 scale=scale, out=out, workspace=ws, err=c0._err, total_tokens_hint=total,
                                 mirrors=mirrors, mirror_batch_stride=mirror_batch_stride)
@@ -1012,9 +1223,14 @@ def attention_together(group: CacheGroup, query_states, layer_idx, scale: float 
     v_new = _batch_view([p[1] for p in pends])
     k_new = torch.cat([p[0] for p in pends], 0) if k_new is None else k_new
     v_new = torch.cat([p[1] for p in pends], 0) if v_new is None else v_new
-    out = ops.flash_decode(query_states, st["kp"], st["vp"], st["bt"], st["hl"], num_kv_heads=c0.num_kv_heads,
-                           scale=scale, out=out, workspace=ws, err=c0._err, total_tokens_hint=total, k_new=k_new,
-                           v_new=v_new, mirrors=mirrors, mirror_batch_stride=mirror_batch_stride)
+    if shared is not None:
+        out = ops.flash_decode_shared(query_states, st["kp"], st["vp"], st["bt"], st["hl"], shared,
+                                      num_kv_heads=c0.num_kv_heads, scale=scale, out=out, workspace=ws, err=c0._err,
+                                      k_new=k_new, v_new=v_new)
+    else:
+        out = ops.flash_decode(query_states, st["kp"], st["vp"], st["bt"], st["hl"], num_kv_heads=c0.num_kv_heads,
+                               scale=scale, out=out, workspace=ws, err=c0._err, total_tokens_hint=total, k_new=k_new,
+                               v_new=v_new, mirrors=mirrors, mirror_batch_stride=mirror_batch_stride)
     main = torch.cuda.current_stream(c0._dev)
     for c, (k, v, q, slot, selected) in zip(members, pends):
         side = c._side()

@@ -184,6 +184,8 @@ class HeadShardedCache:
         KV, H = config.num_kv_heads, config.num_attn_heads
         if H % KV:
             raise ValueError("query heads must be a multiple of KV heads")
+        if getattr(config, "sparse_blocks", 0) or getattr(config, "fused_rope", False):
+            raise NotImplementedError("sparse_blocks and fused_rope: caches on one GPU")
         T = getattr(config, "total_kv_heads", None) or KV * config.num_layers
         self.assignment = head_assignment(config.data, config.num_layers, KV, world, balance,
                                           config.compression_ratio, T)

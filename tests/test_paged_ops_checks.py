@@ -198,3 +198,31 @@ def test_the_library_refuses_bad_arguments():
     assert lib.hc_flash_decode_shared_workspace_size(1, 4, 8, 4, D) > 0
     assert lib.hc_flash_decode_shared_workspace_size(5, 4, 8, 4, D) == 0
     assert lib.hc_block_select_workspace_size(1, 8, 100) >= 8 * 400 * 8
+
+
+def test_fork_pages():
+    """The page tables of a fork: whole pages shared, the last one and private heads copied, spare pages apart."""
+    import numpy as np
+    from heterocache_b200.cache import fork_pages
+    bt = np.full((3, 6), -1, dtype=np.int32)
+    bt[0, :3], bt[1, :2], bt[2, :2] = [0, 1, 2], [3, 4], [5, 6]
+    tables, shared, copies, free, total = fork_pages(bt, [600, 512, 300], 300, 6, {2}, 3)
+    assert shared.tolist() == [512, 512, 0]
+    assert tables[0, 0].tolist() == [0, 1, 2, -1, -1, -1] and tables[0, 2].tolist() == [5, 6, -1, -1, -1, -1]
+    for i in (1, 2):
+        assert tables[i, 0, :2].tolist() == [0, 1] and tables[i, 1, :2].tolist() == [3, 4]
+        own = [tables[i, 0, 2], *tables[i, 2, :2]]
+        assert tables[i, 2, 1] == tables[i, 2, 0] + 1  # retrievals write a private head's pages as one piece
+        assert len(set(own)) == 3 and min(own) >= 7
+        assert [c for c in copies if c[1] in own] == [(2, own[0]), (5, own[1]), (6, own[2])]
+    # 600, 512 and 300 tokens grow by 300: 1, 2 and 1 pages more
+    assert [len(f) for f in free] == [4, 4, 4]
+    ids = sorted(sum(free, []) + [int(c[1]) for c in copies])
+    assert ids == list(range(7, total))
+
+
+def test_config_checks_sparse_blocks():
+    from heterocache_b200.cache import HeteroCacheConfig
+    with pytest.raises(ValueError, match="sparse_blocks"):
+        HeteroCacheConfig({}, sparse_blocks=2, sparse_sink=1, sparse_recent=2)
+    assert HeteroCacheConfig({}).sparse_blocks == 0 and not HeteroCacheConfig({}).fused_rope
