@@ -1193,18 +1193,22 @@ static cudaError_t pdl_launch(void (*kern)(KArgs...), int grid, int threads, siz
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
-// Warps a head of the join: the most of 8, 4, 2, 1 that leave at most 8
-// waves' worth of 4 CTAs an SM; few heads take more warps each, which shortens
-// the chain of loads.
+// Warps a head of the join: 8 where that leaves at most 4 CTAs an SM -- few
+// heads, and a short chain of loads for each -- and 2 beyond (2048 heads of
+// 64 x 131072 shared tokens: the call 176 us with 2 and 181 with 4; 812 heads
+// of 29 x 20001: 40.8 with 2, 41.7 with 8).
+template <typename T, int kMode, int W>
+static int fd_join_warps(FDParams& p, int grid, cudaStream_t st) {
+  const int per = kJWarps / W;
+  const int ctas = (p.R * p.G + per - 1) / per;
+  return pdl_launch(flash_join_kernel<T, kMode, W>, ctas, kJThreads, 0, st, p, grid) == cudaSuccess ? HC_OK
+                                                                                                  : HC_ERR_CUDA;
+}
+
 template <typename T, int kMode>
 static int fd_join(FDParams& p, int grid, cudaStream_t st) {
-  const int heads = p.R * p.G;
-  if (heads <= 148 * 4)
-    return pdl_launch(flash_join_kernel<T, kMode, 8>, heads, kJThreads, 0, st, p, grid) == cudaSuccess ? HC_OK
-                                                                                                      : HC_ERR_CUDA;
-  return pdl_launch(flash_join_kernel<T, kMode, 2>, (heads + 3) / 4, kJThreads, 0, st, p, grid) == cudaSuccess
-             ? HC_OK
-             : HC_ERR_CUDA;
+  if (p.R * p.G <= 4 * device_sms(current_device())) return fd_join_warps<T, kMode, 8>(p, grid, st);
+  return fd_join_warps<T, kMode, 2>(p, grid, st);
 }
 
 template <typename T, int kMode>

@@ -5,6 +5,7 @@
 // The tails (each row's own tokens) run through the split decode kernel
 // (decode_attn.cu, FD_TAIL), whose combine joins both parts' partials.
 #include <algorithm>
+#include <type_traits>
 
 #include "hc_host.cuh"
 #include "hc_params.cuh"
@@ -203,13 +204,9 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
 // Tensor-core form (16-bit types): one CTA per SM, tiles of 128 tokens.
 //   S = Q K^T  (M = 128 query rows on the TMEM lanes, N = 128 tokens)
 //   O += P V   (A = P from tensor memory, B = V as loaded, MN-major)
-// Two streams X = 0, 1, each with its own O accumulator, so that the tensor
-// core works on one while the softmax warps work on the other.  A stream
-// takes its tiles in halves of 64 tokens, with two S accumulators in turn (P
-// is written over the first 32 columns of its S): the scores of a half are
-// computed while the softmax of the one before runs, which halved the time a
-// softmax warp waits (128 tokens a step, one S a stream: 4800 clocks a step,
-// 2700 of them waiting for S).  With at most 128 query rows a group
+// Two streams X = 0, 1, each with its own S (P is written over its first 64
+// columns) and O accumulators, so that the tensor core works on one while
+// the softmax warps work on the other.  With at most 128 query rows a group
 // both streams hold the same rows and take the tiles in turn (X takes tiles
 // X, X + 2, ...): two independent splits of the tokens.  With up to 256 the
 // streams hold 128 rows each and every tile serves both.
@@ -232,8 +229,7 @@ constexpr int kTcTiles = 7;              // tile buffers: queries, keys, values
 constexpr size_t kTcSmem = 1024 + (size_t)kTcTiles * kTcTileBytes;
 constexpr int kTcK = 3;                  // key stages; values have the rest
 constexpr int kTcValidRing = 8;          // tiles whose valid counts are kept
-constexpr int kTcHalf = 64;              // tokens of a step
-// tensor-memory columns: S of stream X, buffer i at 128 X + 64 i, O at 256 + 128 X
+// tensor-memory columns: S of stream X at 128 X (P in its first 64), O at 256 + 128 X
 constexpr uint32_t kTcColS = 0, kTcColO = 256;
 
 // The same answer for the whole warp (each lane polls for itself).
@@ -317,129 +313,104 @@ struct TcWalk {
   }
 };
 
-// What an MMA issuer needs of the CTA's shared memory.
+// What the MMA issuer needs of the CTA's shared memory.
 struct TcSmem {
-  unsigned char *sq, *sk, *sv;
+  unsigned char* tiles;  // buffers 0 .. kTcK - 1 keys, then values, the last one or two queries
   int vst;
-  uint64_t *q_full, *k_full, *k_empty, *v_full, *v_empty;
-  uint64_t (*s_full)[2];
-  uint64_t (*p_ready)[2];
-  uint64_t* o_done;
-  const int* s_valid;
+  uint64_t *q_full, *k_full, *k_empty, *v_empty;
+  uint64_t *s_full, *p_ready, *o_done;
 };
 
-// The MMAs of both streams, called by a whole warp: all lanes wait, one issues
-// (the same one throughout: MMAs of one thread execute in order, so a half's
-// S may follow the O step that reads the P it overwrites).  Half h of a tile
-// has S buffer h.
+// The MMAs of both streams in turn, called by a whole warp: all lanes wait,
+// one issues (the same one throughout: MMAs of one thread execute in order,
+// so a tile's S may follow the O step that reads the P it overwrites).  What
+// this warp does between two MMAs the tensor core waits for, so it does
+// little: the softmax warps have waited for a step's values before they
+// report its P.
 template <typename T>
-__device__ __forceinline__ bool tc_issue(const SPParams& p, const TcSmem& sm, TcWalk& walk, uint32_t tmem, bool wide) {
+__device__ __forceinline__ bool tc_issue(const SPParams& p, const TcSmem& sm, TcWalk& walk, bool wide) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  const uint32_t id_s = idesc_f16_m128(kBf16, kTcHalf);
+  const uint32_t id_s = idesc_f16_m128(kBf16, 128);
   const uint32_t id_o = idesc_f16_m128(kBf16, 128) | kIdescBMajorMN;
-  const int lane = threadIdx.x & 31;
+  const uint32_t tiles = smem_u32(sm.tiles);
+  const uint64_t dq1 = smem_desc_sw128(tiles + (kTcTiles - 1) * kTcTileBytes);
+  const uint64_t dq0 = wide ? smem_desc_sw128(tiles + (kTcTiles - 2) * kTcTileBytes) : dq1;
   int kbase = 0, piece = 0;   // the piece's first tile, pieces
-  int done[2] = {0, 0};       // tiles of earlier pieces per stream
-  int kw = -1, vw = -1;       // last key / value tile waited for
+  int done0 = 0, done1 = 0;   // steps of earlier pieces per stream
   TcPiece pc;
   auto wait_k = [&](int n) {
-    if (n <= kw) return true;
     if (!mbar_wait_warp(&sm.k_full[n % kTcK], (n / kTcK) & 1, p.wait_ns)) return false;
-    kw = n;
     tc_fence_after();
     return true;
   };
-  // the value tile, the tokens that do not count zeroed
-  auto wait_v = [&](int n) {
-    if (n <= vw) return true;
-    if (!mbar_wait_warp(&sm.v_full[n % sm.vst], (n / sm.vst) & 1, p.wait_ns)) return false;
-    vw = n;
-    const int valid = sm.s_valid[n % kTcValidRing];
-    if (valid < kTcTile) {
-      unsigned char* vt = sm.sv + (size_t)(n % sm.vst) * kTcTileBytes;
-      for (int c = valid * 8 + lane; c < kTcTile * 8; c += 32) {
-        *reinterpret_cast<uint4*>(vt + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(vt + kTcBox + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-    }
-    return true;
-  };
-  // S of half h of tile n for stream x; free_k: the tile's last
-  auto issue_s = [&](int x, int n, int h, bool free_k) {
+  // S of tile n for stream x; free_k: no other stream reads the tile later
+  auto issue_s = [&](int x, int n, bool free_k) {
+    const int st = n % kTcK;
     if (elect_one()) {
-      const uint64_t dq = smem_desc_sw128(smem_u32(sm.sq + (wide ? x : 0) * kTcTileBytes));
-      const uint64_t dk = smem_desc_sw128(smem_u32(sm.sk + (size_t)(n % kTcK) * kTcTileBytes) + h * kTcHalf * 128);
-      const uint32_t d = tmem + kTcColS + (uint32_t)(128 * x + 64 * h);
+      const uint64_t dq = x ? dq1 : dq0, dk = smem_desc_sw128(tiles + st * kTcTileBytes);
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
         const uint64_t off = (uint64_t)(((kk >> 2) * kTcBox + (kk & 3) * 32) >> 4);
-        umma_f16(d, dq + off, dk + off, id_s, kk > 0 ? 1u : 0u);
+        umma_f16(kTcColS + 128u * x, dq + off, dk + off, id_s, kk > 0 ? 1u : 0u);
       }
-      umma_commit(&sm.s_full[x][h]);
-      if (free_k) umma_commit(&sm.k_empty[n % kTcK]);
+      umma_commit(&sm.s_full[x]);
+      if (free_k) umma_commit(&sm.k_empty[st]);
     }
     __syncwarp();
   };
-  auto issue_pv = [&](int x, int n, int h, bool first, bool free_v) {
+  auto issue_pv = [&](int x, int n, bool first, bool free_v) {
+    const int st = n % sm.vst;
     if (elect_one()) {
-      const uint64_t dv = smem_desc_sw128_mn(
-          smem_u32(sm.sv + (size_t)(n % sm.vst) * kTcTileBytes) + h * kTcHalf * 128, kTcBox);
-      const uint32_t d = tmem + kTcColO + (uint32_t)(128 * x);
-      const uint32_t pa = tmem + kTcColS + (uint32_t)(128 * x + 64 * h);
+      const uint64_t dv = smem_desc_sw128_mn(tiles + (kTcK + st) * kTcTileBytes, kTcBox);
+      const uint32_t d = kTcColO + 128u * x, pa = kTcColS + 128u * x;
 #pragma unroll
-      for (int kk = 0; kk < kTcHalf / 16; ++kk)
+      for (int kk = 0; kk < 8; ++kk)
         umma_f16_ts(d, pa + (uint32_t)(8 * kk), dv + (uint64_t)((kk * 16 * 128) >> 4), id_o,
                     (!first || kk > 0) ? 1u : 0u);
       umma_commit(&sm.o_done[x]);
-      if (free_v) umma_commit(&sm.v_empty[n % sm.vst]);
+      if (free_v) umma_commit(&sm.v_empty[st]);
     }
     __syncwarp();
   };
-  bool ok = true;
-  while (ok && walk.next(p, pc)) {
+  while (walk.next(p, pc)) {
     const int nt = pc.t1 - pc.t0;
     // each stream's tiles: first, first + step, ..
     const int step = wide ? 1 : 2;
     const bool both = !wide || p.B * p.G - pc.ng * 256 > 128;  // (wide: stream 1 has rows)
     const int n0 = wide ? nt : (nt + 1) >> 1, n1 = !both ? 0 : wide ? nt : nt >> 1;
     const int f0 = kbase, f1 = kbase + (wide ? 0 : 1);
-    // a tile's stage is free once the last stream that reads it has
-    const bool last0 = !wide || !both;
+    // wide: a tile's stage is free once stream 1, which comes second, has read it
+    const bool free0 = !wide || !both;
     kbase += nt;
-    ok = mbar_wait_warp(sm.q_full, piece++ & 1, p.wait_ns) && wait_k(f0);
-    if (!ok) break;
-    for (int h = 0; h < 2; ++h) {
-      issue_s(0, f0, h, last0 && h);
-      if (n1 > 0) {
-        ok = ok && wait_k(f1);
-        if (ok) issue_s(1, f1, h, h);
-      }
+    if (!mbar_wait_warp(sm.q_full, piece++ & 1, p.wait_ns) || !wait_k(f0)) return false;
+    issue_s(0, f0, free0);
+    if (n1 > 0) {
+      if (!wide && !wait_k(f1)) return false;
+      issue_s(1, f1, true);
     }
-    for (int i = 0; ok && i < n0; ++i) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int n = (x ? f1 : f0) + i * step, nx = x ? n1 : n0;
-          if (!ok || i >= nx) continue;
-          ok = wait_v(n) && mbar_wait_warp(&sm.p_ready[x][h], (done[x] + i) & 1, p.wait_ns);
-          if (!ok) continue;
-          tc_fence_after();
-          const bool last = x == 1 || last0;
-          issue_pv(x, n, h, i == 0 && h == 0, last && h);
-          if (i + 1 < nx) {
-            ok = wait_k(n + step);
-            if (ok) issue_s(x, n + step, h, last && h);
-          }
+    for (int i = 0; i < n0; ++i) {
+      const int t0 = f0 + i * step, t1 = f1 + i * step;
+      if (!mbar_wait_warp(&sm.p_ready[0], (done0 + i) & 1, p.wait_ns)) return false;
+      tc_fence_after();
+      issue_pv(0, t0, i == 0, free0);
+      if (i + 1 < n0) {
+        if (!wait_k(t0 + step)) return false;
+        issue_s(0, t0 + step, free0);
+      }
+      if (i < n1) {
+        if (!mbar_wait_warp(&sm.p_ready[1], (done1 + i) & 1, p.wait_ns)) return false;
+        tc_fence_after();
+        issue_pv(1, t1, i == 0, true);
+        if (i + 1 < n1) {
+          if (!wide && !wait_k(t1 + step)) return false;
+          issue_s(1, t1 + step, true);
         }
       }
     }
-    done[0] += n0;
-    done[1] += n1;
+    done0 += n0;
+    done1 += n1;
   }
-  return ok;
+  return true;
 }
 
 template <typename T>
@@ -447,14 +418,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     shared_prefix_tc_kernel(const SPParams p, const __grid_constant__ CUtensorMap tmk,
                             const __grid_constant__ CUtensorMap tmv) {
   extern __shared__ __align__(16) unsigned char smem_dyn[];
-  unsigned char* sq = smem_dyn + ((1024 - (smem_u32(smem_dyn) & 1023)) & 1023);
   const bool wide = p.plan.rows_per > 128;  // the streams hold different rows
   const int nq = wide ? 2 : 1;
   const int vst = kTcTiles - kTcK - nq;
-  unsigned char* sk = sq + nq * kTcTileBytes;
+  // tile buffers: keys, values, queries
+  unsigned char* sk = smem_dyn + ((1024 - (smem_u32(smem_dyn) & 1023)) & 1023);
   unsigned char* sv = sk + kTcK * kTcTileBytes;
+  unsigned char* sq = sk + (kTcTiles - nq) * kTcTileBytes;
   __shared__ __align__(8) uint64_t q_full, k_full[kTcK], k_empty[kTcK], v_full[kTcTiles - kTcK],
-      v_empty[kTcTiles - kTcK], s_full[2][2], p_ready[2][2], o_done[2], all_done;
+      v_empty[kTcTiles - kTcK], s_full[2], p_ready[2], o_done[2], all_done;
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail, s_kissued, s_vissued;
   __shared__ int s_valid[kTcValidRing];  // tokens of the tile that count, by the CTA's tile number
@@ -472,10 +444,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&v_empty[i], 1);
     }
     for (int x = 0; x < 2; ++x) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&s_full[x][i], 1);
-        mbar_init(&p_ready[x][i], 4);
-      }
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_ready[x], 4);
       mbar_init(&o_done[x], 1);
     }
     mbar_init(&all_done, 1);
@@ -490,7 +460,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = s_tmem;  // all 512 columns: column 0 on
   pdl_wait();
   pdl_trigger();
   TcWalk walk;
@@ -556,8 +526,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
   } else if (warp == 1) {
     // ---- MMA issuer
-    const TcSmem sm = {sq, sk, sv, vst, &q_full, k_full, k_empty, v_full, v_empty, s_full, p_ready, o_done, s_valid};
-    const bool ok = tc_issue<T>(p, sm, walk, tmem, wide);
+    const TcSmem sm = {sk, vst, &q_full, k_full, k_empty, v_empty, s_full, p_ready, o_done};
+    const bool ok = tc_issue<T>(p, sm, walk, wide);
     if (!ok && lane == 0) atomicExch(&s_fail, 1);
     // every MMA issued has completed before the tensor memory is released
     if (elect_one()) umma_commit(&all_done);
@@ -569,7 +539,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int x = (warp - 4) >> 2;
     const int row = 32 * (warp & 3) + lane;
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t cs0 = tmem + lane_off + kTcColS + (uint32_t)(128 * x);
+    const uint32_t cs = tmem + lane_off + kTcColS + (uint32_t)(128 * x);
     const uint32_t co = tmem + lane_off + kTcColO + (uint32_t)(128 * x);
     const float sl2 = p.scale_log2;
     const int tid = threadIdx.x - 128;  // of 256
@@ -581,7 +551,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int g0 = pc.ng * p.plan.rows_per;                       // the group's first query row
       const int grows = min(p.plan.rows_per, p.B * p.G - g0);       // its rows
       const int srows = min(128, grows - (wide ? 128 * x : 0));     // this stream's rows (may be <= 0)
-      const int n = 2 * (wide ? (srows > 0 ? nt : 0) : (nt + 1 - x) >> 1);  // steps
+      const int n = wide ? (srows > 0 ? nt : 0) : (nt + 1 - x) >> 1;  // steps: the stream's tiles
       // the queries, 128-byte swizzled; the MMAs that read the old ones, and
       // the loads of the old accumulators, have completed
       named_bar_sync(1, 256);
@@ -614,30 +584,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool active = 32 * (warp & 3) < srows;  // the warp's lanes hold query rows
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n && !dead; ++j) {
-        const int i = steps + j, buf = i & 1;
-        const uint32_t cs = cs0 + (uint32_t)(64 * buf);
-        if (!mbar_wait_warp(&s_full[x][buf], (i >> 1) & 1, p.wait_ns)) {
+        if (!mbar_wait_warp(&s_full[x], (steps + j) & 1, p.wait_ns)) {
           dead = true;
           break;
         }
         tc_fence_after();
         if (active) {
-          const int valid =
-              s_valid[(kbase + (wide ? j >> 1 : (j & ~1) + x)) % kTcValidRing] - (j & 1) * kTcHalf;
-          uint32_t v[kTcHalf];
+          const int valid = s_valid[(kbase + (wide ? j : 2 * j + x)) % kTcValidRing];
+          // the maximum over the tile; the first 64 scores stay in registers,
+          // the others are loaded again for P
+          uint32_t v[64];
+          tmem_ld32(cs + 64u, v);
+          tmem_ld32(cs + 96u, v + 32);
+          tmem_ld_wait();
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (valid < kTcTile) {
+#pragma unroll
+            for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], 64 + k < valid ? __uint_as_float(v[k]) : -INFINITY);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(v[k]));
+          }
           tmem_ld32(cs, v);
           tmem_ld32(cs + 32u, v + 32);
           tmem_ld_wait();
-          if (valid < kTcHalf) {
+          if (valid < 64) {
 #pragma unroll
-            for (int k = 0; k < kTcHalf; ++k)
+            for (int k = 0; k < 64; ++k)
               if (k >= valid) v[k] = 0xff800000u;  // -infinity
           }
-          float mx[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = __uint_as_float(v[k]);
-#pragma unroll
-          for (int k = 4; k < kTcHalf; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(v[k]));
+          for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(v[k]));
           // log2 domain (scale > 0)
           const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2);
           const bool resc = j > 0 && m_new > m_used + 8.f;
@@ -645,9 +622,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (__any_sync(0xffffffffu, resc)) {
             // P stays below 2^8: O and l are rescaled only when the maximum
             // has grown by more since they last were
-            // (S of this step was issued after the O step before last, so at
-            // most the last one is open)
-            if (!mbar_wait_warp(&o_done[x], (i - 1) & 1, p.wait_ns)) {
+            if (!mbar_wait_warp(&o_done[x], (steps + j - 1) & 1, p.wait_ns)) {
               dead = true;
               break;
             }
@@ -671,12 +646,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const uint64_t sl22 = pack_f2(sl2, sl2), nm2 = pack_f2(nm, nm);
           uint64_t ps[2] = {0ull, 0ull};
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 4; ++c) {
+            if (c == 2) {
+              tmem_ld32(cs + 64u, v);
+              tmem_ld32(cs + 96u, v + 32);
+              tmem_ld_wait();
+              if (valid < kTcTile) {
+#pragma unroll
+                for (int k = 0; k < 64; ++k)
+                  if (64 + k >= valid) v[k] = 0xff800000u;
+              }
+            }
             uint32_t w[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              const float2 t = unpack_f2(fma_f2(
-                  pack_f2(__uint_as_float(v[32 * c + 2 * k]), __uint_as_float(v[32 * c + 2 * k + 1])), sl22, nm2));
+              const int at = 32 * (c & 1) + 2 * k;
+              const float2 t =
+                  unpack_f2(fma_f2(pack_f2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), sl22, nm2));
               const float e0 = exp2_approx(t.x), e1 = exp2_approx(t.y);
               ps[k & 1] = add_f2(ps[k & 1], pack_f2(e0, e1));
               w[k] = Elem<T>::cvt2(e0, e1);
@@ -687,15 +673,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           l += sum.x + sum.y;
           tmem_st_wait();
         }
+        // the step's values are there before P is reported; those of tokens
+        // that do not count are zeroed (by both streams alike, where both
+        // read the tile)
+        const int tile = kbase + (wide ? j : 2 * j + x);
+        const int valid_v = s_valid[tile % kTcValidRing];
+        if ((warp & 3) == 0 || valid_v < kTcTile) {
+          if (!mbar_wait_warp(&v_full[tile % vst], (tile / vst) & 1, p.wait_ns)) {
+            dead = true;
+            break;
+          }
+          if (valid_v < kTcTile && row >= valid_v) {
+            unsigned char* vt = sv + (size_t)(tile % vst) * kTcTileBytes + row * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              *reinterpret_cast<uint4*>(vt + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(vt + kTcBox + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+          }
+        }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[x][buf]);
+        if (lane == 0) mbar_arrive(&p_ready[x]);
       }
       // the piece's partials: O relative to the maximum, not divided by the sum
-      // (the last two O steps may both be open: one phase after the other, a
-      // parity tells only neighbouring phases apart)
-      for (int k = 2; k > 0; --k)
-        if (n > 0 && !dead && !mbar_wait_warp(&o_done[x], (steps + n - k) & 1, p.wait_ns)) dead = true;
+      if (n > 0 && !dead && !mbar_wait_warp(&o_done[x], (steps + n - 1) & 1, p.wait_ns)) dead = true;
       const int64_t slot = (int64_t)blockIdx.x + pc.h * p.plan.n_groups + pc.ng;
       float f0 = 1.f, f1 = 0.f;
       if (!wide) {
