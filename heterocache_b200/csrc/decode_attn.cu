@@ -218,9 +218,9 @@ __device__ __forceinline__ void fd_group_compute(const FDParams& p, WarpState<T>
 // fp32: lanes over dims, warp all-reduce per (query head, token).
 __device__ __forceinline__ void fd_group_f32(const FDParams& p, WarpState<float>& st, const float (&qf)[kGMax][4],
                                              const float* kbase, const float* vbase, int valid, float (&mrow)[kGMax],
-                                             float (&lrow)[kGMax], int first = 0) {
+                                             float (&lrow)[kGMax]) {
   const int lane = threadIdx.x & 31;
-  for (int i = first; i < 16; ++i) {
+  for (int i = 0; i < 16; ++i) {
     if (i >= valid) break;
     const float4 k4 = *reinterpret_cast<const float4*>(kbase + i * kD + 4 * lane);
     const float4 v4 = *reinterpret_cast<const float4*>(vbase + i * kD + 4 * lane);
@@ -240,6 +240,58 @@ __device__ __forceinline__ void fd_group_f32(const FDParams& p, WarpState<float>
       st.o[g][1] = st.o[g][1] * corr + pv * v4.y;
       st.o[g][2] = st.o[g][2] * corr + pv * v4.z;
       st.o[g][3] = st.o[g][3] * corr + pv * v4.w;
+    }
+  }
+}
+
+// The same for FD_TAIL and FD_BLOCKS, tokens first .. valid - 1: four tokens'
+// keys and values are in flight at a time and share one update of the running
+// maximum (their rows are short, so a chain of single tokens is what bounds
+// them: 48 rows of 75 tokens took 24 us one token at a time).
+__device__ __forceinline__ void fd_group_f32x4(const FDParams& p, WarpState<float>& st, const float (&qf)[kGMax][4],
+                                               const float* kbase, const float* vbase, int first, int valid,
+                                               float (&mrow)[kGMax], float (&lrow)[kGMax]) {
+  const int lane = threadIdx.x & 31;
+  for (int i = first; i < valid; i += 4) {
+    float4 k4[4], v4[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int t = min(i + u, valid - 1);
+      k4[u] = *reinterpret_cast<const float4*>(kbase + t * kD + 4 * lane);
+      v4[u] = *reinterpret_cast<const float4*>(vbase + t * kD + 4 * lane);
+    }
+#pragma unroll
+    for (int g = 0; g < kGMax; ++g) {
+      if (g >= p.G) continue;
+      float s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        s[u] = qf[g][0] * k4[u].x + qf[g][1] * k4[u].y + qf[g][2] * k4[u].z + qf[g][3] * k4[u].w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], o);
+      float mx = mrow[g];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        s[u] = i + u < valid ? s[u] * p.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[u]);
+      }
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      const float corr = exp2f(mrow[g] - ref);
+      mrow[g] = mx;
+      lrow[g] *= corr;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) st.o[g][d] *= corr;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float pv = exp2f(s[u] - ref);
+        lrow[g] += pv;
+        st.o[g][0] = fmaf(pv, v4[u].x, st.o[g][0]);
+        st.o[g][1] = fmaf(pv, v4[u].y, st.o[g][1]);
+        st.o[g][2] = fmaf(pv, v4[u].z, st.o[g][2]);
+        st.o[g][3] = fmaf(pv, v4[u].w, st.o[g][3]);
+      }
     }
   }
 }
@@ -311,8 +363,10 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
         int blk = page < p.max_blocks ? p.bt[(int64_t)r * p.max_blocks + page] : -1;
         if (blk < 0 || blk >= p.n_blocks) { set_err(p.err, HC_ERR_RANGE); continue; }
         const int64_t off = ((int64_t)blk * kPage + (t & (kPage - 1))) * kD;
-        fd_group_f32(p, st, qf, reinterpret_cast<const float*>(p.kp) + off,
-                     reinterpret_cast<const float*>(p.vp) + off, valid, mrow, lrow, first);
+        const float* kb = reinterpret_cast<const float*>(p.kp) + off;
+        const float* vb = reinterpret_cast<const float*>(p.vp) + off;
+        if constexpr (kMode == FD_ALL) fd_group_f32(p, st, qf, kb, vb, valid, mrow, lrow);
+        else fd_group_f32x4(p, st, qf, kb, vb, first, valid, mrow, lrow);
       }
       if (lane == 0) {
         for (int g = 0; g < kGMax; ++g) { s_m[warp][g] = mrow[g]; s_l[warp][g] = lrow[g]; }
