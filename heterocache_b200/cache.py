@@ -949,6 +949,8 @@ class HeteroCache(_CacheBase):
             raise ValueError("fork: at least one continuation")
         if self.bsz != 1:
             raise NotImplementedError("fork: batch size 1 (a prompt)")
+        if n * self.num_kv_heads > 4096:
+            raise ValueError("fork: at most 4096 rows (continuations x KV heads)")
         if self._group is not None or self.sparse_blocks:
             raise NotImplementedError("fork: a cache of its own, without block-sparse attention")
         if any(self._qcount) or any(p is not None for p in self._pending) or self._deferred \

@@ -284,9 +284,59 @@ def test_fork_refuses_a_cache_in_the_middle_of_decoding(cuda_device):
     q0 = _prefill(c, 700, 5, cuda_device)
     with pytest.raises(ValueError, match="at least one"):
         c.fork(0)
+    with pytest.raises(ValueError, match="4096 rows"):
+        c.fork(513)
     q, k, v = (t.to(cuda_device) for t in DriftingDecode(GEO, seed=1, q0=q0, dtype=torch.bfloat16).step())
     c.update(k, v, 0, {"query_states": q})
     c.attention(q, 0)
     c.decode_select(q, 0)
     with pytest.raises(RuntimeError, match="right after its prefill"):
         c.fork(2)
+
+
+@pytest.mark.parametrize("kind", ["llama", "qwen"])
+@pytest.mark.parametrize("sparse", [0, 6])
+def test_model_graph_with_fused_rope(cuda_device, kind, sparse):
+    """A whole model's decode, eager and from graphs, with the rotation in the append and block-sparse attention:
+    the same tokens and pages."""
+    import transformers
+    from heterocache_b200.attention import patch_transformers
+    from heterocache_b200.graph import ModelDecodeGraph
+    patch_transformers()
+    torch.manual_seed(1)
+    args = dict(hidden_size=1024, num_attention_heads=8, num_key_value_heads=4, intermediate_size=2048,
+                num_hidden_layers=2, vocab_size=512, max_position_embeddings=4096)
+    cfg = transformers.LlamaConfig(head_dim=128, **args) if kind == "llama" else transformers.Qwen2Config(**args)
+    cfg._attn_implementation = "sdpa"
+    cls = transformers.LlamaForCausalLM if kind == "llama" else transformers.Qwen2ForCausalLM
+    model = cls(cfg).to(cuda_device, torch.bfloat16).eval()
+    data = derive_runtime_data(synthetic_roles(2, 4, seed=5, star_size=3), 2, 4)
+    ids = torch.randint(0, 512, (1, 800), device=cuda_device)
+
+    def prefilled():
+        c = HeteroCache(HeteroCacheConfig(data, stable_threshold=0.9, real_offload=False, max_gen_len=32,
+                                          decode_step=5, num_attn_heads=8, num_kv_heads=4, num_layers=2,
+                                          fused_rope=True, sparse_blocks=sparse))
+        with torch.no_grad():
+            out = model(input_ids=ids, past_key_values=c, use_cache=True, logits_to_keep=1)
+        return c, out.logits[:, -1:].argmax(-1)
+
+    eager, tok = prefilled()
+    tokens = []
+    with torch.no_grad():
+        for t in range(12):
+            pos = torch.tensor([[800 + t]], device=cuda_device)
+            out = model(input_ids=tok, past_key_values=eager, use_cache=True, position_ids=pos, cache_position=pos[0],
+                        logits_to_keep=1)
+            tok = out.logits[:, -1:].argmax(-1)
+            tokens.append(int(tok))
+    eager.join_retrievals()
+    graphed, tok = prefilled()
+    runner = ModelDecodeGraph(model, graphed, tok.clone(), torch.tensor([[800]], device=cuda_device))
+    assert [int(runner.step()) for _ in range(12)] == tokens
+    for c in (eager, graphed):
+        c.check_errors()
+    for layer in range(2):
+        assert torch.equal(graphed.heads_len[layer], eager.heads_len[layer])
+        assert torch.equal(graphed.block_tables[layer], eager.block_tables[layer])
+        assert (graphed.key_pools[layer].float() - eager.key_pools[layer].float()).abs().max().item() <= 2e-2

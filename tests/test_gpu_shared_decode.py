@@ -184,3 +184,53 @@ def test_many_rows_of_one_prompt_equal_plain_decode(cuda_device):
     assert int(c.err) == 0
     # both are half a step and a probability's half step from the exact value
     assert float((a.double() - b.double()).abs().max()) <= 4 * 2.0 ** -8 * float(vp.double().abs().max())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_what_rows_hold_before_their_own_tokens_is_not_read(cuda_device, dt):
+    """The page in which the shared tokens end: in the other sequences' copies of it, NaN before their own tokens."""
+    bsz, H, KV, shared = 3, 8, 2, [300, 70]
+    c, q, s = _setup(bsz, H, KV, shared, [[9, 1], [33, 0], [64, 100]], DT[dt], cuda_device)
+    ref, tol = _reference(c, q, s, bsz, H, KV)
+    for r in range(KV, bsz * KV):
+        n, page = shared[r % KV] % PAGE, int(c.table[r, shared[r % KV] // PAGE])
+        c.kp[page, :n], c.vp[page, :n] = float("nan"), float("nan")
+    out = ops.flash_decode_shared(q, c.kp, c.vp, c.table, c.lens, s, num_kv_heads=KV,
+                                  workspace=ops.Workspace(cuda_device), err=c.err)
+    assert int(c.err) == 0 and float((out.double() - ref).abs().max()) <= tol
+
+
+def test_on_another_stream(cuda_device):
+    """Append and both attentions on a side stream, ordered by it alone."""
+    dev, bsz, H, KV, dtype = cuda_device, 4, 8, 2, torch.bfloat16
+    c, q, s = _setup(bsz, H, KV, [700, 400], [[60, 30]] * bsz, dtype, dev)
+    ref, tol = _reference(c, q, s, bsz, H, KV)
+    ws, side = ops.Workspace(dev), torch.cuda.Stream(dev)
+    later = torch.zeros_like(q)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        later.copy_(q)  # the query is there only when the stream gets to it
+        out = ops.flash_decode_shared(later, c.kp, c.vp, c.table, c.lens, s, num_kv_heads=KV, workspace=ws, err=c.err)
+    side.synchronize()
+    assert int(c.err) == 0 and float((out.double() - ref).abs().max()) <= tol
+
+
+def test_a_stalled_prefix_gives_up(cuda_device):
+    """No key tile is loaded (injected): every wait runs out, the flag says so, and the next call is right."""
+    dev, bsz, H, KV = cuda_device, 5, 8, 2
+    c, q, s = _setup(bsz, H, KV, [2000, 300], [[60, 30]] * bsz, torch.bfloat16, dev)
+    ref, tol = _reference(c, q, s, bsz, H, KV)
+    ws = ops.Workspace(dev)
+    call = lambda: ops.flash_decode_shared(q, c.kp, c.vp, c.table, c.lens, s, num_kv_heads=KV, workspace=ws,  # noqa: E731
+                                           err=c.err)
+    ops.set_wait_limits(5_000_000, inject_stall=True)  # 5 ms
+    try:
+        call()
+        torch.cuda.synchronize()
+        assert int(c.err) & (1 << 7)
+    finally:
+        ops.set_wait_limits(0, inject_stall=False)
+    c.err.zero_()
+    out = call()
+    assert int(c.err) == 0 and float((out.double() - ref).abs().max()) <= tol
