@@ -3,8 +3,7 @@
 // same tokens, so B * G query rows are multiplied with each key and value
 // while it is on chip, and the pages are read from HBM once for the batch.
 // The tails (each row's own tokens) run through the split decode kernel
-// (decode_attn.cu, FD_TAIL), whose combine joins both parts' partials.
-#include <algorithm>
+// (decode_attn.cu, FD_TAIL), and a join there merges both parts' partials.
 #include <type_traits>
 
 #include "hc_host.cuh"
@@ -17,7 +16,7 @@ constexpr int kSpThreads = 256;
 constexpr int kSpTok = 32;   // tokens of a tile
 // row pitch of queries and keys in shared memory (elements): 16 bytes more
 // than a row, so that rows start on 16-byte boundaries in different banks
-template <typename T> constexpr int kSpPad = kD + 16 / (int)sizeof(T);
+constexpr int kSpPad = kD + 4;
 constexpr int kSpPP = 36;    // row pitch of the probabilities
 
 __device__ __forceinline__ int sp_len(const SPParams& p, int h) {
@@ -32,9 +31,9 @@ __device__ __forceinline__ int sp_total(const SPParams& p) {
   return n * p.plan.n_groups;
 }
 
-template <typename T> constexpr size_t sp_smem(int RT) {
-  return (size_t)RT * kSpPad<T> * sizeof(T) + 2 * (size_t)kSpTok * kSpPad<T> * sizeof(T) +
-         2 * (size_t)kSpTok * kD * sizeof(T) + (size_t)RT * kSpPP * sizeof(float);
+constexpr size_t sp_smem(int RT) {
+  return ((size_t)RT * kSpPad + 2 * (size_t)kSpTok * kSpPad + 2 * (size_t)kSpTok * kD + (size_t)RT * kSpPP) *
+         sizeof(float);
 }
 
 // 16 bytes to shared memory; nothing is read and zeros are written if !ok.
@@ -42,29 +41,22 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ok) 
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0)
                : "memory");
 }
-template <typename T>
-__device__ __forceinline__ float4 lds4(const T* p) {
-  if constexpr (sizeof(T) == 4) {
-    return *reinterpret_cast<const float4*>(p);
-  } else {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
-    return make_float4(a.x, a.y, b.x, b.y);
-  }
-}
+__device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-// CUDA-core form: RPT query rows a thread (16 * RPT a CTA), tiles of 32
-// tokens, two of them in shared memory by cp.async.  Thread (ty, tx) of the
-// 16 x 16 holds rows ty * RPT + i, scores of tokens tx and tx + 16, outputs
-// of dims 4 tx .. and 64 + 4 tx ...
-template <typename T, int RPT>
+// CUDA-core form, for fp32: RPT query rows a thread (16 * RPT a CTA), tiles
+// of 32 tokens, two of them in shared memory by cp.async.  Thread (ty, tx) of
+// the 16 x 16 holds rows ty * RPT + i, scores of tokens tx and tx + 16,
+// outputs of dims 4 tx .. and 64 + 4 tx ..  Bound by the fp32 units from some
+// ten rows on (4 flops a byte and row), by latency where there are few tiles:
+// 24 rows x 3000 tokens x 8 heads take 20 us.
+template <int RPT>
 __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPParams p) {
   constexpr int RT = 16 * RPT;
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  T* sq = reinterpret_cast<T*>(smem_raw);
-  T* sk = sq + RT * kSpPad<T>;
-  T* sv = sk + 2 * kSpTok * kSpPad<T>;
-  float* sp = reinterpret_cast<float*>(sv + 2 * kSpTok * kD);
+  float* sq = reinterpret_cast<float*>(smem_raw);
+  float* sk = sq + RT * kSpPad;
+  float* sv = sk + 2 * kSpTok * kSpPad;
+  float* sp = sv + 2 * kSpTok * kD;
   pdl_wait();
   pdl_trigger();
   const int total = sp_total(p);
@@ -81,13 +73,13 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
       const int t0 = max(beg, start) - start, t1 = min(end, start + tiles) - start;
       if (t0 >= t1) continue;
       __syncthreads();
-      constexpr int CH = kD * sizeof(T) / 16, CE = 16 / (int)sizeof(T);
+      constexpr int CH = kD / 4, CE = 4;
       for (int i = threadIdx.x; i < RT * CH; i += kSpThreads) {
         const int row = ng * RT + i / CH, c = i % CH;
         const bool ok = row < p.B * p.G;
         const int b = ok ? row / p.G : 0, g = ok ? row % p.G : 0;
-        const T* src = reinterpret_cast<const T*>(p.q) + b * p.qsb + (int64_t)(h * p.G + g) * p.qsh + c * CE;
-        cp_async16(sq + (i / CH) * kSpPad<T> + c * CE, src, ok);
+        const float* src = reinterpret_cast<const float*>(p.q) + b * p.qsb + (int64_t)(h * p.G + g) * p.qsh + c * CE;
+        cp_async16(sq + (i / CH) * kSpPad + c * CE, src, ok);
       }
       auto load = [&](int t, int s) {
         const int pos = t * kSpTok, page = pos >> 8;
@@ -98,8 +90,8 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
         for (int i = threadIdx.x; i < kSpTok * CH; i += kSpThreads) {
           const int row = i / CH, c = i % CH;
           const bool ok = in && pos + row < len;
-          cp_async16(sk + (s * kSpTok + row) * kSpPad<T> + c * CE, reinterpret_cast<const T*>(p.kp) + off + row * kD + c * CE, ok);
-          cp_async16(sv + (s * kSpTok + row) * kD + c * CE, reinterpret_cast<const T*>(p.vp) + off + row * kD + c * CE, ok);
+          cp_async16(sk + (s * kSpTok + row) * kSpPad + c * CE, reinterpret_cast<const float*>(p.kp) + off + row * kD + c * CE, ok);
+          cp_async16(sv + (s * kSpTok + row) * kD + c * CE, reinterpret_cast<const float*>(p.vp) + off + row * kD + c * CE, ok);
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
         return in ? min(kSpTok, len - pos) : 0;
@@ -123,17 +115,17 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
           asm volatile("cp.async.wait_group 0;\n" ::: "memory");
         }
         __syncthreads();
-        const T* kt = sk + s * kSpTok * kSpPad<T>;
-        const T* vt = sv + s * kSpTok * kD;
+        const float* kt = sk + s * kSpTok * kSpPad;
+        const float* vt = sv + s * kSpTok * kD;
         float a[RPT][2];
 #pragma unroll
         for (int i = 0; i < RPT; ++i) a[i][0] = a[i][1] = 0.f;
 #pragma unroll 4
         for (int d = 0; d < kD; d += 4) {
-          const float4 k0 = lds4<T>(kt + tx * kSpPad<T> + d), k1 = lds4<T>(kt + (tx + 16) * kSpPad<T> + d);
+          const float4 k0 = lds4(kt + tx * kSpPad + d), k1 = lds4(kt + (tx + 16) * kSpPad + d);
 #pragma unroll
           for (int i = 0; i < RPT; ++i) {
-            const float4 q = lds4<T>(sq + (ty * RPT + i) * kSpPad<T> + d);
+            const float4 q = lds4(sq + (ty * RPT + i) * kSpPad + d);
             a[i][0] = fmaf(q.x, k0.x, fmaf(q.y, k0.y, fmaf(q.z, k0.z, fmaf(q.w, k0.w, a[i][0]))));
             a[i][1] = fmaf(q.x, k1.x, fmaf(q.y, k1.y, fmaf(q.z, k1.z, fmaf(q.w, k1.w, a[i][1]))));
           }
@@ -164,7 +156,7 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
           for (int i = 0; i < RPT; ++i) pr[i] = *reinterpret_cast<const float4*>(sp + (ty * RPT + i) * kSpPP + j);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float4 v0 = lds4<T>(vt + (j + u) * kD + 4 * tx), v1 = lds4<T>(vt + (j + u) * kD + 64 + 4 * tx);
+            const float4 v0 = lds4(vt + (j + u) * kD + 4 * tx), v1 = lds4(vt + (j + u) * kD + 64 + 4 * tx);
 #pragma unroll
             for (int i = 0; i < RPT; ++i) {
               const float w = u == 0 ? pr[i].x : u == 1 ? pr[i].y : u == 2 ? pr[i].z : pr[i].w;
@@ -210,6 +202,13 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
 // both streams hold the same rows and take the tiles in turn (X takes tiles
 // X, X + 2, ...): two independent splits of the tokens.  With up to 256 the
 // streams hold 128 rows each and every tile serves both.
+// Measured: 64 rows x 8 heads of 6554 to 32768 tokens (96 MB), 26 to 31 us,
+// the steady part near the reading of the pages; 256 rows x 8 heads of up to
+// 131072 tokens (376 MB, 97 GFLOP), 125 us, 0.47 of the measured bf16 rate.
+// There the chain of a stream (S, softmax, O) sets the pace: a step of both
+// takes some 4000 clocks, of which the tensor core works 2048; its 8 MMAs
+// take 512 clocks alone and 600 to 1000 beside the softmax warps' loads of
+// tensor memory, whose exponentials are 2048 clocks of their unit a step.
 // Warps: 0 key producer, 2 value producer (TMA), 1 MMA issuer, 4-7 and 8-11
 // softmax of stream 0 and 1 (one query row a thread); 3 has no role.  The
 // CTA's span may cover several segments (KV head, row group); between them
@@ -828,9 +827,9 @@ static int sp_pdl_launch(K kern, int grid, int threads, size_t smem, cudaStream_
 template <int RPT>
 static int sp_launch_f32(const SPParams& p, int dev, cudaStream_t st) {
   static bool done[kMaxDevices];
-  constexpr size_t smem = sp_smem<float>(16 * RPT);
-  if (!sp_allow_smem(shared_prefix_kernel<float, RPT>, smem, done, dev)) return HC_ERR_CUDA;
-  return sp_pdl_launch(shared_prefix_kernel<float, RPT>, p.plan.n_ctas, kSpThreads, smem, st, p);
+  constexpr size_t smem = sp_smem(16 * RPT);
+  if (!sp_allow_smem(shared_prefix_kernel<RPT>, smem, done, dev)) return HC_ERR_CUDA;
+  return sp_pdl_launch(shared_prefix_kernel<RPT>, p.plan.n_ctas, kSpThreads, smem, st, p);
 }
 
 template <typename T>

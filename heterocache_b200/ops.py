@@ -7,7 +7,6 @@ the reference's tensors: q ``[bsz, H, L, D]``, k/v ``[bsz, KV, L, D]``, pools
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Optional, Tuple
 
 import torch
@@ -344,36 +343,49 @@ def flash_decode(q, k_pool, v_pool, block_table, heads_len, *, num_kv_heads, out
     return out
 
 
-_HERE = contextlib.nullcontext()
+# The checks of the operators below run on every call of a decode loop, where
+# a launch takes a few microseconds of host time: they read each tensor's
+# properties once and build a message only for a refusal.
+_I32 = torch.int32
 
 
 def _refuse(what: str):
     raise ValueError(f"heterocache_b200: {what}")
 
 
-def _same_device(*ts: Optional[torch.Tensor]):
-    """All tensors on one CUDA device; a context in which that device is the
-    current one (the library launches on the current device)."""
-    dev = ts[0].get_device()
+def _call(name: str, fn, args, q: torch.Tensor, ts) -> None:
+    """``fn(*args, stream)`` with q's device the current one (the library
+    launches on the current device) and that device's current stream.  Refuses
+    tensors that are elsewhere."""
+    dev = q.get_device()
     for t in ts:
         if t is not None and t.get_device() != dev:
-            _refuse(f"tensors on different devices ({ts[0].device} and {t.device})")
+            _refuse(f"tensors on different devices ({q.device} and {t.device})")
     if dev < 0:
         for t in ts:
-            if t is not None and t.device != ts[0].device:
-                _refuse(f"tensors on different devices ({ts[0].device} and {t.device})")
+            if t is not None and t.device != q.device:
+                _refuse(f"tensors on different devices ({q.device} and {t.device})")
         _refuse("tensors must live on a CUDA device")
-    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(name, rc)
 
 
-def _raw_stream(t: torch.Tensor) -> int:
-    """``_stream`` without building a stream object (a microsecond of a call's host time)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+def _layout(t: torch.Tensor, name: str):
+    """(shape, strides) of a tensor of contiguous 128-element rows."""
+    shape, st = t.shape, t.stride()
+    if not st or shape[-1] != HEAD_DIM or st[-1] != 1:
+        _refuse(f"{name} must have a contiguous last dim of {HEAD_DIM}")
+    return shape, st
 
 
 def _ints(t: torch.Tensor, name: str, n: int, what: str) -> None:
     """A contiguous int32 tensor of at least n entries."""
-    if t.dtype != torch.int32 or not t.is_contiguous():
+    if t.dtype is not _I32 or not t.is_contiguous():
         _refuse(f"{name} must be a contiguous int32 tensor")
     if t.numel() < n:
         _refuse(what)
@@ -384,7 +396,7 @@ def _pool(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
     s = t.shape
     if len(s) != 4 or s[1] != PAGE or s[2] != 1 or s[3] != HEAD_DIM or not t.is_contiguous():
         _refuse(f"{name} must be a contiguous [n_blocks, {PAGE}, 1, {HEAD_DIM}] pool")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         _refuse(f"{name} must have the dtype of the other operands")
     return s[0]
 
@@ -431,16 +443,18 @@ def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_
     or a free list that is too short, is reported in ``err`` and leaves the
     cache as it was.  ``workspace`` holds a counter; calls that may overlap
     need a workspace each."""
-    _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
-    if q.dim() != 4 or k.dim() != 4:
+    shape, qs = _layout(q, "q")
+    dtype = q.dtype
+    kshape, ks = _layout(k, "k")
+    vshape, vs = _layout(v, "v")
+    if len(shape) != 4 or len(kshape) != 4:
         _refuse("q, k, v need [bsz, heads, tokens, D]")
-    bsz, H, T, D = q.shape
-    shape = k.shape
-    KV, dtype = shape[1], q.dtype
+    bsz, H, T, D = shape
+    KV = kshape[1]
     dt = dtype_code(q)
-    if shape != v.shape or k.dtype != v.dtype:
+    if kshape != vshape or k.dtype is not v.dtype:
         _refuse("k and v must have the same shape and dtype")
-    if shape[0] != bsz or shape[2] != T or k.dtype != dtype:
+    if kshape[0] != bsz or kshape[2] != T or k.dtype is not dtype:
         _refuse("q, k and v must share batch, tokens and dtype")
     R = bsz * KV
     if R <= 0 or H <= 0:
@@ -456,10 +470,11 @@ def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_
     if counts is not None:
         _ints(counts, "counts", bsz, "counts needs an entry per sequence")
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        q_out = q.new_empty(shape)
+        os = q_out.stride()
     else:
-        _rows(q_out, "q_out")
-        if q_out.shape != q.shape or q_out.dtype != dtype:
+        oshape, os = _layout(q_out, "q_out")
+        if oshape != shape or q_out.dtype is not dtype:
             _refuse("q_out must have the queries' shape and dtype")
     if heads_len_out is None:
         heads_len_out = heads_len
@@ -468,54 +483,44 @@ def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_
     if bounds is not None:
         _bounds(bounds, n_pages, dtype)
     counter = workspace.counter
-    qb, qh, qt, _ = q.stride()
-    kb, kh, kt, _ = k.stride()
-    vb, vh, vt, _ = v.stride()
-    ob, oh, ot, _ = q_out.stride()
-    with _same_device(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, heads_len_out, free_blocks, free_ptr,
-                      err, counts, q_out, bounds, counter):
-        rc = lib().hc_rope_append(dt, DTYPES[trig], bsz, H, KV, T, D, q.data_ptr(), qb, qh, qt, k.data_ptr(), kb, kh,
-                                  kt, v.data_ptr(), vb, vh, vt, cos.data_ptr(), cb, ct, sin.data_ptr(), sb, st,
-                                  q_out.data_ptr(), ob, oh, ot, _ptr(counts), k_pool.data_ptr(), v_pool.data_ptr(),
-                                  n_pages, block_table.data_ptr(), width, heads_len.data_ptr(),
-                                  heads_len_out.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(),
-                                  free_ptr.data_ptr(), _ptr(bounds), counter.data_ptr(), err.data_ptr(),
-                                  _raw_stream(q))
-    if rc:
-        check("hc_rope_append", rc)
+    _call("hc_rope_append", lib().hc_rope_append,
+          (dt, DTYPES[trig], bsz, H, KV, T, D, q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
+           v.data_ptr(), vs[0], vs[1], vs[2], cos.data_ptr(), cb, ct, sin.data_ptr(), sb, st, q_out.data_ptr(), os[0],
+           os[1], os[2], _ptr(counts), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
+           heads_len.data_ptr(), heads_len_out.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(),
+           free_ptr.data_ptr(), _ptr(bounds), counter.data_ptr(), err.data_ptr()), q,
+          (k, v, cos, sin, k_pool, v_pool, block_table, heads_len, heads_len_out, free_blocks, free_ptr, err, counts,
+           q_out, bounds, counter))
     LAUNCHES[0] += 1
     return q_out
 
 
 def _trig_strides(t, name: str, bsz: int, T: int, dtype, trig) -> Tuple[int, int]:
     """Batch and token stride of cos or sin, [bsz or 1, T, D] or [T, D]."""
-    _rows(t, name)
-    s = t.shape
-    if len(s) == 2:
-        s = (1,) + tuple(s)
-    if len(s) != 3 or (s[0] != 1 and s[0] != bsz) or s[1] != T:
+    s, st = _layout(t, name)
+    n = len(s)
+    if (n != 3 and n != 2) or s[-2] != T or (n == 3 and s[0] != 1 and s[0] != bsz):
         _refuse(f"{name} needs [bsz or 1, tokens, D]")
-    if t.dtype != trig or (trig != dtype and trig != torch.float32):
+    if t.dtype is not trig or (trig is not dtype and trig is not torch.float32):
         _refuse("cos and sin must share a dtype: the queries', or float32")
-    return (0 if s[0] == 1 else t.stride(0)), t.stride(-2)
+    return (0 if n == 2 or s[0] == 1 else st[0]), st[-2]
 
 
-def _decode_query(q, num_kv_heads: int, name: str) -> Tuple[int, int]:
-    """(bsz, query heads per KV head) of a decode step's query."""
-    _rows(q, "q")
-    s = q.shape
+def _decode_query(q, num_kv_heads: int, name: str):
+    """(bsz, query heads, query heads per KV head, strides) of a decode step's query."""
+    s, st = _layout(q, "q")
     if len(s) != 4 or s[2] != 1:
         _refuse(f"{name} takes one query position, [bsz, H, 1, D]")
-    if s[0] <= 0 or num_kv_heads <= 0 or s[1] <= 0 or s[1] % num_kv_heads:
-        _refuse(f"the {s[1]} query heads do not split evenly over {num_kv_heads} KV heads")
-    return s[0], s[1] // num_kv_heads
+    bsz, H = s[0], s[1]
+    if bsz <= 0 or num_kv_heads <= 0 or H <= 0 or H % num_kv_heads:
+        _refuse(f"the {H} query heads do not split evenly over {num_kv_heads} KV heads")
+    return bsz, H, H // num_kv_heads, st
 
 
-def _decode_out(out, q, bsz: int) -> torch.Tensor:
-    H = q.shape[1]
+def _decode_out(out, q, bsz: int, H: int) -> torch.Tensor:
     if out is None:
-        return torch.empty((bsz, H, HEAD_DIM), dtype=q.dtype, device=q.device)
-    if not out.is_contiguous() or out.numel() != bsz * H * HEAD_DIM or out.dtype != q.dtype:
+        return q.new_empty((bsz, H, HEAD_DIM))
+    if not out.is_contiguous() or out.numel() != bsz * H * HEAD_DIM or out.dtype is not q.dtype:
         _refuse("out must be a contiguous [bsz, H, D] buffer in the query dtype")
     return out
 
@@ -528,35 +533,37 @@ def flash_decode_shared(q, k_pool, v_pool, block_table, heads_len, shared_len, *
     the first sequence's rows of the page table.  Each row's own tokens follow
     from position shared_len[h] to heads_len[r] - 1; with k_new / v_new [bsz,
     KV, 1, D] one more token a row, not in the pages."""
-    bsz, G = _decode_query(q, num_kv_heads, "decode attention")
+    bsz, H, G, qs = _decode_query(q, num_kv_heads, "decode attention")
     n_pages = _pools(k_pool, v_pool, q.dtype)
     width = _cache_rows(block_table, heads_len, bsz * num_kv_heads)
-    out = _decode_out(out, q, bsz)
+    out = _decode_out(out, q, bsz, H)
     _ints(shared_len, "shared_len", num_kv_heads, "shared_len needs an entry per KV head")
     _ints(err, "err", 1, "err needs an entry")
     if (k_new is None) != (v_new is None):
         _refuse("k_new and v_new come together")
     kn = vn = (0, 0)
     if k_new is not None:
-        _rows(k_new, "k_new"), _rows(v_new, "v_new")
+        kn, vn = _layout(k_new, "k_new")[1], _layout(v_new, "v_new")[1]
         _same_shape(k_new, v_new)
-        if tuple(k_new.shape) != (bsz, num_kv_heads, 1, HEAD_DIM) or k_new.dtype != q.dtype:
+        if tuple(k_new.shape) != (bsz, num_kv_heads, 1, HEAD_DIM) or k_new.dtype is not q.dtype:
             _refuse("k_new/v_new must be [bsz, KV, 1, D] in the query dtype")
-        kn, vn = k_new.stride(), v_new.stride()
     dt = dtype_code(q)
     L = lib()
-    with _same_device(q, k_pool, v_pool, block_table, heads_len, shared_len, out, err, k_new, v_new):
-        ws = workspace.get(L.hc_flash_decode_shared_workspace_size(dt, bsz, num_kv_heads, G, HEAD_DIM))
-        qs = q.stride()
-        rc = L.hc_flash_decode_shared(dt, bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1],
-                                      k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
-                                      heads_len.data_ptr(), shared_len.data_ptr(), _ptr(k_new), _ptr(v_new), kn[0],
-                                      kn[1], vn[0], vn[1], float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
-                                      err.data_ptr(), _raw_stream(q))
-    if rc:
-        check("hc_flash_decode_shared", rc)
+    ws = _scratch(workspace, q, L.hc_flash_decode_shared_workspace_size, dt, bsz, num_kv_heads, G, HEAD_DIM)
+    _call("hc_flash_decode_shared", L.hc_flash_decode_shared,
+          (dt, bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1], k_pool.data_ptr(), v_pool.data_ptr(),
+           n_pages, block_table.data_ptr(), width, heads_len.data_ptr(), shared_len.data_ptr(), _ptr(k_new),
+           _ptr(v_new), kn[0], kn[1], vn[0], vn[1], float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
+           err.data_ptr()), q,
+          (k_pool, v_pool, block_table, heads_len, shared_len, out, err, k_new, v_new, ws))
     LAUNCHES[0] += 3
     return out
+
+
+def _scratch(workspace: Workspace, q, size, *args) -> torch.Tensor:
+    """The workspace, as large as ``size(*args)`` says; nothing is asked of it
+    for a query that is not on a CUDA device (the call then refuses)."""
+    return workspace.get(size(*args)) if q.is_cuda else q
 
 
 def block_bounds(k_pool, block_table, heads_len, bounds, err, *, rows=None, last: int = 0) -> torch.Tensor:
@@ -573,13 +580,10 @@ def block_bounds(k_pool, block_table, heads_len, bounds, err, *, rows=None, last
         _refuse("last must not be negative")
     if rows is not None:
         _ints(rows, "rows", 0, "")
-    with _same_device(k_pool, block_table, heads_len, bounds, err, rows):
-        rc = lib().hc_block_bounds(dtype_code(k_pool), n, HEAD_DIM, k_pool.data_ptr(), n_pages,
-                                   block_table.data_ptr(), width, heads_len.data_ptr(), _ptr(rows),
-                                   0 if rows is None else rows.numel(), int(last), bounds.data_ptr(), err.data_ptr(),
-                                   _raw_stream(k_pool))
-    if rc:
-        check("hc_block_bounds", rc)
+    _call("hc_block_bounds", lib().hc_block_bounds,
+          (dtype_code(k_pool), n, HEAD_DIM, k_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
+           heads_len.data_ptr(), _ptr(rows), 0 if rows is None else rows.numel(), int(last), bounds.data_ptr(),
+           err.data_ptr()), k_pool, (block_table, heads_len, bounds, err, rows))
     LAUNCHES[0] += 1
     return bounds
 
@@ -590,13 +594,13 @@ def _select_lists(q, bounds, R: int, n_select: int, sink: int, recent: int, bloc
         _refuse("sink + recent blocks must not be more than n_select, which must be at least 1")
     what = "blocks needs [rows, n_select] and counts an entry per row"
     if blocks is None:
-        blocks = torch.empty((R, n_select), dtype=torch.int32, device=q.device)
+        blocks = q.new_empty((R, n_select), dtype=_I32)
     else:
         _ints(blocks, "blocks", 0, what)
         if tuple(blocks.shape) != (R, n_select):
             _refuse(what)
     if counts is None:
-        counts = torch.empty((R,), dtype=torch.int32, device=q.device)
+        counts = q.new_empty(R, dtype=_I32)
     else:
         _ints(counts, "counts", R, what)
     return blocks, counts
@@ -608,7 +612,7 @@ def block_select(q, bounds, block_table, heads_len, *, num_kv_heads, n_select: i
     each row the first ``sink``, the last ``recent`` and those of the highest
     bound on their scores, n_select in all.  Returns (blocks [rows, n_select]
     int32 ascending, -1 behind; counts [rows] int32)."""
-    bsz, G = _decode_query(q, num_kv_heads, "block_select")
+    bsz, _, G, qs = _decode_query(q, num_kv_heads, "block_select")
     R = bsz * num_kv_heads
     width = _cache_rows(block_table, heads_len, R)
     n_pages = bounds.shape[0]
@@ -616,15 +620,12 @@ def block_select(q, bounds, block_table, heads_len, *, num_kv_heads, n_select: i
     _ints(err, "err", 1, "err needs an entry")
     blocks, counts = _select_lists(q, bounds, R, n_select, sink, recent, blocks, counts)
     L = lib()
-    with _same_device(q, bounds, block_table, heads_len, err, blocks, counts):
-        ws = workspace.get(L.hc_block_select_workspace_size(bsz, num_kv_heads, width))
-        qs = q.stride()
-        rc = L.hc_block_select(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1],
-                               bounds.data_ptr(), n_pages, block_table.data_ptr(), width, heads_len.data_ptr(),
-                               int(n_select), int(sink), int(recent), blocks.data_ptr(), counts.data_ptr(),
-                               ws.data_ptr(), ws.numel(), err.data_ptr(), _raw_stream(q))
-    if rc:
-        check("hc_block_select", rc)
+    ws = _scratch(workspace, q, L.hc_block_select_workspace_size, bsz, num_kv_heads, width)
+    _call("hc_block_select", L.hc_block_select,
+          (dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1], bounds.data_ptr(), n_pages,
+           block_table.data_ptr(), width, heads_len.data_ptr(), int(n_select), int(sink), int(recent),
+           blocks.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr()), q,
+          (bounds, block_table, heads_len, err, blocks, counts, ws))
     LAUNCHES[0] += 2
     return blocks, counts
 
@@ -634,11 +635,11 @@ def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, count
     """Decode attention over each row's listed 64-token blocks alone
     (hc_flash_decode_blocks): blocks [rows, n] int32 ascending, the first
     counts[row] of them used."""
-    bsz, G = _decode_query(q, num_kv_heads, "decode attention")
+    bsz, H, G, qs = _decode_query(q, num_kv_heads, "decode attention")
     n_pages = _pools(k_pool, v_pool, q.dtype)
     R = bsz * num_kv_heads
     width = _cache_rows(block_table, heads_len, R)
-    out = _decode_out(out, q, bsz)
+    out = _decode_out(out, q, bsz, H)
     what = "blocks needs [rows, n] and counts an entry per row"
     _ints(blocks, "blocks", 1, what)
     _ints(counts, "counts", R, what)
@@ -646,16 +647,13 @@ def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, count
     if blocks.dim() != 2 or blocks.shape[0] < R:
         _refuse(what)
     L = lib()
-    with _same_device(q, k_pool, v_pool, block_table, heads_len, blocks, counts, out, err):
-        ws = workspace.get(L.hc_flash_decode_workspace_size(bsz, num_kv_heads, G, HEAD_DIM))
-        qs = q.stride()
-        rc = L.hc_flash_decode_blocks(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1],
-                                      k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
-                                      heads_len.data_ptr(), blocks.data_ptr(), counts.data_ptr(), blocks.shape[1],
-                                      float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr(),
-                                      _raw_stream(q))
-    if rc:
-        check("hc_flash_decode_blocks", rc)
+    ws = _scratch(workspace, q, L.hc_flash_decode_workspace_size, bsz, num_kv_heads, G, HEAD_DIM)
+    _call("hc_flash_decode_blocks", L.hc_flash_decode_blocks,
+          (dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1], k_pool.data_ptr(),
+           v_pool.data_ptr(), n_pages, block_table.data_ptr(), width, heads_len.data_ptr(), blocks.data_ptr(),
+           counts.data_ptr(), blocks.shape[1], float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
+           err.data_ptr()), q,
+          (k_pool, v_pool, block_table, heads_len, blocks, counts, out, err, ws))
     LAUNCHES[0] += 2
     return out
 
@@ -666,25 +664,22 @@ def flash_decode_sparse(q, k_pool, v_pool, block_table, heads_len, bounds, *, nu
     """Block-sparse decode attention (hc_flash_decode_sparse): what
     ``block_select`` and then ``flash_decode_blocks`` over its lists give.
     Returns (out [bsz, H, D], blocks [rows, n_select], counts [rows])."""
-    bsz, G = _decode_query(q, num_kv_heads, "decode attention")
+    bsz, H, G, qs = _decode_query(q, num_kv_heads, "decode attention")
     n_pages = _pools(k_pool, v_pool, q.dtype)
     R = bsz * num_kv_heads
     width = _cache_rows(block_table, heads_len, R)
-    out = _decode_out(out, q, bsz)
+    out = _decode_out(out, q, bsz, H)
     _bounds(bounds, n_pages, q.dtype)
     _ints(err, "err", 1, "err needs an entry")
     blocks, counts = _select_lists(q, bounds, R, n_select, sink, recent, blocks, counts)
     L = lib()
-    with _same_device(q, k_pool, v_pool, block_table, heads_len, bounds, blocks, counts, out, err):
-        ws = workspace.get(L.hc_flash_decode_sparse_workspace_size(bsz, num_kv_heads, G, HEAD_DIM, width))
-        qs = q.stride()
-        rc = L.hc_flash_decode_sparse(dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1],
-                                      k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
-                                      heads_len.data_ptr(), bounds.data_ptr(), int(n_select), int(sink), int(recent),
-                                      float(scale), out.data_ptr(), blocks.data_ptr(), counts.data_ptr(),
-                                      ws.data_ptr(), ws.numel(), err.data_ptr(), _raw_stream(q))
-    if rc:
-        check("hc_flash_decode_sparse", rc)
+    ws = _scratch(workspace, q, L.hc_flash_decode_sparse_workspace_size, bsz, num_kv_heads, G, HEAD_DIM, width)
+    _call("hc_flash_decode_sparse", L.hc_flash_decode_sparse,
+          (dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1], k_pool.data_ptr(),
+           v_pool.data_ptr(), n_pages, block_table.data_ptr(), width, heads_len.data_ptr(), bounds.data_ptr(),
+           int(n_select), int(sink), int(recent), float(scale), out.data_ptr(), blocks.data_ptr(), counts.data_ptr(),
+           ws.data_ptr(), ws.numel(), err.data_ptr()), q,
+          (k_pool, v_pool, block_table, heads_len, bounds, blocks, counts, out, err, ws))
     LAUNCHES[0] += 4
     return out, blocks, counts
 
