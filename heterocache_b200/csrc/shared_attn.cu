@@ -258,6 +258,10 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
+  asm volatile("bar.arrive %0, %1;\n" ::"r"(id), "r"(nthreads) : "memory");
+}
+
 // One lane of the (converged) warp.  A branch on it tells the compiler that
 // one thread is active, so that it need not serialise the instructions whose
 // operands are uniform registers (MMAs, commits).
@@ -467,7 +471,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   TcPiece pc;
 
   if (warp == 0 || warp == 2) {
-    // ---- producers (lane 0 issues)
+    // ---- producers (lane 0 issues).  The first queries are asked for before
+    // the tiles: behind those, at the memory's full rate, they came 1.5 to 2
+    // us later.
+    named_bar_sync(2, 256 + 64);
     const bool keys = warp == 0;
     const int NS = keys ? kTcK : vst;
     uint64_t* full = keys ? k_full : v_full;
@@ -544,7 +551,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int tid = threadIdx.x - 128;  // of 256
     const int gq = 16 % p.G, gb = 16 / p.G;
     int kbase = 0, steps = 0;
-    bool dead = false;
+    bool dead = false, started = false;
     while (walk.next(p, pc)) {
       const int nt = pc.t1 - pc.t0;
       const int g0 = pc.ng * p.plan.rows_per;                       // the group's first query row
@@ -559,24 +566,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int b = (g0 + (tid >> 4)) / p.G, g = (g0 + (tid >> 4)) % p.G;
         const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)pc.h * p.G * p.qsh + c * 8;
         unsigned char* dst = sq + (c >> 3) * kTcBox;
-        for (int r0 = tid >> 4; r0 < nq * 128; r0 += 128) {
-          uint4 w[8];  // eight loads in flight
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            w[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (r0 + 16 * i < grows) w[i] = ldg128(q + b * p.qsb + g * p.qsh);
-            g += gq;
-            b += gb;
-            if (g >= p.G) {
-              g -= p.G;
-              ++b;
-            }
+#pragma unroll 4
+        for (int r = tid >> 4; r < nq * 128; r += 16) {
+          const bool ok = r < grows;
+          cp_async16(dst + (r >> 7) * kTcTileBytes + swz128(r & 127, c & 7), ok ? q + b * p.qsb + g * p.qsh : q, ok);
+          g += gq;
+          b += gb;
+          if (g >= p.G) {
+            g -= p.G;
+            ++b;
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(dst + (r0 >> 7) * kTcTileBytes + swz128((r0 + 16 * i) & 127, c & 7)) = w[i];
         }
       }
+      if (!started) {
+        named_bar_arrive(2, 256 + 64);
+        started = true;
+      }
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
@@ -746,6 +752,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       steps += n;
       kbase += nt;
     }
+    if (!started) named_bar_arrive(2, 256 + 64);  // (no piece)
     if (dead && lane == 0) atomicExch(&s_fail, 1);
   }
   tc_fence_before();
