@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kBbThreads) block_bounds_kernel(const BBParams
 
 template <typename T>
 static int bb_launch(const BBParams& p, cudaStream_t st) {
-  const int64_t blocks = p.last > 0 ? (int64_t)(p.last + HC_SPARSE_BLOCK - 2) / HC_SPARSE_BLOCK + 1
+  const int64_t blocks = p.last > 0 ? ((int64_t)p.last + HC_SPARSE_BLOCK - 2) / HC_SPARSE_BLOCK + 1
                                     : (int64_t)p.max_blocks * kBlkPerPage;
   const int64_t cap = (int64_t)p.max_blocks * kBlkPerPage;
   const int rows = p.rows ? p.n_rows : p.R;
