@@ -147,6 +147,24 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+_PAGED = None
+
+
+def paged():
+    """The native calls of the paged operators (``csrc/binding.cpp``), loaded
+    once; raises if they have not been built."""
+    global _PAGED
+    if _PAGED is None:
+        lib()
+        try:
+            from . import _paged
+        except ImportError as e:
+            raise RuntimeError(f"heterocache_b200: the binding _paged.so cannot be loaded ({e}); run "
+                               "`python -c 'import heterocache_b200.build as b; b.build()'` first") from e
+        _PAGED = _paged
+    return _PAGED
+
+
 class HCError(RuntimeError):
     """A status code returned by the C ABI."""
 

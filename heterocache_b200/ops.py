@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._lib import DriftJob, check, lib
+from ._lib import DriftJob, check, lib, paged
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 POOLING = {"avgpool": 0, "maxpool": 1}
@@ -343,86 +343,10 @@ def flash_decode(q, k_pool, v_pool, block_table, heads_len, *, num_kv_heads, out
     return out
 
 
-# The checks of the operators below run on every call of a decode loop, where
-# a launch takes a few microseconds of host time: they read each tensor's
-# properties once and build a message only for a refusal.
-_I32 = torch.int32
-
-
-def _refuse(what: str):
-    raise ValueError(f"heterocache_b200: {what}")
-
-
-def _call(name: str, fn, args, q: torch.Tensor, ts) -> None:
-    """``fn(*args, stream)`` with q's device the current one (the library
-    launches on the current device) and that device's current stream.  Refuses
-    tensors that are elsewhere."""
-    dev = q.get_device()
-    for t in ts:
-        if t is not None and t.get_device() != dev:
-            _refuse(f"tensors on different devices ({q.device} and {t.device})")
-    if dev < 0:
-        for t in ts:
-            if t is not None and t.device != q.device:
-                _refuse(f"tensors on different devices ({q.device} and {t.device})")
-        _refuse("tensors must live on a CUDA device")
-    if dev == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        check(name, rc)
-
-
-def _layout(t: torch.Tensor, name: str):
-    """(shape, strides) of a tensor of contiguous 128-element rows."""
-    shape, st = t.shape, t.stride()
-    if not st or shape[-1] != HEAD_DIM or st[-1] != 1:
-        _refuse(f"{name} must have a contiguous last dim of {HEAD_DIM}")
-    return shape, st
-
-
-def _ints(t: torch.Tensor, name: str, n: int, what: str) -> None:
-    """A contiguous int32 tensor of at least n entries."""
-    if t.dtype is not _I32 or not t.is_contiguous():
-        _refuse(f"{name} must be a contiguous int32 tensor")
-    if t.numel() < n:
-        _refuse(what)
-
-
-def _pool(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
-    """A page pool; returns its number of pages."""
-    s = t.shape
-    if len(s) != 4 or s[1] != PAGE or s[2] != 1 or s[3] != HEAD_DIM or not t.is_contiguous():
-        _refuse(f"{name} must be a contiguous [n_blocks, {PAGE}, 1, {HEAD_DIM}] pool")
-    if t.dtype is not dtype:
-        _refuse(f"{name} must have the dtype of the other operands")
-    return s[0]
-
-
-def _pools(k_pool, v_pool, dtype: torch.dtype) -> int:
-    n = _pool(k_pool, "k_pool", dtype)
-    if _pool(v_pool, "v_pool", dtype) != n:
-        _refuse("k_pool and v_pool must have the same shape")
-    return n
-
-
-def _cache_rows(block_table, heads_len, rows: int) -> int:
-    """The page table's and the lengths' rows; returns the table's width."""
-    s = block_table.shape
-    what = "block_table and heads_len need a row per (batch row, KV head)"
-    _ints(block_table, "block_table", 0, what)
-    if len(s) != 2 or s[0] < rows:
-        _refuse(what)
-    _ints(heads_len, "heads_len", rows, what)
-    return s[1]
-
-
-def _bounds(bounds, n_blocks: int, dtype: torch.dtype) -> None:
-    if (bounds.dtype != dtype or tuple(bounds.shape) != (n_blocks, PAGE // BLOCK, 2, HEAD_DIM)
-            or not bounds.is_contiguous()):
-        _refuse(f"bounds must be a contiguous [n_blocks, {PAGE // BLOCK}, 2, {HEAD_DIM}] tensor in the pool dtype")
+# The paged operators of a decode step run once or more per layer and token,
+# for a few microseconds each: their checks, outputs and C calls are one native
+# function each (csrc/binding.cpp), which returns a status in place of its
+# outputs if the library refused or failed.
 
 
 def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_blocks, free_ptr, err, *,
@@ -443,85 +367,11 @@ def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_
     or a free list that is too short, is reported in ``err`` and leaves the
     cache as it was.  ``workspace`` holds a counter; calls that may overlap
     need a workspace each."""
-    shape, qs = _layout(q, "q")
-    dtype = q.dtype
-    kshape, ks = _layout(k, "k")
-    vshape, vs = _layout(v, "v")
-    if len(shape) != 4 or len(kshape) != 4:
-        _refuse("q, k, v need [bsz, heads, tokens, D]")
-    bsz, H, T, D = shape
-    KV = kshape[1]
-    dt = dtype_code(q)
-    if kshape != vshape or k.dtype is not v.dtype:
-        _refuse("k and v must have the same shape and dtype")
-    if kshape[0] != bsz or kshape[2] != T or k.dtype is not dtype:
-        _refuse("q, k and v must share batch, tokens and dtype")
-    R = bsz * KV
-    if R <= 0 or H <= 0:
-        _refuse("q, k and v need at least one sequence and one head")
-    n_pages = _pools(k_pool, v_pool, dtype)
-    width = _cache_rows(block_table, heads_len, R)
-    _ints(free_blocks, "free_blocks", 0, "")
-    _ints(free_ptr, "free_ptr", 1, "free_ptr and err need an entry")
-    _ints(err, "err", 1, "free_ptr and err need an entry")
-    trig = cos.dtype
-    cb, ct = _trig_strides(cos, "cos", bsz, T, dtype, trig)
-    sb, st = _trig_strides(sin, "sin", bsz, T, dtype, trig)
-    if counts is not None:
-        _ints(counts, "counts", bsz, "counts needs an entry per sequence")
-    if q_out is None:
-        q_out = q.new_empty(shape)
-        os = q_out.stride()
-    else:
-        oshape, os = _layout(q_out, "q_out")
-        if oshape != shape or q_out.dtype is not dtype:
-            _refuse("q_out must have the queries' shape and dtype")
-    if heads_len_out is None:
-        heads_len_out = heads_len
-    else:
-        _ints(heads_len_out, "heads_len_out", R, "heads_len_out needs a row per (batch row, KV head)")
-    if bounds is not None:
-        _bounds(bounds, n_pages, dtype)
-    counter = workspace.counter
-    _call("hc_rope_append", lib().hc_rope_append,
-          (dt, DTYPES[trig], bsz, H, KV, T, D, q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
-           v.data_ptr(), vs[0], vs[1], vs[2], cos.data_ptr(), cb, ct, sin.data_ptr(), sb, st, q_out.data_ptr(), os[0],
-           os[1], os[2], _ptr(counts), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
-           heads_len.data_ptr(), heads_len_out.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(),
-           free_ptr.data_ptr(), _ptr(bounds), counter.data_ptr(), err.data_ptr()), q,
-          (k, v, cos, sin, k_pool, v_pool, block_table, heads_len, heads_len_out, free_blocks, free_ptr, err, counts,
-           q_out, bounds, counter))
+    out = paged().rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_blocks, free_ptr, err,
+                              workspace.counter, counts, q_out, heads_len_out, bounds)
+    if out.__class__ is int:
+        check("hc_rope_append", out)
     LAUNCHES[0] += 1
-    return q_out
-
-
-def _trig_strides(t, name: str, bsz: int, T: int, dtype, trig) -> Tuple[int, int]:
-    """Batch and token stride of cos or sin, [bsz or 1, T, D] or [T, D]."""
-    s, st = _layout(t, name)
-    n = len(s)
-    if (n != 3 and n != 2) or s[-2] != T or (n == 3 and s[0] != 1 and s[0] != bsz):
-        _refuse(f"{name} needs [bsz or 1, tokens, D]")
-    if t.dtype is not trig or (trig is not dtype and trig is not torch.float32):
-        _refuse("cos and sin must share a dtype: the queries', or float32")
-    return (0 if n == 2 or s[0] == 1 else st[0]), st[-2]
-
-
-def _decode_query(q, num_kv_heads: int, name: str):
-    """(bsz, query heads, query heads per KV head, strides) of a decode step's query."""
-    s, st = _layout(q, "q")
-    if len(s) != 4 or s[2] != 1:
-        _refuse(f"{name} takes one query position, [bsz, H, 1, D]")
-    bsz, H = s[0], s[1]
-    if bsz <= 0 or num_kv_heads <= 0 or H <= 0 or H % num_kv_heads:
-        _refuse(f"the {H} query heads do not split evenly over {num_kv_heads} KV heads")
-    return bsz, H, H // num_kv_heads, st
-
-
-def _decode_out(out, q, bsz: int, H: int) -> torch.Tensor:
-    if out is None:
-        return q.new_empty((bsz, H, HEAD_DIM))
-    if not out.is_contiguous() or out.numel() != bsz * H * HEAD_DIM or out.dtype is not q.dtype:
-        _refuse("out must be a contiguous [bsz, H, D] buffer in the query dtype")
     return out
 
 
@@ -533,37 +383,12 @@ def flash_decode_shared(q, k_pool, v_pool, block_table, heads_len, shared_len, *
     the first sequence's rows of the page table.  Each row's own tokens follow
     from position shared_len[h] to heads_len[r] - 1; with k_new / v_new [bsz,
     KV, 1, D] one more token a row, not in the pages."""
-    bsz, H, G, qs = _decode_query(q, num_kv_heads, "decode attention")
-    n_pages = _pools(k_pool, v_pool, q.dtype)
-    width = _cache_rows(block_table, heads_len, bsz * num_kv_heads)
-    out = _decode_out(out, q, bsz, H)
-    _ints(shared_len, "shared_len", num_kv_heads, "shared_len needs an entry per KV head")
-    _ints(err, "err", 1, "err needs an entry")
-    if (k_new is None) != (v_new is None):
-        _refuse("k_new and v_new come together")
-    kn = vn = (0, 0)
-    if k_new is not None:
-        kn, vn = _layout(k_new, "k_new")[1], _layout(v_new, "v_new")[1]
-        _same_shape(k_new, v_new)
-        if tuple(k_new.shape) != (bsz, num_kv_heads, 1, HEAD_DIM) or k_new.dtype is not q.dtype:
-            _refuse("k_new/v_new must be [bsz, KV, 1, D] in the query dtype")
-    dt = dtype_code(q)
-    L = lib()
-    ws = _scratch(workspace, q, L.hc_flash_decode_shared_workspace_size, dt, bsz, num_kv_heads, G, HEAD_DIM)
-    _call("hc_flash_decode_shared", L.hc_flash_decode_shared,
-          (dt, bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1], k_pool.data_ptr(), v_pool.data_ptr(),
-           n_pages, block_table.data_ptr(), width, heads_len.data_ptr(), shared_len.data_ptr(), _ptr(k_new),
-           _ptr(v_new), kn[0], kn[1], vn[0], vn[1], float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
-           err.data_ptr()), q,
-          (k_pool, v_pool, block_table, heads_len, shared_len, out, err, k_new, v_new, ws))
+    out = paged().flash_decode_shared(q, k_pool, v_pool, block_table, heads_len, shared_len, num_kv_heads, out, scale,
+                                      workspace, err, k_new, v_new)
+    if out.__class__ is int:
+        check("hc_flash_decode_shared", out)
     LAUNCHES[0] += 3
     return out
-
-
-def _scratch(workspace: Workspace, q, size, *args) -> torch.Tensor:
-    """The workspace, as large as ``size(*args)`` says; nothing is asked of it
-    for a query that is not on a CUDA device (the call then refuses)."""
-    return workspace.get(size(*args)) if q.is_cuda else q
 
 
 def block_bounds(k_pool, block_table, heads_len, bounds, err, *, rows=None, last: int = 0) -> torch.Tensor:
@@ -571,39 +396,11 @@ def block_bounds(k_pool, block_table, heads_len, bounds, err, *, rows=None, last
     into ``bounds`` [n_blocks, 4, 2, D]: of every row, or of those listed in
     ``rows`` (int32); of all its blocks, or of those that hold its last
     ``last`` tokens."""
-    n_pages = _pool(k_pool, "k_pool", k_pool.dtype)
-    n = block_table.shape[0]
-    width = _cache_rows(block_table, heads_len, n)
-    _bounds(bounds, n_pages, k_pool.dtype)
-    _ints(err, "err", 1, "err needs an entry")
-    if last < 0:
-        _refuse("last must not be negative")
-    if rows is not None:
-        _ints(rows, "rows", 0, "")
-    _call("hc_block_bounds", lib().hc_block_bounds,
-          (dtype_code(k_pool), n, HEAD_DIM, k_pool.data_ptr(), n_pages, block_table.data_ptr(), width,
-           heads_len.data_ptr(), _ptr(rows), 0 if rows is None else rows.numel(), int(last), bounds.data_ptr(),
-           err.data_ptr()), k_pool, (block_table, heads_len, bounds, err, rows))
+    out = paged().block_bounds(k_pool, block_table, heads_len, bounds, err, rows, last)
+    if out.__class__ is int:
+        check("hc_block_bounds", out)
     LAUNCHES[0] += 1
-    return bounds
-
-
-def _select_lists(q, bounds, R: int, n_select: int, sink: int, recent: int, blocks, counts):
-    """Checks of the selection's own operands; returns (blocks, counts)."""
-    if n_select < 1 or sink < 0 or recent < 0 or sink + recent > n_select:
-        _refuse("sink + recent blocks must not be more than n_select, which must be at least 1")
-    what = "blocks needs [rows, n_select] and counts an entry per row"
-    if blocks is None:
-        blocks = q.new_empty((R, n_select), dtype=_I32)
-    else:
-        _ints(blocks, "blocks", 0, what)
-        if tuple(blocks.shape) != (R, n_select):
-            _refuse(what)
-    if counts is None:
-        counts = q.new_empty(R, dtype=_I32)
-    else:
-        _ints(counts, "counts", R, what)
-    return blocks, counts
+    return out
 
 
 def block_select(q, bounds, block_table, heads_len, *, num_kv_heads, n_select: int, sink: int = 1, recent: int = 1,
@@ -612,22 +409,12 @@ def block_select(q, bounds, block_table, heads_len, *, num_kv_heads, n_select: i
     each row the first ``sink``, the last ``recent`` and those of the highest
     bound on their scores, n_select in all.  Returns (blocks [rows, n_select]
     int32 ascending, -1 behind; counts [rows] int32)."""
-    bsz, _, G, qs = _decode_query(q, num_kv_heads, "block_select")
-    R = bsz * num_kv_heads
-    width = _cache_rows(block_table, heads_len, R)
-    n_pages = bounds.shape[0]
-    _bounds(bounds, n_pages, q.dtype)
-    _ints(err, "err", 1, "err needs an entry")
-    blocks, counts = _select_lists(q, bounds, R, n_select, sink, recent, blocks, counts)
-    L = lib()
-    ws = _scratch(workspace, q, L.hc_block_select_workspace_size, bsz, num_kv_heads, width)
-    _call("hc_block_select", L.hc_block_select,
-          (dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1], bounds.data_ptr(), n_pages,
-           block_table.data_ptr(), width, heads_len.data_ptr(), int(n_select), int(sink), int(recent),
-           blocks.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr()), q,
-          (bounds, block_table, heads_len, err, blocks, counts, ws))
+    out = paged().block_select(q, bounds, block_table, heads_len, num_kv_heads, n_select, sink, recent, workspace, err,
+                               blocks, counts)
+    if out.__class__ is int:
+        check("hc_block_select", out)
     LAUNCHES[0] += 2
-    return blocks, counts
+    return out
 
 
 def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, counts, *, num_kv_heads, out=None,
@@ -635,25 +422,10 @@ def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, count
     """Decode attention over each row's listed 64-token blocks alone
     (hc_flash_decode_blocks): blocks [rows, n] int32 ascending, the first
     counts[row] of them used."""
-    bsz, H, G, qs = _decode_query(q, num_kv_heads, "decode attention")
-    n_pages = _pools(k_pool, v_pool, q.dtype)
-    R = bsz * num_kv_heads
-    width = _cache_rows(block_table, heads_len, R)
-    out = _decode_out(out, q, bsz, H)
-    what = "blocks needs [rows, n] and counts an entry per row"
-    _ints(blocks, "blocks", 1, what)
-    _ints(counts, "counts", R, what)
-    _ints(err, "err", 1, "err needs an entry")
-    if blocks.dim() != 2 or blocks.shape[0] < R:
-        _refuse(what)
-    L = lib()
-    ws = _scratch(workspace, q, L.hc_flash_decode_workspace_size, bsz, num_kv_heads, G, HEAD_DIM)
-    _call("hc_flash_decode_blocks", L.hc_flash_decode_blocks,
-          (dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1], k_pool.data_ptr(),
-           v_pool.data_ptr(), n_pages, block_table.data_ptr(), width, heads_len.data_ptr(), blocks.data_ptr(),
-           counts.data_ptr(), blocks.shape[1], float(scale), out.data_ptr(), ws.data_ptr(), ws.numel(),
-           err.data_ptr()), q,
-          (k_pool, v_pool, block_table, heads_len, blocks, counts, out, err, ws))
+    out = paged().flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, counts, num_kv_heads, out, scale,
+                                      workspace, err)
+    if out.__class__ is int:
+        check("hc_flash_decode_blocks", out)
     LAUNCHES[0] += 2
     return out
 
@@ -664,24 +436,12 @@ def flash_decode_sparse(q, k_pool, v_pool, block_table, heads_len, bounds, *, nu
     """Block-sparse decode attention (hc_flash_decode_sparse): what
     ``block_select`` and then ``flash_decode_blocks`` over its lists give.
     Returns (out [bsz, H, D], blocks [rows, n_select], counts [rows])."""
-    bsz, H, G, qs = _decode_query(q, num_kv_heads, "decode attention")
-    n_pages = _pools(k_pool, v_pool, q.dtype)
-    R = bsz * num_kv_heads
-    width = _cache_rows(block_table, heads_len, R)
-    out = _decode_out(out, q, bsz, H)
-    _bounds(bounds, n_pages, q.dtype)
-    _ints(err, "err", 1, "err needs an entry")
-    blocks, counts = _select_lists(q, bounds, R, n_select, sink, recent, blocks, counts)
-    L = lib()
-    ws = _scratch(workspace, q, L.hc_flash_decode_sparse_workspace_size, bsz, num_kv_heads, G, HEAD_DIM, width)
-    _call("hc_flash_decode_sparse", L.hc_flash_decode_sparse,
-          (dtype_code(q), bsz, num_kv_heads, G, HEAD_DIM, q.data_ptr(), qs[0], qs[1], k_pool.data_ptr(),
-           v_pool.data_ptr(), n_pages, block_table.data_ptr(), width, heads_len.data_ptr(), bounds.data_ptr(),
-           int(n_select), int(sink), int(recent), float(scale), out.data_ptr(), blocks.data_ptr(), counts.data_ptr(),
-           ws.data_ptr(), ws.numel(), err.data_ptr()), q,
-          (k_pool, v_pool, block_table, heads_len, bounds, blocks, counts, out, err, ws))
+    out = paged().flash_decode_sparse(q, k_pool, v_pool, block_table, heads_len, bounds, num_kv_heads, n_select, sink,
+                                      recent, out, scale, workspace, err, blocks, counts)
+    if out.__class__ is int:
+        check("hc_flash_decode_sparse", out)
     LAUNCHES[0] += 4
-    return out, blocks, counts
+    return out
 
 
 def drift_check(qbuf, k_pool, block_table, *, num_kv_heads, groups, steps, seq_len, pooling, kernel_size, topk,
