@@ -19,9 +19,9 @@
 // heads) of a thread in flight: 16 x 4096 tokens of 32 + 8 heads, 1.36 GB,
 // take 238 us (88% of the copy rate; with fp32 minima and one token in
 // flight at 111 registers, 441 us).  Every key/value CTA derives the page allocation for
-// itself from the state the call found; the last of them to finish (a
-// counter) writes the page table, the lengths and the
-// free-list pointer, so nothing is written while another CTA still reads.
+// itself from the state the call found; the last of them to have read it (a
+// counter) writes the page table, the lengths and the free-list pointer, so
+// nothing is written while another CTA still reads.
 #include "hc_host.cuh"
 #include "hc_params.cuh"
 
@@ -30,6 +30,7 @@ namespace hc {
 constexpr int kRaThreads = 256;
 constexpr int kRaWarps = kRaThreads / 32;
 constexpr int kRaHeads = 4;  // query heads of one query unit
+constexpr int kRaRun = 4;    // most blocks of a key/value CTA
 
 template <typename T> struct RaRow {
   static constexpr int E = 16 / (int)sizeof(T);     // elements of a 16-byte chunk
@@ -239,19 +240,23 @@ __device__ __forceinline__ int ra_page(const RAParams& p, int r, int len, int pg
   return p.free_blocks[take];
 }
 
-// The last key/value CTA to get here: page table, lengths, free-list pointer.
-__device__ __forceinline__ void ra_finish(const RAParams& p, int status, int base, int total, int* s_warp) {
-  __shared__ int s_last;
+// Called by all threads of a key/value CTA once each has read what it needs of
+// the lengths, the page table and the free list, and before any of its stores
+// (so the fence finds none in flight).  *last: the CTA is the last of the launch
+// to get here, known after the next barrier.
+__device__ __forceinline__ void ra_arrive(const RAParams& p, int* last) {
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
     const unsigned int n = atomicAdd(p.done, 1u);
-    s_last = n == (unsigned int)p.kv_ctas - 1;
-    if (s_last) *p.done = 0u;
+    *last = n == (unsigned int)p.kv_ctas - 1;
+    if (*last) *p.done = 0u;
     __threadfence();
   }
-  __syncthreads();
-  if (!s_last) return;
+}
+
+// The last CTA to arrive: page table, lengths, free-list pointer.
+__device__ __forceinline__ void ra_finish(const RAParams& p, int status, int base, int total, int* s_warp) {
   if (status) {
     if (threadIdx.x == 0) set_err(p.err, status);
     return;
@@ -319,13 +324,12 @@ __device__ __forceinline__ void ra_query_unit(const RAParams& p, int unit) {
 // chunk c of both halves of the key, the other CH2 those of the value; two
 // tokens a thread are in flight.
 template <typename T, typename TT>
-__device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int cnt, int blk, int take,
+__device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int cnt, int blk, int phys,
                                          uint32_t* s_mm) {
   constexpr int E = RaRow<T>::E, CH2 = RaRow<T>::CH2, PER = 2 * CH2, TOK = kRaThreads / PER;
   constexpr int RW = kD * (int)sizeof(T) / 4;  // 32-bit words of a row
   const int b = r / p.KV, h = r % p.KV;
   const int beg = max(blk * HC_SPARSE_BLOCK, len), end = min((blk + 1) * HC_SPARSE_BLOCK, len + cnt);
-  const int phys = ra_page(p, r, len, beg >> 8, take);
   const int c = threadIdx.x % PER;
   const bool key = c < CH2;
   const int d0 = (key ? c : c - CH2) * E;
@@ -416,60 +420,74 @@ __host__ __device__ constexpr int ra_rows() {
 
 // One token a sequence: a row's token takes as many threads as a token of
 // ra_block, and a CTA a run of rows from r0 on (16 of a 16-bit cache), so
-// that few CTAs go through all rows for the allocation.  `take`: the free
-// list's index of row r0's first free page.
-template <typename T, typename TT>
-__device__ __forceinline__ void ra_token(const RAParams& p, int r0, int take) {
-  constexpr int E = RaRow<T>::E, CH2 = RaRow<T>::CH2, PER = 2 * CH2;
-  constexpr int RW = kD * (int)sizeof(T) / 4;
-  const int r = r0 + (int)threadIdx.x / PER;
-  if (r >= p.B * p.KV) return;
-  const int b = r / p.KV, h = r % p.KV;
-  if (ra_count(p, b) == 0) return;
-  const int pos = p.heads_len[r];
-  int phys = p.bt[(int64_t)r * p.max_blocks + (pos >> 8)];
-  if (phys == -1) {
+// that few CTAs go through all rows for the allocation.  What is appended does
+// not hang on the allocation: it is loaded first.
+template <typename T, typename TT> struct RaToken {
+  static constexpr int E = RaRow<T>::E, CH2 = RaRow<T>::CH2, PER = 2 * CH2;
+  static constexpr int RW = kD * (int)sizeof(T) / 4;
+  int r, b, c, pos, phys;
+  bool ok, key;
+  uint4 w1, w2;
+  Trig<TT, E> g;
+
+  __device__ __forceinline__ void load(const RAParams& p, int r0) {
+    r = r0 + (int)threadIdx.x / PER;
+    c = threadIdx.x % PER;
+    key = c < CH2;
+    ok = r < p.B * p.KV;
+    if (!ok) return;
+    b = r / p.KV;
+    const int h = r % p.KV;
+    const int d0 = (key ? c : c - CH2) * E;
+    const T* src = key ? reinterpret_cast<const T*>(p.k) + b * p.ksb + h * p.ksh + d0
+                       : reinterpret_cast<const T*>(p.v) + b * p.vsb + h * p.vsh + d0;
+    w1 = ldg128(src);
+    w2 = ldg128(src + kD / 2);
+    if (key) load_rotation<TT, E>(p, b, 0, d0, g);
+    ok = ra_count(p, b) > 0;
+  }
+  // Where the token goes; `take`: the free list's index of row r0's first free page.
+  __device__ __forceinline__ void place(const RAParams& p, int r0, int take) {
+    if (!ok) return;
+    pos = p.heads_len[r];
+    phys = p.bt[(int64_t)r * p.max_blocks + (pos >> 8)];
+    if (phys != -1) return;
     bool bad = false;
     for (int k = r0; k < r; ++k) take += ra_need(p, k, bad);
     phys = p.free_blocks[take];
   }
-  const int c = threadIdx.x % PER;
-  const bool key = c < CH2;
-  const int d0 = (key ? c : c - CH2) * E;
-  const T* src = key ? reinterpret_cast<const T*>(p.k) + b * p.ksb + h * p.ksh + d0
-                     : reinterpret_cast<const T*>(p.v) + b * p.vsb + h * p.vsh + d0;
-  uint4 w1 = ldg128(src), w2 = ldg128(src + kD / 2);
-  if (key) {
-    Trig<TT, E> g;
-    load_rotation<TT, E>(p, b, 0, d0, g);
-    rotate<T, TT, E>(g, w1, w2);
+  __device__ __forceinline__ void store(const RAParams& p) {
+    if (!ok) return;
+    const int d0 = (key ? c : c - CH2) * E;
+    if (key) rotate<T, TT, E>(g, w1, w2);
+    T* dst = reinterpret_cast<T*>(key ? p.kp : p.vp) + ((int64_t)phys * kPage + (pos & (kPage - 1))) * kD + d0;
+    *reinterpret_cast<uint4*>(dst) = w1;
+    *reinterpret_cast<uint4*>(dst + kD / 2) = w2;
+    if (!key || !p.bounds) return;
+    uint32_t* lim = reinterpret_cast<uint32_t*>(p.bounds) +
+                    ((int64_t)phys * (kPage / HC_SPARSE_BLOCK) + ((pos & (kPage - 1)) / HC_SPARSE_BLOCK)) * 2 * RW +
+                    c * 4;
+    merge(lim, w1);
+    merge(lim + RW / 2, w2);
   }
-  T* dst = reinterpret_cast<T*>(key ? p.kp : p.vp) + ((int64_t)phys * kPage + (pos & (kPage - 1))) * kD + d0;
-  *reinterpret_cast<uint4*>(dst) = w1;
-  *reinterpret_cast<uint4*>(dst + kD / 2) = w2;
-  if (!key || !p.bounds) return;
-  uint32_t* lim = reinterpret_cast<uint32_t*>(p.bounds) +
-                  ((int64_t)phys * (kPage / HC_SPARSE_BLOCK) + ((pos & (kPage - 1)) / HC_SPARSE_BLOCK)) * 2 * RW + c * 4;
-  const bool more = (pos & (HC_SPARSE_BLOCK - 1)) != 0;  // the block held tokens before
-  auto merge = [&](uint32_t* at, const uint4& w) {
+  __device__ __forceinline__ void merge(uint32_t* at, const uint4& w) {
     uint4 lo = w, hi = w;
-    if (more) {
+    if ((pos & (HC_SPARSE_BLOCK - 1)) != 0) {  // the block held tokens before
       const uint4 a = *reinterpret_cast<const uint4*>(at), z = *reinterpret_cast<const uint4*>(at + RW);
       lo = make_uint4(Word<T>::min(a.x, w.x), Word<T>::min(a.y, w.y), Word<T>::min(a.z, w.z), Word<T>::min(a.w, w.w));
       hi = make_uint4(Word<T>::max(z.x, w.x), Word<T>::max(z.y, w.y), Word<T>::max(z.z, w.z), Word<T>::max(z.w, w.w));
     }
     *reinterpret_cast<uint4*>(at) = lo;
     *reinterpret_cast<uint4*>(at + RW) = hi;
-  };
-  merge(lim, w1);
-  merge(lim + RW / 2, w2);
-}
+  }
+};
 
 template <typename T, typename TT>
 __global__ void __launch_bounds__(kRaThreads, 3) rope_append_kernel(const RAParams p) {
   __shared__ int2 s_red[kRaWarps];
   __shared__ int s_warp[32];
   __shared__ uint32_t s_mm[kRaWarps * 2 * kD * sizeof(T) / 4];
+  __shared__ int s_phys[kRaRun], s_last;
   pdl_wait();
   pdl_trigger();
   if ((int)blockIdx.x >= p.kv_ctas) {
@@ -480,19 +498,31 @@ __global__ void __launch_bounds__(kRaThreads, 3) rope_append_kernel(const RAPara
   const bool single = p.T == 1;
   const int r = single ? (int)blockIdx.x * ra_rows<T>() : (int)blockIdx.x / per_row;
   const int u0 = (blockIdx.x % per_row) * p.run;
+  RaToken<T, TT> tok;
+  if (single) tok.load(p, r);
   const int base = *p.free_ptr;
   int before, total;
   const int status = ra_plan(p, r, base, s_red, before, total);
+  int len = 0, cnt = 0;
   if (!status && single) {
-    ra_token<T, TT>(p, r, base + before);
+    tok.place(p, r, base + before);
   } else if (!status) {
-    const int len = p.heads_len[r], cnt = ra_count(p, r / p.KV);
+    len = p.heads_len[r], cnt = ra_count(p, r / p.KV);
+    const int blk = len / HC_SPARSE_BLOCK + u0 + (int)threadIdx.x;
+    if (threadIdx.x < p.run && cnt > 0 && blk * HC_SPARSE_BLOCK < len + cnt)
+      s_phys[threadIdx.x] = ra_page(p, r, len, max(blk * HC_SPARSE_BLOCK, len) >> 8, base + before);
+  }
+  ra_arrive(p, &s_last);
+  if (!status && single) {
+    tok.store(p);
+  } else if (!status) {
     for (int u = u0; u < min(u0 + p.run, p.units); ++u) {
       const int blk = len / HC_SPARSE_BLOCK + u;
-      if (cnt > 0 && blk * HC_SPARSE_BLOCK < len + cnt) ra_block<T, TT>(p, r, len, cnt, blk, base + before, s_mm);
+      if (cnt > 0 && blk * HC_SPARSE_BLOCK < len + cnt) ra_block<T, TT>(p, r, len, cnt, blk, s_phys[u - u0], s_mm);
     }
   }
-  ra_finish(p, status, base, total, s_warp);
+  __syncthreads();
+  if (s_last) ra_finish(p, status, base, total, s_warp);
 }
 
 template <typename T, typename TT>
@@ -502,7 +532,7 @@ static int ra_launch(RAParams& p, cudaStream_t st) {
   p.units = (p.T + HC_SPARSE_BLOCK - 2) / HC_SPARSE_BLOCK + 1;  // blocks that T tokens can touch
   // a CTA finds the allocation once for a run of 4 blocks, where there are
   // still CTAs enough to fill the GPU
-  p.run = R * p.units >= 4 * 8 * (int64_t)device_sms(current_device()) ? 4 : 1;
+  p.run = R * p.units >= kRaRun * 8 * (int64_t)device_sms(current_device()) ? kRaRun : 1;
   const int64_t kv = p.T == 1 ? (R + ra_rows<T>() - 1) / ra_rows<T>() : R * ((p.units + p.run - 1) / p.run);
   const int64_t q = (((int64_t)p.B * p.T + TOK - 1) / TOK) * ((p.H + kRaHeads - 1) / kRaHeads);
   if (kv + q > 0x7fffffffLL) return HC_ERR_UNSUPPORTED;
