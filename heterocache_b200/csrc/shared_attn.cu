@@ -12,7 +12,6 @@
 
 namespace hc {
 
-constexpr int kSpThreads = 256;
 constexpr int kSpTok = 32;   // tokens of a tile
 // row pitch of queries and keys in shared memory (elements): 16 bytes more
 // than a row, so that rows start on 16-byte boundaries in different banks
@@ -41,17 +40,49 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ok) 
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0)
                : "memory");
 }
-__device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+// Two fp32 values in one 64-bit register: a * b + c, a + b and a * b of both.
+__device__ __forceinline__ uint64_t pack_f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
-// CUDA-core form, for fp32: RPT query rows a thread (16 * RPT a CTA), tiles
-// of 32 tokens, two of them in shared memory by cp.async.  Thread (ty, tx) of
-// the 16 x 16 holds rows ty * RPT + i, scores of tokens tx and tx + 16,
-// outputs of dims 4 tx .. and 64 + 4 tx ..  Bound by the fp32 units from some
-// ten rows on (4 flops a byte and row), by latency where there are few tiles:
-// 24 rows x 3000 tokens x 8 heads take 20 us.
-template <int RPT>
-__global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPParams p) {
-  constexpr int RT = 16 * RPT;
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Four floats of shared memory as two pairs.
+__device__ __forceinline__ ulonglong2 lds4(const float* p) { return *reinterpret_cast<const ulonglong2*>(p); }
+
+// CUDA-core form, for fp32: RT query rows a CTA, a warp for 4 RPT of them,
+// tiles of 32 tokens, two of them in shared memory by cp.async.  Thread
+// (ty, tx) of a warp's 4 x 8 holds rows RPT ty + i: scores of tokens tx + 8 u,
+// then outputs of dims 4 tx + 32 c ..  Bound by what comes out of shared memory
+// (a 16-byte load of a warp takes 4 clocks, broadcast or not), so a thread's
+// tile is large: 4 x 4 scores for 8 loads, 4 x 16 outputs for 20 loads of 4
+// tokens.  With 16 rows two a thread, for twice the warps.  20000 tokens x 8
+// heads take 68 us for up to 16 rows (102 with one row a thread and 16 x 16
+// threads), 145 for 64 (161; 179 with eight a thread, too few warps); 3000
+// tokens x 8 heads for 24 rows 28 (31).
+template <int RT, int RPT>
+__global__ void __launch_bounds__(8 * RT / RPT, 2) shared_prefix_kernel(const SPParams p) {
+  constexpr int kThreads = 8 * RT / RPT;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   float* sq = reinterpret_cast<float*>(smem_raw);
   float* sk = sq + RT * kSpPad;
@@ -63,7 +94,8 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
   const int span = (total + gridDim.x - 1) / (int)gridDim.x;
   const int beg = blockIdx.x * span, end = min(total, beg + span);
   if (beg >= end) return;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int tx = threadIdx.x & 7;
+  const int row0 = RPT * (threadIdx.x >> 3);  // the thread's first row
   const int NG = p.plan.n_groups;
   int start = 0;  // first tile of the head's segments
   for (int h = 0; h < p.KV; ++h) {
@@ -74,7 +106,7 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
       if (t0 >= t1) continue;
       __syncthreads();
       constexpr int CH = kD / 4, CE = 4;
-      for (int i = threadIdx.x; i < RT * CH; i += kSpThreads) {
+      for (int i = threadIdx.x; i < RT * CH; i += kThreads) {
         const int row = ng * RT + i / CH, c = i % CH;
         const bool ok = row < p.B * p.G;
         const int b = ok ? row / p.G : 0, g = ok ? row % p.G : 0;
@@ -87,7 +119,8 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
         const bool in = blk >= 0 && blk < p.n_blocks;
         if (!in && threadIdx.x == 0) set_err(p.err, HC_ERR_RANGE);
         const int64_t off = ((int64_t)(in ? blk : 0) * kPage + (pos & (kPage - 1))) * kD;
-        for (int i = threadIdx.x; i < kSpTok * CH; i += kSpThreads) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < kSpTok * CH; i += kThreads) {
           const int row = i / CH, c = i % CH;
           const bool ok = in && pos + row < len;
           cp_async16(sk + (s * kSpTok + row) * kSpPad + c * CE, reinterpret_cast<const float*>(p.kp) + off + row * kD + c * CE, ok);
@@ -96,13 +129,14 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
         asm volatile("cp.async.commit_group;\n" ::: "memory");
         return in ? min(kSpTok, len - pos) : 0;
       };
-      float m[RPT], l[RPT], o[RPT][8];
+      float m[RPT], l[RPT];
+      uint64_t o[RPT][8];  // pairs of dims
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[i][d] = 0.f;
+        for (int d = 0; d < 8; ++d) o[i][d] = 0ull;
       }
       int valid = load(t0, 0);
       for (int t = t0; t < t1; ++t) {
@@ -117,57 +151,68 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
         __syncthreads();
         const float* kt = sk + s * kSpTok * kSpPad;
         const float* vt = sv + s * kSpTok * kD;
-        float a[RPT][2];
+        uint64_t a[RPT][4];  // sums over even and odd dims
 #pragma unroll
-        for (int i = 0; i < RPT; ++i) a[i][0] = a[i][1] = 0.f;
+        for (int i = 0; i < RPT; ++i)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) a[i][u] = 0ull;
 #pragma unroll 4
         for (int d = 0; d < kD; d += 4) {
-          const float4 k0 = lds4(kt + tx * kSpPad + d), k1 = lds4(kt + (tx + 16) * kSpPad + d);
+          ulonglong2 k[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) k[u] = lds4(kt + (tx + 8 * u) * kSpPad + d);
 #pragma unroll
           for (int i = 0; i < RPT; ++i) {
-            const float4 q = lds4(sq + (ty * RPT + i) * kSpPad + d);
-            a[i][0] = fmaf(q.x, k0.x, fmaf(q.y, k0.y, fmaf(q.z, k0.z, fmaf(q.w, k0.w, a[i][0]))));
-            a[i][1] = fmaf(q.x, k1.x, fmaf(q.y, k1.y, fmaf(q.z, k1.z, fmaf(q.w, k1.w, a[i][1]))));
+            const ulonglong2 q = lds4(sq + (row0 + i) * kSpPad + d);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) a[i][u] = fma_f2(q.y, k[u].y, fma_f2(q.x, k[u].x, a[i][u]));
           }
         }
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-          const float s0 = tx < valid ? a[i][0] * p.scale_log2 : -INFINITY;
-          const float s1 = tx + 16 < valid ? a[i][1] * p.scale_log2 : -INFINITY;
-          float mx = fmaxf(s0, s1);
+          float x[4], mx = -INFINITY;
 #pragma unroll
-          for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          for (int u = 0; u < 4; ++u) {
+            const float2 v = unpack_f2(a[i][u]);
+            x[u] = tx + 8 * u < valid ? (v.x + v.y) * p.scale_log2 : -INFINITY;
+            mx = fmaxf(mx, x[u]);
+          }
+#pragma unroll
+          for (int y = 4; y > 0; y >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, y));
           const float mn = fmaxf(m[i], mx);
           const float ref = mn == -INFINITY ? 0.f : mn;
           const float corr = exp2f(m[i] - ref);
-          const float p0 = exp2f(s0 - ref), p1 = exp2f(s1 - ref);
           m[i] = mn;
-          l[i] = l[i] * corr + p0 + p1;  // this thread's tokens; summed over tx at the end
-#pragma unroll
-          for (int d = 0; d < 8; ++d) o[i][d] *= corr;
-          sp[(ty * RPT + i) * kSpPP + tx] = p0;
-          sp[(ty * RPT + i) * kSpPP + tx + 16] = p1;
-        }
-        __syncwarp();  // a row's 16 threads are lanes of one warp
-#pragma unroll 2
-        for (int j = 0; j < kSpTok; j += 4) {
-          float4 pr[RPT];
-#pragma unroll
-          for (int i = 0; i < RPT; ++i) pr[i] = *reinterpret_cast<const float4*>(sp + (ty * RPT + i) * kSpPP + j);
+          l[i] *= corr;  // this thread's tokens; summed over tx at the end
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float4 v0 = lds4(vt + (j + u) * kD + 4 * tx), v1 = lds4(vt + (j + u) * kD + 64 + 4 * tx);
+            const float e = exp2f(x[u] - ref);
+            l[i] += e;
+            sp[(row0 + i) * kSpPP + tx + 8 * u] = e;
+          }
+#pragma unroll
+          for (int d = 0; d < 8; ++d) o[i][d] = mul_f2(o[i][d], pack_f2(corr, corr));
+        }
+        __syncwarp();  // a row's threads are lanes of one warp
+#pragma unroll 2
+        for (int j = 0; j < kSpTok; j += 4) {
+          float pr[RPT][4];
+#pragma unroll
+          for (int i = 0; i < RPT; ++i)
+            *reinterpret_cast<float4*>(pr[i]) = *reinterpret_cast<const float4*>(sp + (row0 + i) * kSpPP + j);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            ulonglong2 v[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = lds4(vt + (j + u) * kD + 32 * c + 4 * tx);
 #pragma unroll
             for (int i = 0; i < RPT; ++i) {
-              const float w = u == 0 ? pr[i].x : u == 1 ? pr[i].y : u == 2 ? pr[i].z : pr[i].w;
-              o[i][0] = fmaf(w, v0.x, o[i][0]);
-              o[i][1] = fmaf(w, v0.y, o[i][1]);
-              o[i][2] = fmaf(w, v0.z, o[i][2]);
-              o[i][3] = fmaf(w, v0.w, o[i][3]);
-              o[i][4] = fmaf(w, v1.x, o[i][4]);
-              o[i][5] = fmaf(w, v1.y, o[i][5]);
-              o[i][6] = fmaf(w, v1.z, o[i][6]);
-              o[i][7] = fmaf(w, v1.w, o[i][7]);
+              const uint64_t w = pack_f2(pr[i][u], pr[i][u]);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                o[i][2 * c] = fma_f2(w, v[c].x, o[i][2 * c]);
+                o[i][2 * c + 1] = fma_f2(w, v[c].y, o[i][2 * c + 1]);
+              }
             }
           }
         }
@@ -179,14 +224,15 @@ __global__ void __launch_bounds__(kSpThreads, 2) shared_prefix_kernel(const SPPa
       for (int i = 0; i < RPT; ++i) {
         float s = l[i];
 #pragma unroll
-        for (int x = 8; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        const int row = ty * RPT + i;
+        for (int y = 4; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
+        const int row = row0 + i;
         if (ng * RT + row >= p.B * p.G) continue;
         if (tx == 0) p.plan.part_ml[slot * RT + row] = make_float2(m[i], s);
-        // dims 4 tx .. of each half: half an 8-dim group of the layout
+        // dims 4 tx + 32 c ..: half an 8-dim group of the layout
         float* dst = p.plan.part_o + slot * RT * kD + ((int64_t)(tx >> 1) * RT + row) * 8 + (tx & 1) * 4;
-        *reinterpret_cast<float4*>(dst) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-        *reinterpret_cast<float4*>(dst + (int64_t)8 * RT * 8) = make_float4(o[i][4], o[i][5], o[i][6], o[i][7]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<ulonglong2*>(dst + (int64_t)4 * c * RT * 8) = make_ulonglong2(o[i][2 * c], o[i][2 * c + 1]);
       }
     }
   }
@@ -234,28 +280,6 @@ constexpr uint32_t kTcColS = 0, kTcColO = 256;
 // The same answer for the whole warp (each lane polls for itself).
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit_ns));
-}
-
-// Two fp32 values in one 64-bit register: a * b + c and a + b of both.
-__device__ __forceinline__ uint64_t pack_f2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpack_f2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-  return r;
 }
 
 __device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
@@ -831,12 +855,12 @@ static int sp_pdl_launch(K kern, int grid, int threads, size_t smem, cudaStream_
   return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? HC_OK : HC_ERR_CUDA;
 }
 
-template <int RPT>
+template <int RT, int RPT>
 static int sp_launch_f32(const SPParams& p, int dev, cudaStream_t st) {
   static bool done[kMaxDevices];
-  constexpr size_t smem = sp_smem(16 * RPT);
-  if (!sp_allow_smem(shared_prefix_kernel<RPT>, smem, done, dev)) return HC_ERR_CUDA;
-  return sp_pdl_launch(shared_prefix_kernel<RPT>, p.plan.n_ctas, kSpThreads, smem, st, p);
+  constexpr size_t smem = sp_smem(RT);
+  if (!sp_allow_smem(shared_prefix_kernel<RT, RPT>, smem, done, dev)) return HC_ERR_CUDA;
+  return sp_pdl_launch(shared_prefix_kernel<RT, RPT>, p.plan.n_ctas, 8 * RT / RPT, smem, st, p);
 }
 
 template <typename T>
@@ -863,9 +887,9 @@ int shared_prefix_dispatch(int dtype, SPParams& p, void* ws, size_t ws_bytes, cu
   switch (dtype) {
     case HC_F32:
       switch (p.plan.rows_per) {
-        case 16: return sp_launch_f32<1>(p, dev, st);
-        case 32: return sp_launch_f32<2>(p, dev, st);
-        default: return sp_launch_f32<4>(p, dev, st);
+        case 16: return sp_launch_f32<16, 2>(p, dev, st);
+        case 32: return sp_launch_f32<32, 4>(p, dev, st);
+        default: return sp_launch_f32<64, 4>(p, dev, st);
       }
     case HC_BF16: return sp_launch_tc<__nv_bfloat16>(p, dtype, dev, st);
     case HC_F16: return sp_launch_tc<__half>(p, dtype, dev, st);
