@@ -244,14 +244,20 @@ __device__ __forceinline__ void fd_group_f32(const FDParams& p, WarpState<float>
   }
 }
 
-// The same for FD_TAIL and FD_BLOCKS, tokens first .. valid - 1: four tokens'
-// keys and values are in flight at a time and share one update of the running
-// maximum (their rows are short, so a chain of single tokens is what bounds
-// them: 48 rows of 75 tokens took 24 us one token at a time).
+// fp32, FD_TAIL and FD_BLOCKS: four tokens at a time for four heads at a time,
+// 4 dims a lane.  The 16 sums over the warp are folded: each exchange halves
+// the values a lane holds, so that 16 shuffles in place of 80 leave the score
+// of head (lane >> 3) and token (lane >> 1) & 3 in each lane, which keeps that
+// head's maximum and its own tokens' sum (m, l: one for each four heads) and
+// takes one exponential; the probabilities come back through shared memory.
+// With the next tokens loaded meanwhile the registers leave three CTAs an SM
+// in place of four, which is slower: 32 rows x 64 blocks, 8 heads each, the
+// block-sparse call 71 us, 81 so (114 with a butterfly of all 80 shuffles).
 __device__ __forceinline__ void fd_group_f32x4(const FDParams& p, WarpState<float>& st, const float (&qf)[kGMax][4],
                                                const float* kbase, const float* vbase, int first, int valid,
-                                               float (&mrow)[kGMax], float (&lrow)[kGMax]) {
+                                               float (&m)[kGMax / 4], float (&l)[kGMax / 4], float* s_p) {
   const int lane = threadIdx.x & 31;
+  const int token = (lane >> 1) & 3;
   for (int i = first; i < valid; i += 4) {
     float4 k4[4], v4[4];
 #pragma unroll
@@ -261,43 +267,65 @@ __device__ __forceinline__ void fd_group_f32x4(const FDParams& p, WarpState<floa
       v4[u] = *reinterpret_cast<const float4*>(vbase + t * kD + 4 * lane);
     }
 #pragma unroll
-    for (int g = 0; g < kGMax; ++g) {
-      if (g >= p.G) continue;
-      float s[4];
+    for (int c = 0; c < kGMax / 4; ++c) {
+      if (4 * c >= p.G) continue;
+      float s[16];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        s[u] = qf[g][0] * k4[u].x + qf[g][1] * k4[u].y + qf[g][2] * k4[u].z + qf[g][3] * k4[u].w;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], o);
-      float mx = mrow[g];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        s[u] = i + u < valid ? s[u] * p.scale_log2 : -INFINITY;
-        mx = fmaxf(mx, s[u]);
+      for (int j = 0; j < 16; ++j) {
+        const float(&q)[4] = qf[4 * c + (j >> 2)];
+        const float4& k = k4[j & 3];
+        s[j] = q[0] * k.x + q[1] * k.y + q[2] * k.z + q[3] * k.w;
       }
+#pragma unroll
+      for (int n = 8, o = 16; n > 0; n >>= 1, o >>= 1) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+          const float keep = upper ? s[n + j] : s[j], send = upper ? s[j] : s[n + j];
+          s[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      }
+      float x = s[0] + __shfl_xor_sync(0xffffffffu, s[0], 1);
+      x = i + token < valid ? x * p.scale_log2 : -INFINITY;
+      float mx = fmaxf(m[c], x);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float ref = mx == -INFINITY ? 0.f : mx;
-      const float corr = exp2f(mrow[g] - ref);
-      mrow[g] = mx;
-      lrow[g] *= corr;
+      const float corr = exp2f(m[c] - ref), e = exp2f(x - ref);
+      const bool grown = mx > m[c];
+      m[c] = mx;
+      l[c] = l[c] * corr + e;
+      __syncwarp();  // the last probabilities are read
+      if ((lane & 1) == 0) s_p[lane >> 1] = e;
+      __syncwarp();
+      if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-      for (int d = 0; d < 4; ++d) st.o[g][d] *= corr;
+        for (int g = 0; g < 4; ++g) {
+          const float f = __shfl_sync(0xffffffffu, corr, 8 * g);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float pv = exp2f(s[u] - ref);
-        lrow[g] += pv;
-        st.o[g][0] = fmaf(pv, v4[u].x, st.o[g][0]);
-        st.o[g][1] = fmaf(pv, v4[u].y, st.o[g][1]);
-        st.o[g][2] = fmaf(pv, v4[u].z, st.o[g][2]);
-        st.o[g][3] = fmaf(pv, v4[u].w, st.o[g][3]);
+          for (int d = 0; d < 4; ++d) st.o[4 * c + g][d] *= f;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 w = *reinterpret_cast<const float4*>(s_p + 4 * g);
+        const float pv[4] = {w.x, w.y, w.z, w.w};
+        float(&o)[4] = st.o[4 * c + g];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          o[0] = fmaf(pv[u], v4[u].x, o[0]);
+          o[1] = fmaf(pv[u], v4[u].y, o[1]);
+          o[2] = fmaf(pv[u], v4[u].z, o[2]);
+          o[3] = fmaf(pv[u], v4[u].w, o[3]);
+        }
       }
     }
   }
 }
 
+// (four CTAs an SM: the grid, that of FD_ALL, is then one wave)
 template <typename T, int kMode>
-__global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
+__global__ void __launch_bounds__(kFThreads, kMode == FD_ALL ? 1 : 4) flash_decode_kernel(FDParams p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   int* s_start = reinterpret_cast<int*>(smem_raw);
   __shared__ int s_warp[32];
@@ -339,7 +367,13 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
 
     if constexpr (std::is_same<T, float>::value) {
       float qf[kGMax][4];
-      float mrow[kGMax], lrow[kGMax];
+      float mrow[kGMax], lrow[kGMax];  // FD_ALL
+      float m4[kGMax / 4], l4[kGMax / 4];
+#pragma unroll
+      for (int c = 0; c < kGMax / 4; ++c) {
+        m4[c] = -INFINITY;
+        l4[c] = 0.f;
+      }
 #pragma unroll
       for (int g = 0; g < kGMax; ++g) {
         mrow[g] = -INFINITY;
@@ -366,10 +400,22 @@ __global__ void __launch_bounds__(kFThreads) flash_decode_kernel(FDParams p) {
         const float* kb = reinterpret_cast<const float*>(p.kp) + off;
         const float* vb = reinterpret_cast<const float*>(p.vp) + off;
         if constexpr (kMode == FD_ALL) fd_group_f32(p, st, qf, kb, vb, valid, mrow, lrow);
-        else fd_group_f32x4(p, st, qf, kb, vb, first, valid, mrow, lrow);
+        else fd_group_f32x4(p, st, qf, kb, vb, first, valid, m4, l4, s_p[warp]);
       }
-      if (lane == 0) {
-        for (int g = 0; g < kGMax; ++g) { s_m[warp][g] = mrow[g]; s_l[warp][g] = lrow[g]; }
+      if constexpr (kMode == FD_ALL) {
+        if (lane == 0) {
+          for (int g = 0; g < kGMax; ++g) { s_m[warp][g] = mrow[g]; s_l[warp][g] = lrow[g]; }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < kGMax / 4; ++c) {
+          l4[c] += __shfl_xor_sync(0xffffffffu, l4[c], 4);
+          l4[c] += __shfl_xor_sync(0xffffffffu, l4[c], 2);
+          if ((lane & 7) == 0) {
+            s_m[warp][4 * c + (lane >> 3)] = m4[c];
+            s_l[warp][4 * c + (lane >> 3)] = l4[c];
+          }
+        }
       }
     } else {
       uint32_t qa[8][2];
