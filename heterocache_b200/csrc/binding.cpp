@@ -39,14 +39,17 @@ struct PyErrorIsSet {};  // a Python call failed
 
 using at::Tensor;
 
+[[noreturn]] void not_a_tensor(const char* name) {
+  throw Refusal{PyExc_TypeError, std::string("heterocache_b200: ") + name + " must be a tensor"};
+}
 const Tensor* opt_tensor(PyObject* o, const char* name) {
   if (o == Py_None) return nullptr;
-  if (!THPVariable_Check(o)) throw Refusal{PyExc_TypeError, std::string("heterocache_b200: ") + name + " must be a tensor"};
+  if (!THPVariable_Check(o)) not_a_tensor(name);
   return &THPVariable_Unpack(o);
 }
 const Tensor& tensor(PyObject* o, const char* name) {
   const Tensor* t = opt_tensor(o, name);
-  if (!t) throw Refusal{PyExc_TypeError, std::string("heterocache_b200: ") + name + " must be a tensor"};
+  if (!t) not_a_tensor(name);
   return *t;
 }
 int integer(PyObject* o, const char* name) {
@@ -198,7 +201,8 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor &cos = tensor(a[3], "cos"), &sin = tensor(a[4], "sin");
     const Tensor &kp = tensor(a[5], "k_pool"), &vp = tensor(a[6], "v_pool"), &table = tensor(a[7], "block_table"),
                  &lens = tensor(a[8], "heads_len"), &free_blocks = tensor(a[9], "free_blocks"),
-                 &free_ptr = tensor(a[10], "free_ptr"), &err = tensor(a[11], "err"), &counter = tensor(a[12], "counter");
+                 &free_ptr = tensor(a[10], "free_ptr"), &err = tensor(a[11], "err"),
+                 &counter = tensor(a[12], "counter");
     const Tensor *counts = opt_tensor(a[13], "counts"), *q_out = opt_tensor(a[14], "q_out"),
                  *lens_out = opt_tensor(a[15], "heads_len_out"), *bounds = opt_tensor(a[16], "bounds");
     if (q.dim() != 4 || k.dim() != 4) refuse("q, k, v need [bsz, heads, tokens, D]");
@@ -437,7 +441,8 @@ PyObject* flash_decode_sparse(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-#define HC_ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+#define HC_ENTRY(name) \
+  {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {HC_ENTRY(rope_append),
                           HC_ENTRY(flash_decode_shared),
                           HC_ENTRY(block_bounds),

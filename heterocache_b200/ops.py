@@ -422,8 +422,8 @@ def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, count
     """Decode attention over each row's listed 64-token blocks alone
     (hc_flash_decode_blocks): blocks [rows, n] int32 ascending, the first
     counts[row] of them used."""
-    out = paged().flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, counts, num_kv_heads, out, scale,
-                                      workspace, err)
+    out = paged().flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, counts, num_kv_heads, out,
+                                      scale, workspace, err)
     if out.__class__ is int:
         check("hc_flash_decode_blocks", out)
     LAUNCHES[0] += 2
