@@ -264,7 +264,9 @@ __device__ __forceinline__ void fd_group_f32x4(const FDParams& p, WarpState<floa
     for (int u = 0; u < 4; ++u) {
       const int t = min(i + u, valid - 1);
       k4[u] = *reinterpret_cast<const float4*>(kbase + t * kD + 4 * lane);
-      v4[u] = *reinterpret_cast<const float4*>(vbase + t * kD + 4 * lane);
+      // (a token that is not there adds nothing, whatever the last one's values are)
+      v4[u] = i + u < valid ? *reinterpret_cast<const float4*>(vbase + t * kD + 4 * lane)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int c = 0; c < kGMax / 4; ++c) {

@@ -143,3 +143,24 @@ def test_bounds_of_any_number_of_last_tokens(cuda_device, last):
             page = int(c.table[r, j // 4])
             want = whole[page, j % 4] if j >= max(0, n - last) // 64 else torch.full_like(whole[0, 0], 7.0)
             assert torch.equal(part[page, j % 4], want), (r, j)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("own", [1, 2, 3, 63, 66])
+def test_an_infinite_value_of_the_last_token(cuda_device, dt, own):
+    """Infinity times a probability that is not zero is infinity, in its dim alone; what is behind it adds nothing."""
+    lens = [64 + own] * KV
+    c = Cache(lens, dt, cuda_device)
+    for r in range(KV):
+        c.vp[c.table[r, 0], lens[r] - 1, 0, 5] = float("inf")
+    q = torch.randn(1, H, 1, D, generator=torch.Generator().manual_seed(1)).to(dt).to(cuda_device)
+    shared = torch.full((KV,), 64, dtype=torch.int32, device=cuda_device)
+    bounds = torch.zeros(c.kp.shape[0], 4, 2, D, dtype=dt, device=cuda_device)
+    ops.block_bounds(c.kp, c.table, c.lens, bounds, c.err)
+    ws = ops.Workspace(cuda_device)
+    a = ops.flash_decode_shared(q, c.kp, c.vp, c.table, c.lens, shared, num_kv_heads=KV, workspace=ws, err=c.err)
+    b = ops.flash_decode_sparse(q, c.kp, c.vp, c.table, c.lens, bounds, num_kv_heads=KV, n_select=4, workspace=ws,
+                                err=c.err)[0]
+    for out in (a, b):
+        assert int(c.err) == 0 and (out[..., 5] == float("inf")).all()
+        assert out[..., :5].isfinite().all() and out[..., 6:].isfinite().all()
