@@ -255,7 +255,8 @@ struct RAParams {
   void* bounds;  // block bounds to keep up to date, or null
   unsigned int* done;  // zero before and after a launch
   int B, H, KV, T;
-  int units, run, kv_ctas;  // 64-token blocks a row may touch, a CTA's; key/value CTAs (set at launch)
+  // set at launch: 64-token blocks a row may touch, a CTA's; rows of a CTA (one token a sequence); key/value CTAs
+  int units, run, rows, kv_ctas;
   int32_t* err;
 };
 int rope_append_dispatch(int dtype, RAParams& p, cudaStream_t st);

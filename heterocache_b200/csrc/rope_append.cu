@@ -9,7 +9,10 @@
 // through the page table.  Pages a row reaches that are not mapped (-1) are
 // taken from the free list in (row, page) order, as the one-token append
 // (kv_copy.cu) takes them.  With `bounds`, the least and greatest key of each
-// 64-token block, per channel, follow: [page][4 blocks][min, max][128].
+// 64-token block, per channel, follow: [page][4 blocks][min, max][128].  In the
+// block that held tokens before, they are taken over those tokens' keys in the
+// page as well, not from its old bounds: these may hold tokens that were
+// appended as drafts and dropped since.
 //
 // Bandwidth bound (each element is read once and written once); one launch.
 // Work is split into units of one aligned 64-token block of one row (so a
@@ -31,6 +34,7 @@ constexpr int kRaThreads = 256;
 constexpr int kRaWarps = kRaThreads / 32;
 constexpr int kRaHeads = 4;  // query heads of one query unit
 constexpr int kRaRun = 4;    // most blocks of a key/value CTA
+constexpr int kRaCtas = 3;   // CTAs an SM
 
 template <typename T> struct RaRow {
   static constexpr int E = 16 / (int)sizeof(T);     // elements of a 16-byte chunk
@@ -322,7 +326,8 @@ __device__ __forceinline__ void ra_query_unit(const RAParams& p, int unit) {
 
 // One aligned 64-token block of one row: threads c < CH2 of a token take
 // chunk c of both halves of the key, the other CH2 those of the value; two
-// tokens a thread are in flight.
+// tokens a thread are in flight.  With bounds the key threads start at the
+// block's first token, whose key is in the page if the row held it before.
 template <typename T, typename TT>
 __device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int cnt, int blk, int phys,
                                          uint32_t* s_mm) {
@@ -343,23 +348,28 @@ __device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int 
     mn[i] = Word<T>::kInf;
     mx[i] = Word<T>::kNegInf;
   }
-  for (int pos0 = beg + (int)threadIdx.x / PER; pos0 < end; pos0 += 2 * TOK) {
+  const int from = p.bounds ? blk * HC_SPARSE_BLOCK : beg;
+  for (int pos0 = from + (int)threadIdx.x / PER; pos0 < end; pos0 += 2 * TOK) {
     uint4 w1[2], w2[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (pos0 + u * TOK < end) {
-        const T* x = src + (pos0 + u * TOK - len) * sst;
-        w1[u] = ldg128(x);
-        w2[u] = ldg128(x + kD / 2);
-      }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int pos = pos0 + u * TOK;
-      if (pos >= end) continue;
+      if (pos < end && (pos >= len || key)) {
+        const T* x = pos >= len ? src + (pos - len) * sst : pool + (int64_t)(pos & (kPage - 1)) * kD;
+        w1[u] = *reinterpret_cast<const uint4*>(x);
+        w2[u] = *reinterpret_cast<const uint4*>(x + kD / 2);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int pos = pos0 + u * TOK;
+      if (pos >= end || (pos < len && !key)) continue;
       if (key) {
-        Trig<TT, E> g;
-        load_rotation<TT, E>(p, b, pos - len, d0, g);
-        rotate<T, TT, E>(g, w1[u], w2[u]);
+        if (pos >= len) {
+          Trig<TT, E> g;
+          load_rotation<TT, E>(p, b, pos - len, d0, g);
+          rotate<T, TT, E>(g, w1[u], w2[u]);
+        }
         if (p.bounds) {  // of the rounded keys: what the pages hold
           const uint32_t x[8] = {w1[u].x, w1[u].y, w1[u].z, w1[u].w, w2[u].x, w2[u].y, w2[u].z, w2[u].w};
 #pragma unroll
@@ -369,6 +379,7 @@ __device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int 
           }
         }
       }
+      if (pos < len) continue;
       T* dst = pool + (int64_t)(pos & (kPage - 1)) * kD;
       *reinterpret_cast<uint4*>(dst) = w1[u];
       *reinterpret_cast<uint4*>(dst + kD / 2) = w2[u];
@@ -406,25 +417,85 @@ __device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int 
     const uint32_t y = s_mm[(w * 2 + which) * RW + d];
     x = which ? Word<T>::max(x, y) : Word<T>::min(x, y);
   }
-  if (blk * HC_SPARSE_BLOCK < len) {  // the block held tokens before
-    const uint32_t y = *out;
-    x = which ? Word<T>::max(x, y) : Word<T>::min(x, y);
-  }
   *out = x;
-}
-
-template <typename T>
-__host__ __device__ constexpr int ra_rows() {
-  return kRaThreads / (2 * RaRow<T>::CH2);
 }
 
 // One token a sequence: a row's token takes as many threads as a token of
 // ra_block, and a CTA a run of rows from r0 on (16 of a 16-bit cache), so
 // that few CTAs go through all rows for the allocation.  What is appended does
-// not hang on the allocation: it is loaded first.
+// not hang on the allocation: it is loaded first.  With bounds a CTA has a
+// quarter of the rows where all CTAs are resident at once all the same: its
+// warps then read a row's earlier keys four at a time.  (Of 64 sequences of 8
+// rows, 2000 tokens or fewer each: 6.9 us without bounds, 8.8 with; of 512
+// sequences 27 and 32, and 53 with a quarter of the rows there too.)
+template <typename T>
+__host__ __device__ constexpr int ra_rows() {
+  return kRaThreads / (2 * RaRow<T>::CH2);
+}
+// Warps of a row's earlier keys: those of a CTA of `rows` rows, one if it has more rows than warps.
+__host__ __device__ constexpr int ra_row_warps(int rows) { return rows < kRaWarps ? kRaWarps / rows : 1; }
+
+// Least and greatest key, per channel, of the tokens before the new one in its
+// block, of the CTA's `rows` rows: row r0 + i's partials at s_mm[i * WPR ..][least,
+// greatest].  What ra_plan will find bad is not read.
+template <typename T, int WPR>
+__device__ __forceinline__ void ra_past(const RAParams& p, int r0, uint32_t* s_mm) {
+  constexpr int RW = kD * (int)sizeof(T) / 4, CH = RW / 4, TW = 32 / CH;  // a row's words, chunks; tokens of a warp
+  constexpr int STEP = WPR * TW, U = 8;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll 1
+  for (int slot = warp; slot < p.rows * WPR; slot += kRaWarps) {
+    const int r = r0 + slot / WPR;
+    int n = 0;
+    const uint4* x = nullptr;
+    if (r < p.B * p.KV && ra_count(p, r / p.KV) > 0) {
+      const int len = p.heads_len[r];
+      if (len > 0 && (len >> 8) < p.max_blocks) n = len & (HC_SPARSE_BLOCK - 1);
+      if (n > 0) {
+        const int phys = p.bt[(int64_t)r * p.max_blocks + (len >> 8)];
+        if (phys < 0 || phys >= p.n_blocks) n = 0;
+        else x = reinterpret_cast<const uint4*>(p.kp) + ((int64_t)phys * kPage + (len & (kPage - 1)) - n) * CH + lane % CH;
+      }
+    }
+    uint32_t mn[4], mx[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      mn[i] = Word<T>::kInf;
+      mx[i] = Word<T>::kNegInf;
+    }
+    for (int t0 = (slot % WPR) * TW + lane / CH; t0 < n; t0 += U * STEP) {
+      uint4 w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (t0 + u * STEP < n) w[u] = x[(t0 + u * STEP) * CH];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (t0 + u * STEP < n) {
+          const uint32_t y[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            mn[i] = Word<T>::min(mn[i], y[i]);
+            mx[i] = Word<T>::max(mx[i], y[i]);
+          }
+        }
+    }
+#pragma unroll
+    for (int o = CH; o < 32; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mn[i] = Word<T>::min(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
+        mx[i] = Word<T>::max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+      }
+    if (lane < CH) {
+      uint4* out = reinterpret_cast<uint4*>(s_mm) + slot * 2 * CH + lane;
+      out[0] = make_uint4(mn[0], mn[1], mn[2], mn[3]);
+      out[CH] = make_uint4(mx[0], mx[1], mx[2], mx[3]);
+    }
+  }
+}
+
 template <typename T, typename TT> struct RaToken {
   static constexpr int E = RaRow<T>::E, CH2 = RaRow<T>::CH2, PER = 2 * CH2;
-  static constexpr int RW = kD * (int)sizeof(T) / 4;
   int r, b, c, pos, phys;
   bool ok, key;
   uint4 w1, w2;
@@ -434,7 +505,7 @@ template <typename T, typename TT> struct RaToken {
     r = r0 + (int)threadIdx.x / PER;
     c = threadIdx.x % PER;
     key = c < CH2;
-    ok = r < p.B * p.KV;
+    ok = r < p.B * p.KV && r - r0 < p.rows;
     if (!ok) return;
     b = r / p.KV;
     const int h = r % p.KV;
@@ -456,7 +527,7 @@ template <typename T, typename TT> struct RaToken {
     for (int k = r0; k < r; ++k) take += ra_need(p, k, bad);
     phys = p.free_blocks[take];
   }
-  __device__ __forceinline__ void store(const RAParams& p) {
+  __device__ __forceinline__ void store(const RAParams& p, int r0, const uint32_t* s_mm) {
     if (!ok) return;
     const int d0 = (key ? c : c - CH2) * E;
     if (key) rotate<T, TT, E>(g, w1, w2);
@@ -464,29 +535,31 @@ template <typename T, typename TT> struct RaToken {
     *reinterpret_cast<uint4*>(dst) = w1;
     *reinterpret_cast<uint4*>(dst + kD / 2) = w2;
     if (!key || !p.bounds) return;
-    uint32_t* lim = reinterpret_cast<uint32_t*>(p.bounds) +
-                    ((int64_t)phys * (kPage / HC_SPARSE_BLOCK) + ((pos & (kPage - 1)) / HC_SPARSE_BLOCK)) * 2 * RW +
-                    c * 4;
-    merge(lim, w1);
-    merge(lim + RW / 2, w2);
+    uint4* lim = reinterpret_cast<uint4*>(p.bounds) +
+                 ((int64_t)phys * (kPage / HC_SPARSE_BLOCK) + ((pos & (kPage - 1)) / HC_SPARSE_BLOCK)) * 4 * CH2 + c;
+    const int n = ra_row_warps(p.rows);
+    const uint4* past = reinterpret_cast<const uint4*>(s_mm) + (r - r0) * n * 4 * CH2 + c;
+    merge(lim, past, n, w1);
+    merge(lim + CH2, past + CH2, n, w2);
   }
-  __device__ __forceinline__ void merge(uint32_t* at, const uint4& w) {
+  // The bounds of a chunk: of the new key and the partials of ra_past.
+  __device__ __forceinline__ void merge(uint4* at, const uint4* past, int n, const uint4& w) {
     uint4 lo = w, hi = w;
-    if ((pos & (HC_SPARSE_BLOCK - 1)) != 0) {  // the block held tokens before
-      const uint4 a = *reinterpret_cast<const uint4*>(at), z = *reinterpret_cast<const uint4*>(at + RW);
-      lo = make_uint4(Word<T>::min(a.x, w.x), Word<T>::min(a.y, w.y), Word<T>::min(a.z, w.z), Word<T>::min(a.w, w.w));
-      hi = make_uint4(Word<T>::max(z.x, w.x), Word<T>::max(z.y, w.y), Word<T>::max(z.z, w.z), Word<T>::max(z.w, w.w));
+    for (int i = 0; i < n; ++i) {
+      const uint4 a = past[i * 4 * CH2], z = past[i * 4 * CH2 + 2 * CH2];
+      lo = make_uint4(Word<T>::min(a.x, lo.x), Word<T>::min(a.y, lo.y), Word<T>::min(a.z, lo.z), Word<T>::min(a.w, lo.w));
+      hi = make_uint4(Word<T>::max(z.x, hi.x), Word<T>::max(z.y, hi.y), Word<T>::max(z.z, hi.z), Word<T>::max(z.w, hi.w));
     }
-    *reinterpret_cast<uint4*>(at) = lo;
-    *reinterpret_cast<uint4*>(at + RW) = hi;
+    at[0] = lo;
+    at[2 * CH2] = hi;
   }
 };
 
 template <typename T, typename TT>
-__global__ void __launch_bounds__(kRaThreads, 3) rope_append_kernel(const RAParams p) {
+__global__ void __launch_bounds__(kRaThreads, kRaCtas) rope_append_kernel(const RAParams p) {
   __shared__ int2 s_red[kRaWarps];
   __shared__ int s_warp[32];
-  __shared__ uint32_t s_mm[kRaWarps * 2 * kD * sizeof(T) / 4];
+  __shared__ __align__(16) uint32_t s_mm[(ra_rows<T>() > kRaWarps ? ra_rows<T>() : kRaWarps) * 2 * kD * sizeof(T) / 4];
   __shared__ int s_phys[kRaRun], s_last;
   pdl_wait();
   pdl_trigger();
@@ -496,9 +569,13 @@ __global__ void __launch_bounds__(kRaThreads, 3) rope_append_kernel(const RAPara
   }
   const int per_row = (p.units + p.run - 1) / p.run;
   const bool single = p.T == 1;
-  const int r = single ? (int)blockIdx.x * ra_rows<T>() : (int)blockIdx.x / per_row;
+  const int r = single ? (int)blockIdx.x * p.rows : (int)blockIdx.x / per_row;
   const int u0 = (blockIdx.x % per_row) * p.run;
   RaToken<T, TT> tok;
+  if (single && p.bounds) {
+    if (p.rows == ra_rows<T>()) ra_past<T, ra_row_warps(ra_rows<T>())>(p, r, s_mm);
+    else ra_past<T, ra_row_warps(ra_rows<T>() / 4)>(p, r, s_mm);
+  }
   if (single) tok.load(p, r);
   const int base = *p.free_ptr;
   int before, total;
@@ -514,7 +591,7 @@ __global__ void __launch_bounds__(kRaThreads, 3) rope_append_kernel(const RAPara
   }
   ra_arrive(p, &s_last);
   if (!status && single) {
-    tok.store(p);
+    tok.store(p, r, s_mm);
   } else if (!status) {
     for (int u = u0; u < min(u0 + p.run, p.units); ++u) {
       const int blk = len / HC_SPARSE_BLOCK + u;
@@ -533,7 +610,9 @@ static int ra_launch(RAParams& p, cudaStream_t st) {
   // a CTA finds the allocation once for a run of 4 blocks, where there are
   // still CTAs enough to fill the GPU
   p.run = R * p.units >= kRaRun * 8 * (int64_t)device_sms(current_device()) ? kRaRun : 1;
-  const int64_t kv = p.T == 1 ? (R + ra_rows<T>() - 1) / ra_rows<T>() : R * ((p.units + p.run - 1) / p.run);
+  p.rows = ra_rows<T>();
+  if (p.bounds && (R + p.rows / 4 - 1) / (p.rows / 4) <= kRaCtas * (int64_t)device_sms(current_device())) p.rows /= 4;
+  const int64_t kv = p.T == 1 ? (R + p.rows - 1) / p.rows : R * ((p.units + p.run - 1) / p.run);
   const int64_t q = (((int64_t)p.B * p.T + TOK - 1) / TOK) * ((p.H + kRaHeads - 1) / kRaHeads);
   if (kv + q > 0x7fffffffLL) return HC_ERR_UNSUPPORTED;
   p.kv_ctas = (int)kv;

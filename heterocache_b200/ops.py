@@ -363,7 +363,10 @@ def rope_append(q, k, v, cos, sin, k_pool, v_pool, block_table, heads_len, free_
     int32 says how many of the T tokens each sequence has (a padded batch);
     the rest is left as it was.  The new lengths go to ``heads_len_out``
     (default: heads_len).  ``bounds`` [n_blocks, 4, 2, D]: block bounds of
-    ``flash_decode_sparse`` to keep up to date.  A bad length, count or page,
+    ``flash_decode_sparse`` to keep up to date: those of the blocks appended to
+    are then of the tokens the row holds, drafts that were dropped since left
+    out.  (Where tokens are dropped and none appended, ``block_bounds`` with
+    ``last=1`` does it.)  A bad length, count or page,
     or a free list that is too short, is reported in ``err`` and leaves the
     cache as it was.  ``workspace`` holds a counter; calls that may overlap
     need a workspace each."""

@@ -259,6 +259,10 @@ int hc_flash_decode_with_new(int dtype, int bsz, int num_kv_heads, int groups, i
  * heads_len[r] + count: heads_len itself, or another array (drafted tokens
  * that may be dropped: the pages stay mapped to the row).
  *   bounds: block bounds to keep up to date (see hc_block_bounds), or NULL.
+ *   Those of the blocks appended to are taken over the keys that the row holds:
+ *   tokens appended before and dropped since (heads_len not moved) are left
+ *   out.  Where tokens are dropped and none appended, the last block's bounds
+ *   still hold them: hc_block_bounds with last = 1.
  *   counter: one int32 of device memory, zero before the first call; a call
  *   leaves it zero.  Calls that may overlap need one each, and a call that
  *   was cut off leaves it to be zeroed by the caller.
