@@ -324,6 +324,7 @@ PyObject* block_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (list) ints(*list, "rows");
     const int dt = dtype_code(dtype);
     same_device(kp, {&table, &lens, &bounds, &err, list});
+    if (list && list->numel() == 0) return same(a[3]);  // no rows (a null pointer would be all of them)
     c10::cuda::CUDAGuard guard(kp.device());
     const int rc = hc_block_bounds(dt, narrow(R, "rows"), (int)kD, ptr(kp), n_pages, iptr(table), width, iptr(lens),
                                    iptr(list), list ? narrow(list->numel(), "rows") : 0, last, ptr(bounds), iptr(err),

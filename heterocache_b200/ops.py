@@ -402,7 +402,8 @@ def block_bounds(k_pool, block_table, heads_len, bounds, err, *, rows=None, last
     out = paged().block_bounds(k_pool, block_table, heads_len, bounds, err, rows, last)
     if out.__class__ is int:
         check("hc_block_bounds", out)
-    LAUNCHES[0] += 1
+    if rows is None or rows.numel():
+        LAUNCHES[0] += 1
     return out
 
 
