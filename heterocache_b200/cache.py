@@ -390,6 +390,7 @@ class HeteroCache(_CacheBase):
                 for b in range(self.bsz):
                     for h in keep:
                         self._hlen[layer_idx][b * self.num_kv_heads + h] = seq_len
+            self._refresh_bounds(layer_idx)
             if not upd:
                 self.key_cache_cpu.append(None)
                 self.value_cache_cpu.append(None)
@@ -488,7 +489,8 @@ class HeteroCache(_CacheBase):
 
     def _ensure_bounds(self, layer_idx) -> None:
         """The layer's block bounds, from its pages (once, before its first
-        sparse decode step; appends and retrievals keep them up to date)."""
+        sparse decode step; appends, retrievals and another prompt's prefill
+        keep them up to date, in place, since graphs hold their address)."""
         if self._bounds[layer_idx] is None:
             kp = self.key_pools[layer_idx]
             self._bounds[layer_idx] = torch.zeros(kp.shape[0], PAGE // ops.BLOCK, 2, self.head_dim, dtype=kp.dtype,
@@ -600,6 +602,7 @@ class HeteroCache(_CacheBase):
         kl = keep_lens.numpy().astype(np.int64)
         for b in range(bsz):
             self._hlen[layer_idx][b * self.num_kv_heads:b * self.num_kv_heads + nc] = kl
+        self._refresh_bounds(layer_idx)
         if keep_idx:
             self._kept[layer_idx] = (idx, kl.copy())
 
