@@ -144,6 +144,39 @@ class _LayerJobs:
         self.median = None
 
 
+def _append_room(cache, layer_idx: int):
+    """The check of ``HeteroCache._append_bookkeeping``: the rows that the append maps
+    a page for (a mask), or None where the slack says that there is none."""
+    if cache._slack[layer_idx] > 0:
+        return None
+    hl = cache._hlen[layer_idx]
+    width = cache.block_tables[layer_idx].shape[1]
+    logical = hl // PAGE
+    if np.any(logical >= width):
+        raise IndexError(f"Layer {layer_idx}: block table has no column for the next decode token")
+    grow = logical >= cache._mapped[layer_idx]
+    need = int(np.count_nonzero(grow))
+    if need > 0 and cache.free_block_pointers[layer_idx] + need > cache.free_blocks[layer_idx].size(0):
+        raise RuntimeError(f"Layer {layer_idx} OOM.")
+    return grow
+
+
+def _append_advance(cache, layer_idx: int, grow) -> None:
+    """The mirrors after an append, given what ``_append_room`` said of it."""
+    hl = cache._hlen[layer_idx]
+    hl += 1
+    if grow is None:
+        cache._slack[layer_idx] -= 1
+        return
+    need = int(np.count_nonzero(grow))
+    if need > 0:
+        cache.free_block_pointers[layer_idx] += need
+        cache._mapped[layer_idx] += grow
+    width = cache.block_tables[layer_idx].shape[1]
+    room = np.minimum(cache._mapped[layer_idx], width) * PAGE - hl
+    cache._slack[layer_idx] = max(int(room.min()), 0) if room.size else 0
+
+
 class HeteroCache(_CacheBase):
     def __init__(self, cache_config):
         if _CacheBase is not object:
@@ -467,11 +500,14 @@ class HeteroCache(_CacheBase):
             raise ValueError("update_rope: one token per sequence (prefill goes through update)")
         if self.key_pools[layer_idx] is None:
             raise RuntimeError("update_rope: the layer has no pages yet (prefill first)")
+        kp = self.key_pools[layer_idx]
+        if (tuple(query_states.shape) != (self.bsz, self.num_attn_heads, 1, self.head_dim)
+                or query_states.dtype != kp.dtype or query_states.device != kp.device):
+            raise ValueError(f"update_rope: the query must be [{self.bsz}, {self.num_attn_heads}, 1, {self.head_dim}] "
+                             f"of {kp.dtype} on {kp.device}, as the pages are")
         if self._deferred and layer_idx in self._deferred:
             self.flush_checks()
-        self._append_bookkeeping(layer_idx)
-        if layer_idx == 0:
-            self._seen_tokens += 1
+        grow = _append_room(self, layer_idx)
         self._wait_retrieval(layer_idx)
         self._wait_append(layer_idx)
         q_out = None
@@ -484,6 +520,10 @@ class HeteroCache(_CacheBase):
                                 self.value_pools[layer_idx], self.block_tables[layer_idx], self.heads_len[layer_idx],
                                 self.free_blocks[layer_idx], self._free_ptr[layer_idx], self._err,
                                 workspace=self._ws_fd, q_out=q_out, bounds=self._bounds[layer_idx])
+        # (a refused call leaves the mirrors where they were)
+        _append_advance(self, layer_idx, grow)
+        if layer_idx == 0:
+            self._seen_tokens += 1
         self._q_staged[layer_idx] = self.bsz == 1
         return q_out
 
@@ -516,27 +556,7 @@ class HeteroCache(_CacheBase):
         the checks, which would find nothing (a few numpy calls per layer and
         step on the host, which sets the pace of a captured decode step over
         many small caches)."""
-        hl = self._hlen[layer_idx]
-        s = self._slack[layer_idx]
-        if s > 0:
-            self._slack[layer_idx] = s - 1
-            hl += 1
-            return
-        width = self.block_tables[layer_idx].shape[1]
-        logical = hl // PAGE
-        if np.any(logical >= width):
-            raise IndexError(f"Layer {layer_idx}: block table has no column for the next decode token")
-        grow = logical >= self._mapped[layer_idx]
-        need = int(np.count_nonzero(grow))
-        if need > 0:
-            ptr = self.free_block_pointers[layer_idx]
-            if ptr + need > self.free_blocks[layer_idx].size(0):
-                raise RuntimeError(f"Layer {layer_idx} OOM.")
-            self.free_block_pointers[layer_idx] += need
-            self._mapped[layer_idx] += grow
-        hl += 1
-        room = np.minimum(self._mapped[layer_idx], width) * PAGE - hl
-        self._slack[layer_idx] = max(int(room.min()), 0) if room.size else 0
+        _append_advance(self, layer_idx, _append_room(self, layer_idx))
 
     def init_coefficient(self, query_states, key_states, layer_idx):
         """Pivot reference sets (heterocache/cache_utils.py:1149-1190)."""
