@@ -60,21 +60,29 @@ def _i32(t: torch.Tensor, name: str) -> None:
 
 
 class Workspace:
-    """Grow-only, zero-initialised scratch buffer owned by the caller."""
+    """Grow-only, zero-initialised scratch buffer owned by the caller.  A buffer
+    that became too small stays allocated as long as the workspace: captured
+    graphs, and kernels on a stream other than the one it was made on, may
+    still use it.  (Each is at least half as large again as the one before.)"""
 
     def __init__(self, device):
         self.device = torch.device(device)
         self.buf = torch.zeros(0, dtype=torch.uint8, device=self.device)
+        self._outgrown = []
         # rope_append's counter: apart from buf, where other calls leave their scratch
         self.counter = torch.zeros(4, dtype=torch.int32, device=self.device)
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf.numel() < nbytes:
-            self.buf = torch.zeros(int(nbytes) + (1 << 20), dtype=torch.uint8, device=self.device)
+            if self.buf.numel():
+                self._outgrown.append(self.buf)
+            self.buf = torch.zeros(max(int(nbytes) + (1 << 20), self.buf.numel() * 3 // 2), dtype=torch.uint8,
+                                   device=self.device)
         return self.buf
 
     def reset(self) -> None:
-        self.buf.zero_()
+        for buf in (*self._outgrown, self.buf):
+            buf.zero_()
         self.counter.zero_()
 
 
