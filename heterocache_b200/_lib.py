@@ -156,6 +156,10 @@ def paged():
     global _PAGED
     if _PAGED is None:
         lib()
+        from .build import binding_built_for_another
+        if binding_built_for_another():
+            raise RuntimeError("heterocache_b200: the binding _paged.so was built for another torch or Python; run "
+                               "`python -c 'import heterocache_b200.build as b; b.build()'` first")
         try:
             from . import _paged
         except ImportError as e:

@@ -25,6 +25,7 @@ INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(PKG, "libhcb200.so")
 BINDING = os.path.join(CSRC, "binding.cpp")
 BINDING_OUT = os.path.join(PKG, "_paged.so")
+BINDING_NOTE = os.path.join(PKG, "_paged.built")  # what _paged.so was built for
 OBJ_DIR = os.path.join(PKG, "_build")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -53,12 +54,27 @@ def _run(cmd, verbose):
     return res
 
 
-def _binding_stale() -> bool:
-    if not os.path.exists(BINDING_OUT):
-        return True
+def _binding_for() -> str:
+    """What a binding belongs to: the torch and the Python it is built with."""
     import torch
+    return (f"torch {torch.__version__} {torch.version.git_version} cxx11_abi {int(torch.compiled_with_cxx11_abi())} "
+            f"{sys.implementation.cache_tag}\n")
+
+
+def binding_built_for_another() -> bool:
+    """Whether the note beside the binding names another torch or Python."""
+    try:
+        with open(BINDING_NOTE) as f:
+            return f.read() != _binding_for()
+    except OSError:
+        return False  # no note
+
+
+def _binding_stale() -> bool:
+    if not os.path.exists(BINDING_OUT) or not os.path.exists(BINDING_NOTE) or binding_built_for_another():
+        return True
     t = os.path.getmtime(BINDING_OUT)
-    deps = [BINDING, os.path.join(INCLUDE, "heterocache_b200.h"), os.path.abspath(__file__), torch.version.__file__]
+    deps = [BINDING, os.path.join(INCLUDE, "heterocache_b200.h"), os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > t for d in deps)
 
 
@@ -73,7 +89,11 @@ def _build_binding(verbose: bool) -> None:
           "-I" + sysconfig.get_paths()["include"], *(x for d in system for x in ("-isystem", d)), BINDING,
           "-o", BINDING_OUT + ".tmp", "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
           "-ltorch_python", "-L" + PKG, "-l:" + os.path.basename(OUT), "-Wl,-rpath,$ORIGIN"], verbose)
+    if os.path.exists(BINDING_NOTE):
+        os.remove(BINDING_NOTE)  # (a build that is cut off here leaves a stale binding, not a wrong note)
     os.replace(BINDING_OUT + ".tmp", BINDING_OUT)
+    with open(BINDING_NOTE, "w") as f:
+        f.write(_binding_for())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
