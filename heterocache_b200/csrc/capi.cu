@@ -388,6 +388,11 @@ int with_new_params(hc::FDParams& p, int dtype, int bsz, int num_kv_heads, int g
   p.q_stage = q_stage;
   return HC_OK;
 }
+
+// What every attention needs (pools may be missing where there are no pages).
+bool has_buffers(const hc::FDParams& p) {
+  return p.q && p.out && p.bt && p.heads_len && (p.n_blocks <= 0 || (p.kp && p.vp));
+}
 }  // namespace
 
 extern "C" {
@@ -832,6 +837,9 @@ int hc_rope_append(int dtype, int trig_dtype, int bsz, int num_heads, int num_kv
     return HC_ERR_INVALID;
   if (!heads_len || !heads_len_out || !block_table || !free_ptr || !counter || (n_free > 0 && !free_blocks))
     return HC_ERR_INVALID;
+  // (a call of no tokens, and one into no pages, may come without the buffers)
+  if (n_tokens > 0 && (!k || !v || !cos || !sin || (num_heads > 0 && (!q || !q_out)))) return HC_ERR_INVALID;
+  if (n_pool_blocks > 0 && (!k_pool || !v_pool)) return HC_ERR_INVALID;
   if ((int64_t)max_blocks * HC_PAGE_SIZE > 0x7fffffffLL || (int64_t)bsz * num_kv_heads > 0x7fffffffLL)
     return HC_ERR_UNSUPPORTED;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(cos) || !aligned16(sin) || !aligned16(q_out) ||
@@ -901,6 +909,7 @@ int hc_block_bounds(int dtype, int rows_total, int head_dim, const void* k_pool,
   if (head_dim != HC_HEAD_DIM || rows_total <= 0 || max_blocks <= 0 || n_pool_blocks < 0 || last < 0 || n_rows < 0)
     return HC_ERR_INVALID;
   if (!aligned16(k_pool) || !aligned16(bounds) || !block_table || !heads_len) return HC_ERR_INVALID;
+  if (n_pool_blocks > 0 && (!k_pool || !bounds)) return HC_ERR_INVALID;
   if ((int64_t)max_blocks * HC_PAGE_SIZE > 0x7fffffffLL) return HC_ERR_UNSUPPORTED;
   if (rows && n_rows == 0) return HC_OK;
   hc::BBParams p;
@@ -933,7 +942,9 @@ int hc_block_select(int dtype, int bsz, int num_kv_heads, int groups, int head_d
     return HC_ERR_INVALID;
   if (n_select < 1 || sink < 0 || recent < 0 || (int64_t)sink + recent > n_select) return HC_ERR_INVALID;
   if (!aligned16(q) || !aligned16(bounds) || !block_table || !heads_len || !blocks || !counts) return HC_ERR_INVALID;
+  if (!q || (n_pool_blocks > 0 && !bounds)) return HC_ERR_INVALID;
   if (!stride_ok(dtype, qsb) || !stride_ok(dtype, qsh)) return HC_ERR_INVALID;
+  if (!aligned16(workspace)) return HC_ERR_WORKSPACE;
   hc::BSParams p;
   std::memset(&p, 0, sizeof(p));
   p.q = q;
@@ -966,7 +977,8 @@ int hc_flash_decode_blocks(int dtype, int bsz, int num_kv_heads, int groups, int
                                  n_pool_blocks, block_table, max_blocks, heads_len, nullptr, nullptr, 0, 0, 0, 0,
                                  scale, out, nullptr, err_flag, false);
   if (rc != HC_OK) return rc;
-  if (!blocks || !counts || n_select < 1) return HC_ERR_INVALID;
+  if (!blocks || !counts || n_select < 1 || !has_buffers(p)) return HC_ERR_INVALID;
+  if (!aligned16(workspace)) return HC_ERR_WORKSPACE;
   if ((int64_t)max_blocks * HC_PAGE_SIZE > 0x7fffffffLL ||
       (int64_t)bsz * num_kv_heads * n_select * HC_SPARSE_BLOCK > 0x7fffffffLL)
     return HC_ERR_UNSUPPORTED;
@@ -994,6 +1006,7 @@ int hc_flash_decode_sparse(int dtype, int bsz, int num_kv_heads, int groups, int
   if (!valid_dtype(dtype)) return HC_ERR_DTYPE;
   if (bsz <= 0 || num_kv_heads <= 0 || max_blocks <= 0 || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out))
     return HC_ERR_INVALID;
+  if (!out || (n_pool_blocks > 0 && (!k_pool || !v_pool))) return HC_ERR_INVALID;
   if ((int64_t)bsz * num_kv_heads * n_select * HC_SPARSE_BLOCK > 0x7fffffffLL) return HC_ERR_UNSUPPORTED;
   if (workspace_bytes < hc_flash_decode_sparse_workspace_size(bsz, num_kv_heads, groups, head_dim, max_blocks))
     return HC_ERR_WORKSPACE;
@@ -1025,7 +1038,7 @@ int hc_flash_decode_shared(int dtype, int bsz, int num_kv_heads, int groups, int
                                  n_pool_blocks, block_table, max_blocks, heads_len, k_new, v_new, kn_sb, kn_sh,
                                  vn_sb, vn_sh, scale, out, nullptr, err_flag, false);
   if (rc != HC_OK) return rc;
-  if (!shared_len) return HC_ERR_INVALID;
+  if (!shared_len || !has_buffers(p)) return HC_ERR_INVALID;
   if (groups > hc::kGMax || (int64_t)bsz * num_kv_heads > hc::kMaxRowsFD ||
       (int64_t)max_blocks * HC_PAGE_SIZE > 0x7fffffffLL)
     return HC_ERR_UNSUPPORTED;
