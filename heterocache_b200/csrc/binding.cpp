@@ -19,6 +19,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <climits>
 #include <initializer_list>
 #include <string>
@@ -80,6 +81,19 @@ const Tensor& rows(const Tensor& t, const char* name) {
   if (n == 0 || t.size(n - 1) != kD || t.stride(n - 1) != 1)
     refuse(std::string(name) + " must have a contiguous last dim of 128");
   return t;
+}
+// A tensor of 128-element rows that is written to: no two rows may share
+// memory.  (By increasing stride, each dimension steps over all of those before.)
+void apart(const Tensor& t, const char* name) {
+  int64_t dims[3], n = 0, span = kD;
+  for (int64_t d = 0; d < t.dim() - 1; ++d)
+    if (t.size(d) > 1) dims[n++] = d;
+  std::sort(dims, dims + n, [&](int64_t a, int64_t b) { return t.stride(a) < t.stride(b); });
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t s = t.stride(dims[i]);
+    if (s < span) refuse(std::string(name) + " must not overlap itself");
+    span += s * (t.size(dims[i]) - 1);
+  }
 }
 // A contiguous int32 tensor of at least n entries.
 void ints(const Tensor& t, const char* name, int64_t n, const char* what) {
@@ -225,6 +239,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (counts) ints(*counts, "counts", bsz, "counts needs an entry per sequence");
     if (q_out && (rows(*q_out, "q_out").sizes() != q.sizes() || q_out->scalar_type() != dtype))
       refuse("q_out must have the queries' shape and dtype");
+    if (q_out && q_out->numel()) apart(*q_out, "q_out");
     if (lens_out) ints(*lens_out, "heads_len_out", R, "heads_len_out needs a row per (batch row, KV head)");
     if (bounds) check_bounds(*bounds, n_pages, dtype);
     same_device(q, {&k, &v, &cos, &sin, &kp, &vp, &table, &lens, lens_out, &free_blocks, &free_ptr, &err, counts, q_out,
