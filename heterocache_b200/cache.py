@@ -77,8 +77,9 @@ class HeteroCacheConfig:
                  num_layers: Optional[int] = 32, window_size: int = 1,
                  total_kv_heads: Optional[int] = None, fused_rope: bool = False, sparse_blocks: int = 0,
                  sparse_sink: int = 1, sparse_recent: int = 2):
-        if sparse_blocks and not 0 <= sparse_sink + sparse_recent <= sparse_blocks:
-            raise ValueError("sparse_sink + sparse_recent must not be more than sparse_blocks")
+        if sparse_blocks and (min(sparse_blocks, sparse_sink, sparse_recent) < 0
+                              or sparse_sink + sparse_recent > sparse_blocks):
+            raise ValueError("sparse_sink + sparse_recent must not be more than sparse_blocks, and none of them negative")
         self.fused_rope = fused_rope
         self.sparse_blocks, self.sparse_sink, self.sparse_recent = sparse_blocks, sparse_sink, sparse_recent
         self.data = data
