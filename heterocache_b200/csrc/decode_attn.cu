@@ -45,7 +45,12 @@ template <int kMode>
 __device__ __forceinline__ int fd_row_len(const FDParams& p, int r) {
   if constexpr (kMode == FD_BLOCKS) return min(max(p.counts[r], 0), p.n_select) * HC_SPARSE_BLOCK;
   const int len = p.heads_len[r];
-  if constexpr (kMode == FD_TAIL) return len > fd_tail_lo(p, r) ? len - fd_tail_base(p, r) : 0;
+  if constexpr (kMode == FD_TAIL) {
+    // (no further than the page table: a length that is out of range would
+    // overflow the sums over the rows; the join reports it)
+    const int end = min(len, p.max_blocks * kPage);
+    return end > fd_tail_lo(p, r) ? end - fd_tail_base(p, r) : 0;
+  }
   return len;
 }
 
@@ -1001,6 +1006,7 @@ __global__ void __launch_bounds__(kJThreads) flash_join_kernel(FDParams p, int n
   int before = 0, total = 0, tiles = 0;
   for (int r = threadIdx.x; r < p.R; r += kJThreads) {
     const int len = max(0, fd_row_len<kMode>(p, r));
+    if (kMode == FD_TAIL && blockIdx.x == 0 && p.heads_len[r] > p.max_blocks * kPage) set_err(p.err, HC_ERR_RANGE);
     const int pad = (len + p.gran - 1) / p.gran * p.gran;
     total += pad;
     before += r < r_first ? pad : 0;
