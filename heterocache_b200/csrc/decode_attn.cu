@@ -591,7 +591,12 @@ __device__ __forceinline__ void fd_group_tc(const FDParams& p, TcState& st, cons
     st.ot[mt][2] *= c0;
     st.ot[mt][3] *= c1;
   }
-  // P^T as the B operand: tokens 2tig.. (n-tile 0) and 8+2tig.. (n-tile 1)
+  // P^T as the B operand: tokens 2tig.. (n-tile 0) and 8+2tig.. (n-tile 1).
+  // The product takes 16-bit operands: each probability is rounded once (half a
+  // step, relative), independently of the output's rounding, so that the error
+  // is some sqrt(2) of that of probabilities in 32 bits; a second product of the
+  // remainders would double the values' part of the work.  The sum l is of the
+  // unrounded ones, and sums and outputs are in fp32.
   const uint32_t b0 = pack2<T>(sv[0], sv[1]);
   const uint32_t b1 = pack2<T>(sv[2], sv[3]);
   const int vrow = tok0 + 8 * (mi >> 1) + j;
@@ -650,7 +655,7 @@ __global__ void __launch_bounds__(kTThreads, 2)
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gid = lane >> 2, tig = lane & 3;
-  // programmatic dependent launch: wait for the kernel before (the page
+  // programmatic dependent launch (the rules are at pdl_launch): wait for the kernel before (the page
   // append) to finish, then let the combine get resident; it reads row
   // lengths before its own wait and waits for this grid's partials.
   // FD_TAIL: the kernel before is the prefix part, whose CTAs let this grid
@@ -1283,8 +1288,19 @@ size_t flash_decode_ws_bytes(int R, int G) {
 }
 
 // Launch with programmatic stream serialization: the grid may start while the
-// previous kernel in the stream drains; every kernel launched this way
-// executes griddepcontrol.wait before it reads anything.
+// previous kernel in the stream drains (once all of that kernel's CTAs have
+// triggered or ended).  What a kernel may read before its own wait follows from
+// where the one before triggers:
+// * flash_decode with FD_ALL or FD_BLOCKS waits before it reads anything.
+// * FD_TAIL reads lengths, page tables, queries and pages, and writes its
+//   partials, before its wait.  It may be launched only directly behind the
+//   prefix part (shared_attn.cu), whose CTAs trigger after their own wait, when
+//   all that came before is complete.  Every CTA of it waits before it ends:
+//   the join, which waits for this grid alone, so finds the prefix part's
+//   results as well.
+// * The combine and the join read lengths, counts, shared lengths, q and k_new
+//   before their wait: those come from before the attention kernel, whose CTAs
+//   trigger after their wait (FD_TAIL: start after the prefix part's).
 template <typename... KArgs, typename... Args>
 static cudaError_t pdl_launch(void (*kern)(KArgs...), int grid, int threads, size_t smem, cudaStream_t st,
                               Args&&... args) {

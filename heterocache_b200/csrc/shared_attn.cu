@@ -88,6 +88,8 @@ __global__ void __launch_bounds__(8 * RT / RPT, 2) shared_prefix_kernel(const SP
   float* sk = sq + RT * kSpPad;
   float* sv = sk + 2 * kSpTok * kSpPad;
   float* sp = sv + 2 * kSpTok * kD;
+  // in this order: the tails' kernel starts at the trigger and relies on what
+  // came before this kernel being complete (decode_attn.cu, pdl_launch)
   pdl_wait();
   pdl_trigger();
   const int total = sp_total(p);
@@ -252,9 +254,11 @@ __global__ void __launch_bounds__(8 * RT / RPT, 2) shared_prefix_kernel(const SP
 // the steady part near the reading of the pages; 256 rows x 8 heads of up to
 // 131072 tokens (376 MB, 97 GFLOP), 125 us, 0.47 of the measured bf16 rate.
 // There the chain of a stream (S, softmax, O) sets the pace: a step of both
-// takes some 4000 clocks, of which the tensor core works 2048; its 8 MMAs
-// take 512 clocks alone and 600 to 1000 beside the softmax warps' loads of
-// tensor memory, whose exponentials are 2048 clocks of their unit a step.
+// takes some 4300 clocks (the difference between calls of 8 and 16 tiles a
+// CTA; 4900 to 5400 in long ones, under the power limit), of which the tensor
+// core works 2048; its 8 MMAs take 512 clocks alone and 600 to 1000 beside the
+// softmax warps' loads of tensor memory, whose exponentials are 2048 clocks of
+// their unit a step.
 // Warps: 0 key producer, 2 value producer (TMA), 1 MMA issuer, 4-7 and 8-11
 // softmax of stream 0 and 1 (one query row a thread); 3 has no role.  The
 // CTA's span may cover several segments (KV head, row group); between them
@@ -488,6 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;  // all 512 columns: column 0 on
+  // in this order, by every CTA, as in the CUDA-core form
   pdl_wait();
   pdl_trigger();
   TcWalk walk;
@@ -694,6 +699,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                   unpack_f2(fma_f2(pack_f2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), sl22, nm2));
               const float e0 = exp2_approx(t.x), e1 = exp2_approx(t.y);
               ps[k & 1] = add_f2(ps[k & 1], pack_f2(e0, e1));
+              // one rounding to 16 bits, what the product takes; l is of the
+              // unrounded ones (64 rows x 32768: 0.0023 from 64 bits, relative,
+              // where probabilities in 32 bits give 0.0017, the output's own)
               w[k] = Elem<T>::cvt2(e0, e1);
             }
             tmem_st16(cs + (uint32_t)(16 * c), w);

@@ -90,8 +90,9 @@ def set_wait_limits(limit_ns: int = 0, inject_stall: bool = False) -> None:
     """Limit of every device-side wait of the library's kernels (0: the
     defaults, 2 s per grid barrier and 1 s per mbarrier wait); with
     ``inject_stall`` the scoring kernels' grid barriers wait for an arrival
-    that never comes and the prefill attention loads no key tile, so the
-    limit runs out (tests of the timeout path)."""
+    that never comes, and the prefill attention and the 16-bit shared-prefix
+    attention load no key tile, so the limit runs out (tests of the timeout
+    path)."""
     check("hc_set_wait_limits", lib().hc_set_wait_limits(int(limit_ns), 1 if inject_stall else 0))
 
 
@@ -433,7 +434,7 @@ def flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, count
                         scale: float = 0.0, workspace: Workspace, err) -> torch.Tensor:
     """Decode attention over each row's listed 64-token blocks alone
     (hc_flash_decode_blocks): blocks [rows, n] int32 ascending, the first
-    counts[row] of them used."""
+    counts[row] of them used (one that is listed twice counts twice)."""
     out = paged().flash_decode_blocks(q, k_pool, v_pool, block_table, heads_len, blocks, counts, num_kv_heads, out,
                                       scale, workspace, err)
     if out.__class__ is int:

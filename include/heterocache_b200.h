@@ -301,7 +301,8 @@ int hc_rope_append(int dtype, int trig_dtype, int bsz, int num_heads, int num_kv
  * ascending, -1 behind the counts[row] listed ones.  q as in hc_flash_decode.
  *
  * hc_flash_decode_blocks: hc_flash_decode over the listed blocks of each row
- * alone (a row with none gives zeros); workspace as hc_flash_decode's.
+ * alone (a row with none gives zeros; a block that is listed twice counts
+ * twice); workspace as hc_flash_decode's.
  *
  * hc_flash_decode_sparse: the selection, then the attention over what it
  * lists, in one call.
