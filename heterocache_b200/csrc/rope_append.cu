@@ -423,11 +423,12 @@ __device__ __forceinline__ void ra_block(const RAParams& p, int r, int len, int 
 // One token a sequence: a row's token takes as many threads as a token of
 // ra_block, and a CTA a run of rows from r0 on (16 of a 16-bit cache), so
 // that few CTAs go through all rows for the allocation.  What is appended does
-// not hang on the allocation: it is loaded first.  With bounds a CTA has a
-// quarter of the rows where all CTAs are resident at once all the same: its
-// warps then read a row's earlier keys four at a time.  (Of 64 sequences of 8
-// rows, 2000 tokens or fewer each: 6.9 us without bounds, 8.8 with; of 512
-// sequences 27 and 32, and 53 with a quarter of the rows there too.)
+// not hang on the allocation: it is loaded first.  With bounds a CTA has an
+// eighth or a quarter of the rows where all CTAs are resident at once all the
+// same: its warps then read a row's earlier keys eight or four at a time.  (Of
+// 64 sequences of 8 rows: 6.9 us without bounds, 8.4 with an eighth of the rows
+// a CTA, 8.9 with a quarter; of 512 sequences 27 without, 32 with all rows, 53
+// with a quarter.)
 template <typename T>
 __host__ __device__ constexpr int ra_rows() {
   return kRaThreads / (2 * RaRow<T>::CH2);
@@ -438,13 +439,14 @@ __host__ __device__ constexpr int ra_row_warps(int rows) { return rows < kRaWarp
 // Least and greatest key, per channel, of the tokens before the new one in its
 // block, of the CTA's `rows` rows: row r0 + i's partials at s_mm[i * WPR ..][least,
 // greatest].  What ra_plan will find bad is not read.
-template <typename T, int WPR>
+template <typename T, int ROWS>
 __device__ __forceinline__ void ra_past(const RAParams& p, int r0, uint32_t* s_mm) {
+  constexpr int WPR = ra_row_warps(ROWS);
   constexpr int RW = kD * (int)sizeof(T) / 4, CH = RW / 4, TW = 32 / CH;  // a row's words, chunks; tokens of a warp
   constexpr int STEP = WPR * TW, U = 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll 1
-  for (int slot = warp; slot < p.rows * WPR; slot += kRaWarps) {
+  for (int slot = warp; slot < ROWS * WPR; slot += kRaWarps) {
     const int r = r0 + slot / WPR;
     int n = 0;
     const uint4* x = nullptr;
@@ -573,8 +575,9 @@ __global__ void __launch_bounds__(kRaThreads, kRaCtas) rope_append_kernel(const 
   const int u0 = (blockIdx.x % per_row) * p.run;
   RaToken<T, TT> tok;
   if (single && p.bounds) {
-    if (p.rows == ra_rows<T>()) ra_past<T, ra_row_warps(ra_rows<T>())>(p, r, s_mm);
-    else ra_past<T, ra_row_warps(ra_rows<T>() / 4)>(p, r, s_mm);
+    if (p.rows == ra_rows<T>() / 8) ra_past<T, ra_rows<T>() / 8>(p, r, s_mm);
+    else if (p.rows == ra_rows<T>() / 4) ra_past<T, ra_rows<T>() / 4>(p, r, s_mm);
+    else ra_past<T, ra_rows<T>()>(p, r, s_mm);
   }
   if (single) tok.load(p, r);
   const int base = *p.free_ptr;
@@ -611,7 +614,9 @@ static int ra_launch(RAParams& p, cudaStream_t st) {
   // still CTAs enough to fill the GPU
   p.run = R * p.units >= kRaRun * 8 * (int64_t)device_sms(current_device()) ? kRaRun : 1;
   p.rows = ra_rows<T>();
-  if (p.bounds && (R + p.rows / 4 - 1) / (p.rows / 4) <= kRaCtas * (int64_t)device_sms(current_device())) p.rows /= 4;
+  if (p.bounds)
+    for (const int part : {8, 4})
+      if (p.rows == ra_rows<T>() && R * part / p.rows < kRaCtas * (int64_t)device_sms(current_device())) p.rows /= part;
   const int64_t kv = p.T == 1 ? (R + p.rows - 1) / p.rows : R * ((p.units + p.run - 1) / p.run);
   const int64_t q = (((int64_t)p.B * p.T + TOK - 1) / TOK) * ((p.H + kRaHeads - 1) / kRaHeads);
   if (kv + q > 0x7fffffffLL) return HC_ERR_UNSUPPORTED;
