@@ -20,7 +20,7 @@
 // units of 32 tokens x up to 4 heads (the cosines and sines are loaded once
 // for the 4 heads).  Registers are kept to three CTAs an SM, two tokens (four
 // heads) of a thread in flight: 16 x 4096 tokens of 32 + 8 heads, 1.36 GB,
-// take 236 to 241 us (87 to 89% of the copy rate; with fp32 minima and one
+// take 236 to 245 us (86 to 89% of the copy rate; with fp32 minima and one
 // token in flight at 111 registers, 441 us).  Every key/value CTA derives the
 // page allocation for itself from the state the call found; the last of them to have read it (a
 // counter) writes the page table, the lengths and the free-list pointer, so

@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(8 * RT / RPT, 2) shared_prefix_kernel(const SP
 // streams hold 128 rows each and every tile serves both.
 // Measured: 64 rows x 8 heads of 6554 to 32768 tokens (96 MB), 26 to 31 us,
 // the steady part near the reading of the pages; 256 rows x 8 heads of up to
-// 131072 tokens (376 MB, 97 GFLOP), 125 us, 0.47 of the measured bf16 rate.
+// 131072 tokens (376 MB, 97 GFLOP), 123 us, 0.47 of the measured bf16 rate.
 // There the chain of a stream (S, softmax, O) sets the pace: a step of both
 // takes some 4300 clocks (the difference between calls of 8 and 16 tiles a
 // CTA; 4900 to 5400 in long ones, under the power limit), of which the tensor

@@ -83,9 +83,10 @@ def test_bounds_of_the_last_block_after_a_drop(cuda_device):
 
 
 @pytest.mark.parametrize("T", [1, 2])
-def test_many_rows(cuda_device, T):
-    """Four thousand rows and a few, each with bounds to follow."""
-    dev, dtype, bsz, KV = cuda_device, torch.bfloat16, 513, 8
+@pytest.mark.parametrize("dt,bsz", [("bf16", 140), ("bf16", 513), ("fp32", 70), ("fp32", 300)])
+def test_many_rows(cuda_device, T, dt, bsz):
+    """Up to four thousand rows and a few, each with bounds to follow."""
+    dev, dtype, KV = cuda_device, DT[dt], 8
     lens = rng_lens(bsz * KV, 0, 300, 3)
     c, lim = _start(lens, dtype, dev, T)
     used = sum((n + T + 255) // 256 - (n + 255) // 256 for n in lens)
